@@ -1,0 +1,705 @@
+// Attention over the 8-bit cache (q8_page.h): softmax(q k^T * scale) v with the keys and values that the pages hold,
+// for the rows of a step, each row seeing its sequence's tokens up to its own position (and no further back than the
+// window).  One library per head size.  Queries and results are bfloat16; scores, softmax statistics and sums float32.
+//
+// A byte becomes a bfloat16 number exactly (one conversion instruction for two, the keys' power of two among its
+// operands), so the products round nothing that the cache has not rounded already, except the probabilities: they are
+// rounded to bfloat16 (half a step: 2^-9 of each, in the sum over the keys less than the result's own rounding) for the
+// matrix instructions, as in the attention over a bfloat16 cache; the softmax's sum takes them unrounded.
+//
+//   attn_decode_kernel   steps that bring a few rows a sequence (a single token, drafted tokens): the pages of one
+//                        (sequence, kv head) are dealt to the waves of a block, and to several blocks where there are
+//                        too few; the columns of the matrix products are the group's heads of the sequence's rows.
+//   attn_combine_kernel  joins what several blocks left for a row.
+//   attn_prefill_kernel  prompts and pieces of prompts: 128 or 256 columns a block, pages turned to bfloat16 on their
+//                        way into LDS.
+//
+// computerex/dlgo attends over float32 rows of the cache, one query at a time (models/llm/forward.go:258-278).
+#include "q8_page.h"
+
+#ifndef HEAD_DIM
+#error "compile with -DHEAD_DIM=<head size>"
+#endif
+static_assert(HEAD_DIM % 16 == 0 && HEAD_DIM >= 16 && HEAD_DIM <= 256, "head sizes come in steps of 16, up to 256");
+
+#define HD HEAD_DIM
+#define PIECES (HD / 16)                    // 16-byte pieces of a key, and rows of 16 of the turned values
+#define KLOADS ((PIECES + 3) / 4)           // loads of a wave that bring 16 keys
+#define PART_ROW (HD + 4)                   // floats of a partial result: values, maximum, sum
+
+struct AttnQ8 {
+  const bf16_t* q;
+  bf16_t* out;
+  float* part;
+  const int32_t* cu_q;
+  const int32_t* start_pos;
+  const int32_t* slots;          // null: row i of page_table belongs to sequence i
+  const int32_t* page_table;
+  const uint8_t* cache;
+  long long page_stride;
+  int ldq, ldo, n_rows, n_seq, n_heads, n_kv, group, n_slots, max_pages, n_pages, window;
+  float scale_log2e;             // not negative; `flip` is its sign
+  uint32_t flip;
+  int splits, fill, waves;       // blocks that a sequence's pages may be dealt to: see splits_of
+};
+
+// How many of the launch's blocks a sequence with n pages uses: enough to fill the chip (`fill`, known at the launch),
+// but not more than leave each wave a page, and so many that a wave has at most 16 pages.
+__device__ __forceinline__ int splits_of(const AttnQ8& a, int n) {
+  const int by_wave = (n + a.waves - 1) / a.waves, by_16 = (n + 16 * a.waves - 1) / (16 * a.waves);
+  int s = a.fill < by_wave ? a.fill : by_wave;
+  if (s < by_16) s = by_16;
+  return s < 1 ? 1 : (s > a.splits ? a.splits : s);
+}
+
+// The rows and pages of a sequence, from numbers that live on the device; nothing outside the buffers whatever they are.
+struct Span {
+  int row0, rows, start, len, slot, first_page, n_pages;
+};
+__device__ __forceinline__ Span span_of(const AttnQ8& a, int seq) {
+  Span s;
+  s.row0 = a.cu_q[seq];
+  int row1 = a.cu_q[seq + 1];
+  s.start = a.start_pos[seq];
+  s.slot = a.slots ? a.slots[seq] : seq;
+  if (s.row0 < 0) s.row0 = 0;
+  if (row1 > a.n_rows) row1 = a.n_rows;
+  s.rows = row1 - s.row0;
+  if (s.start < 0 || s.slot < 0 || s.slot >= a.n_slots) s.rows = 0;
+  if (s.rows < 0) s.rows = 0;
+  s.len = s.start + s.rows;
+  const int lo = a.window > 0 && s.start - a.window + 1 > 0 ? s.start - a.window + 1 : 0;
+  s.first_page = lo / Q8_PAGE;
+  int last = (s.len - 1) / Q8_PAGE;
+  if (last >= a.max_pages) last = a.max_pages - 1;
+  s.n_pages = s.rows > 0 && last >= s.first_page ? last - s.first_page + 1 : 0;
+  return s;
+}
+
+__device__ __forceinline__ float fast_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
+
+typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2_t;
+template <bool HI> __device__ __forceinline__ uint32_t pair_of(uint32_t w, float scale) {
+  return __builtin_bit_cast(uint32_t, (bf16x2_t)__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)w, scale, HI));
+}
+// eight bytes -> eight bfloat16, times one power of two
+__device__ __forceinline__ bf16x8_t eight(uint32_t w0, uint32_t w1, float scale) {
+  uint4 u;
+  u.x = pair_of<false>(w0, scale);
+  u.y = pair_of<true>(w0, scale);
+  u.z = pair_of<false>(w1, scale);
+  u.w = pair_of<true>(w1, scale);
+  return __builtin_bit_cast(bf16x8_t, u);
+}
+// the first `n` of a word's four bytes (n may be anything)
+__device__ __forceinline__ uint32_t first_bytes(uint32_t w, int n) { return n >= 4 ? w : (n <= 0 ? 0u : w & ((1u << (8 * n)) - 1u)); }
+
+// ---------------------------------------------------------------------------------------------------------------------
+// Few rows a sequence.  grid (kv heads * chunks of columns, sequences, splits), WAVES waves.  A wave holds a whole page of
+// its head in registers: the keys of 16 tokens are KLOADS loads of 16 bytes a lane, the values of 16 elements one, all
+// of them consecutive in memory, and each is an operand of the matrix instructions as it lies once its bytes are
+// converted.  The next page's loads are on their way while this one is multiplied.  The scores come out with a lane
+// holding four neighbouring tokens of a column, which is the order of the values' bytes: no lane hands anything to
+// another but the two exchanges of the maximum.
+// Bound by memory: see the notes at the launcher.
+#define COLS(NC) (16 * (NC))
+#define NC_MOST (HD <= 64 ? 4 : (HD <= 128 ? 2 : 1))       // blocks of 16 columns whose sums a wave's registers hold beside two pages
+
+struct PageRegs {
+  uint4 k[4][KLOADS];
+  uint4 v[PIECES];
+  uint32_t ks;          // the scales of the keys of tokens 16 t + (lane % 16), t = 0 .. 3
+  uint4 vs;             // the scales of the values of tokens 16 t + 4 (lane / 16) + r
+};
+
+static __device__ __forceinline__ void fetch_page(PageRegs& p, const uint8_t* head, int lane) {
+#pragma unroll
+  for (int t = 0; t < 4; ++t)
+#pragma unroll
+    for (int j = 0; j < KLOADS; ++j) {
+      // lanes whose piece lies beyond the head read the page's first bytes instead and count as zero below
+      const bool ok = PIECES % 4 == 0 || 4 * j + (lane >> 4) < PIECES;
+      p.k[t][j] = *(const uint4*)(head + (ok ? (t * PIECES + 4 * j) * 256 + lane * 16 : 0));
+    }
+#pragma unroll
+  for (int c = 0; c < PIECES; ++c) p.v[c] = *(const uint4*)(head + Q8_PAGE * HD + c * 1024 + lane * 16);
+  p.ks = *(const uint32_t*)(head + 2 * Q8_PAGE * HD + (lane & 15) * 4);
+  p.vs = *(const uint4*)(head + 2 * Q8_PAGE * HD + 64 + (lane >> 4) * 16);
+}
+
+template <int NC, int WAVES>
+__global__ __launch_bounds__(WAVES* WAVE) void attn_decode_kernel(AttnQ8 a) {
+  constexpr int QK = 2 * KLOADS;                         // matrix instructions for the scores of 16 tokens
+  extern __shared__ __attribute__((aligned(16))) float merge[];    // [WAVES][COLS][HD], then [WAVES][COLS] maxima and sums
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, n = lane & 15;
+  const int kvh = blockIdx.x % a.n_kv, chunk = blockIdx.x / a.n_kv, seq = blockIdx.y, split = blockIdx.z;
+  const Span s = span_of(a, seq);
+  const int cols = s.rows * a.group, col0 = chunk * COLS(NC);
+  if (col0 >= cols) return;
+  const int used = splits_of(a, s.n_pages);
+  if (split >= used) return;
+  const int per = (s.n_pages + used - 1) / used;
+  const int pg0 = s.first_page + split * per;
+  const int pg1 = pg0 + per < s.first_page + s.n_pages ? pg0 + per : s.first_page + s.n_pages;      // pages [pg0, pg1)
+
+  // this lane's column of each of the NC blocks of 16: a row of the step and a head
+  bf16x8_t qf[NC][QK];
+  int pos[NC], lo[NC];
+#pragma unroll
+  for (int b = 0; b < NC; ++b) {
+    const int col = col0 + 16 * b + n;
+    const bool real = col < cols;
+    const int row = real ? col / a.group : 0, hig = real ? col % a.group : 0;
+    pos[b] = real ? s.start + row : -1;
+    lo[b] = a.window > 0 && pos[b] - a.window + 1 > 0 ? pos[b] - a.window + 1 : 0;
+    const bf16_t* src = a.q + (size_t)(s.row0 + row) * a.ldq + (size_t)(kvh * a.group + hig) * HD;
+#pragma unroll
+    for (int j = 0; j < KLOADS; ++j)
+#pragma unroll
+      for (int m = 0; m < 2; ++m) {
+        const int piece = 4 * j + g;
+        uint4 u = *(const uint4*)(src + (piece < PIECES ? piece * 16 + m * 8 : 0));
+        if (!real || piece >= PIECES) u = make_uint4(0, 0, 0, 0);
+        else u = make_uint4(u.x ^ a.flip, u.y ^ a.flip, u.z ^ a.flip, u.w ^ a.flip);
+        qf[b][2 * j + m] = __builtin_bit_cast(bf16x8_t, u);
+      }
+  }
+  f32x4_t o[NC][PIECES];
+  float m[NC], l[NC];
+#pragma unroll
+  for (int b = 0; b < NC; ++b) {
+    m[b] = -INFINITY;
+    l[b] = 0.f;
+#pragma unroll
+    for (int c = 0; c < PIECES; ++c) o[b][c] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
+  }
+
+  const int32_t* table = a.page_table + (size_t)s.slot * a.max_pages;
+  const size_t head = (size_t)kvh * q8_head_bytes(HD);
+  // the numbers of this wave's pages, 64 at a time, one a lane
+  int ids = 0, ids_from = -1;
+  auto page_id = [&](int k) {                          // the wave's k-th page
+    const int from = k & ~63;
+    if (from != ids_from) {
+      const int pg = pg0 + wave + (from + lane) * WAVES;
+      ids = table[pg < pg1 ? pg : pg0];
+      ids_from = from;
+    }
+    return __builtin_amdgcn_readlane(ids, k & 63);
+  };
+  auto fetch = [&](PageRegs& p, int id) {
+    const bool ok = id >= 0 && id < a.n_pages;         // a hole reads page 0 and counts nothing
+    fetch_page(p, (const uint8_t*)uniform_ptr(a.cache + (size_t)(ok ? id : 0) * a.page_stride + head), lane);
+    return ok;
+  };
+
+  const int turns = pg1 - pg0 > wave ? (pg1 - pg0 - wave + WAVES - 1) / WAVES : 0;
+  PageRegs cur;
+  bool cur_ok = false;
+  if (turns > 0) cur_ok = fetch(cur, page_id(0));
+  for (int k = 0; k < turns; ++k) {
+    PageRegs next;
+    bool next_ok = false;
+    if (k + 1 < turns) next_ok = fetch(next, page_id(k + 1));
+    if (cur_ok) {
+      const int key0 = (pg0 + wave + k * WAVES) * Q8_PAGE;
+      f32x4_t sc[NC][4];
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        const float ksc = q8_scale((cur.ks >> (8 * t)) & 255u);
+#pragma unroll
+        for (int b = 0; b < NC; ++b) sc[b][t] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int j = 0; j < KLOADS; ++j) {
+          uint4 u = cur.k[t][j];
+          if (PIECES % 4 != 0 && 4 * j + g >= PIECES) u = make_uint4(0, 0, 0, 0);
+          const bf16x8_t k0 = eight(u.x, u.y, ksc), k1 = eight(u.z, u.w, ksc);
+#pragma unroll
+          for (int b = 0; b < NC; ++b) {
+            sc[b][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k0, qf[b][2 * j], sc[b][t], 0, 0, 0);
+            sc[b][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k1, qf[b][2 * j + 1], sc[b][t], 0, 0, 0);
+          }
+        }
+      }
+      // element r of sc[b][t] is key  key0 + 16 t + 4 g + r  of column n
+      if (key0 + Q8_PAGE > s.len) {                    // tokens that the sequence does not hold: their bytes are anybody's
+#pragma unroll
+        for (int c = 0; c < PIECES; ++c) {
+          const int k0 = s.len - key0 - 4 * g;
+          cur.v[c] = make_uint4(first_bytes(cur.v[c].x, k0), first_bytes(cur.v[c].y, k0 - 16), first_bytes(cur.v[c].z, k0 - 32),
+                                first_bytes(cur.v[c].w, k0 - 48));
+        }
+      }
+      bf16x8_t pf[NC][2];
+#pragma unroll
+      for (int b = 0; b < NC; ++b) {
+        const bool mask = key0 + Q8_PAGE - 1 > s.start || a.window > 0;
+        if (mask) {
+#pragma unroll
+          for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              const int key = key0 + 16 * t + 4 * g + r;
+              sc[b][t][r] = key <= pos[b] && key >= lo[b] ? sc[b][t][r] : -INFINITY;
+            }
+        }
+        float mx = -INFINITY;
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) mx = fmaxf(mx, sc[b][t][r]);
+        mx = fmaxf(mx, __shfl_xor(mx, 16, WAVE));
+        mx = fmaxf(mx, __shfl_xor(mx, 32, WAVE));
+        const float m_new = fmaxf(m[b], mx);
+        const float off = m_new == -INFINITY ? 0.f : -m_new * a.scale_log2e;
+        if (__any(m_new != m[b])) {
+          const float keep = m[b] == -INFINITY ? 0.f : fast_exp2(fmaf(m[b], a.scale_log2e, off));
+          l[b] *= keep;
+#pragma unroll
+          for (int c = 0; c < PIECES; ++c) o[b][c] *= keep;
+          m[b] = m_new;
+        }
+        float p[16];
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const float e = mask && sc[b][t][r] == -INFINITY ? 0.f : fast_exp2(fmaf(sc[b][t][r], a.scale_log2e, off));
+            l[b] += e;
+            // the value's power of two goes into the probability: exact, and its own bits are at hand
+            const uint32_t w = t == 0 ? cur.vs.x : (t == 1 ? cur.vs.y : (t == 2 ? cur.vs.z : cur.vs.w));
+            const float f = q8_scale((w >> (8 * r)) & 255u);
+            p[4 * t + r] = mask && sc[b][t][r] == -INFINITY ? 0.f : e * f;
+          }
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) pf[b][h][e] = (__bf16)p[8 * h + e];
+      }
+#pragma unroll
+      for (int c = 0; c < PIECES; ++c) {
+        const bf16x8_t v0 = eight(cur.v[c].x, cur.v[c].y, 1.f), v1 = eight(cur.v[c].z, cur.v[c].w, 1.f);
+#pragma unroll
+        for (int b = 0; b < NC; ++b) {
+          o[b][c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v0, pf[b][0], o[b][c], 0, 0, 0);
+          o[b][c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v1, pf[b][1], o[b][c], 0, 0, 0);
+        }
+      }
+    }
+    cur = next;
+    cur_ok = next_ok;
+  }
+
+  // the waves' results meet in LDS: element 4 g + r of o[b][c] is element 16 c + 4 g + r of the head, of column n
+  float* mw = merge + WAVES * COLS(NC) * HD;
+  float* lw = mw + WAVES * COLS(NC);
+#pragma unroll
+  for (int b = 0; b < NC; ++b) {
+    l[b] += __shfl_xor(l[b], 16, WAVE);
+    l[b] += __shfl_xor(l[b], 32, WAVE);
+    const int col = 16 * b + n;
+    if (g == 0) {
+      mw[wave * COLS(NC) + col] = m[b];
+      lw[wave * COLS(NC) + col] = l[b];
+    }
+    // 16 columns a row of the head apart would all fall on the same banks: pieces of 4 floats are moved by the column
+#pragma unroll
+    for (int c = 0; c < PIECES; ++c)
+      *(f32x4_t*)(merge + (size_t)(wave * COLS(NC) + col) * HD + (((4 * c + g) + col) % (HD / 4)) * 4) = o[b][c];
+  }
+  __syncthreads();
+  const int left = cols - col0 < COLS(NC) ? cols - col0 : COLS(NC);
+  for (int i = threadIdx.x; i < left * (HD / 4); i += WAVES * WAVE) {
+    const int col = i / (HD / 4), e4 = i % (HD / 4);
+    float M = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) M = fmaxf(M, mw[w * COLS(NC) + col]);
+    float L = 0.f;
+    f32x4_t acc = (f32x4_t){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) {
+      const float mm = mw[w * COLS(NC) + col], ll = lw[w * COLS(NC) + col];
+      const float f = mm == -INFINITY ? 0.f : fast_exp2((mm - M) * a.scale_log2e);
+      const f32x4_t v = *(const f32x4_t*)(merge + (size_t)(w * COLS(NC) + col) * HD + ((e4 + col) % (HD / 4)) * 4);
+      // a wave whose scores are all NaN has no maximum but a sum that is NaN: it must reach the row
+      L += mm == -INFINITY ? ll : f * ll;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[e] += mm == -INFINITY ? v[e] : f * v[e];
+    }
+    const int row = s.row0 + (col0 + col) / a.group, h = kvh * a.group + (col0 + col) % a.group;
+    if (used == 1) {
+      const float inv = L == 0.f ? 0.f : 1.0f / L;       // a row that sees no token at all (its pages are missing): zeros
+      Elem<bf16_t>::store4(a.out + (size_t)row * a.ldo + (size_t)h * HD + e4 * 4, acc[0] * inv, acc[1] * inv, acc[2] * inv, acc[3] * inv);
+    } else {
+      float* dst = a.part + ((size_t)((size_t)row * a.n_heads + h) * a.splits + split) * PART_ROW;
+      *(f32x4_t*)(dst + e4 * 4) = acc;
+      if (e4 == 0) {
+        dst[HD] = M;
+        dst[HD + 1] = L;
+      }
+    }
+  }
+}
+
+// One wave for each row and head that several blocks left results of.  grid (most rows a sequence * heads, sequences).
+#include "exact_begin.h"
+__global__ __launch_bounds__(WAVE) void attn_combine_kernel(AttnQ8 a) {
+  const int lane = threadIdx.x, h = blockIdx.x % a.n_heads, r = blockIdx.x / a.n_heads;
+  const Span s = span_of(a, blockIdx.y);
+  if (r >= s.rows) return;
+  const int used = splits_of(a, s.n_pages);
+  if (used == 1) return;                               // written by its block
+  const int row = s.row0 + r;
+  const float* base = a.part + (size_t)((size_t)row * a.n_heads + h) * a.splits * PART_ROW;
+  const int per = (s.n_pages + used - 1) / used;
+  const int filled = (s.n_pages + per - 1) / per;      // blocks that were given pages
+  float M = -INFINITY;
+  for (int i = 0; i < filled; ++i) M = fmaxf(M, base[(size_t)i * PART_ROW + HD]);
+  constexpr int NE = (HD + WAVE - 1) / WAVE;
+  float L = 0.f, acc[NE];
+#pragma unroll
+  for (int e = 0; e < NE; ++e) acc[e] = 0.f;
+  for (int i = 0; i < filled; ++i) {
+    const float* p = base + (size_t)i * PART_ROW;
+    const float mm = p[HD], f = mm == -INFINITY ? 1.f : exp2f((mm - M) * a.scale_log2e);     // -inf: zeros, or NaN
+    L = fmaf(f, p[HD + 1], L);
+#pragma unroll
+    for (int e = 0; e < NE; ++e) acc[e] = fmaf(f, p[e * WAVE + lane < HD ? e * WAVE + lane : 0], acc[e]);
+  }
+  const float inv = L == 0.f ? 0.f : 1.0f / L;
+#pragma unroll
+  for (int e = 0; e < NE; ++e)
+    if (e * WAVE + lane < HD) a.out[(size_t)row * a.ldo + (size_t)h * HD + e * WAVE + lane] = f32_to_bf16(acc[e] * inv);
+}
+#include "exact_end.h"
+
+// ---------------------------------------------------------------------------------------------------------------------
+// Prompts.  A block of four waves takes 128 * CW columns (tokens x the heads of a group) of a sequence and walks the pages.
+// A page's bytes are turned to bfloat16 once for all its columns on the way into LDS (keys and values with their powers
+// of two: exact), the next page's bytes are on their way meanwhile, and the two places in LDS are used in turn, so that
+// a page costs one barrier.  Scores are kept transposed (keys x columns): a lane owns a column.
+#define PF_WAVES 4
+#define DT ((HD + 31) / 32)                 // tiles of 32 elements of the result
+#define KS (HD / 16)                        // steps of 16 along the head
+#define LDS_K (Q8_PAGE * HD * 2)            // [element / 8][token][8 elements]
+#define LDS_V (4 * 2 * DT * 32 * 16)        // [t][h][element][8 tokens: 16 t + 8 a + 4 h + r]
+#define NPC ((4 * HD + 255) / 256)          // 16-byte pieces of a page's keys (of its values) a thread brings
+
+template <int CW>
+__global__ __launch_bounds__(PF_WAVES* WAVE) void attn_prefill_kernel(AttnQ8 a, int tokens, int n_tiles) {
+  extern __shared__ __attribute__((aligned(16))) char pf_lds[];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5;
+  // Late tiles see more keys than early ones: tiles are dealt longest first, 256 blocks (one a compute unit) at a time,
+  // every other time in reverse, so that the blocks that share a unit add up to about the same number of pages.
+  const int total = gridDim.x, width = a.n_seq * a.n_kv;
+  const int turn = blockIdx.x >> 8, in_turn = total - (turn << 8) < 256 ? total - (turn << 8) : 256;
+  const int place = turn & 1 ? (turn << 8) + in_turn - 1 - (blockIdx.x & 255) : blockIdx.x;
+  const int tile = n_tiles - 1 - place / width, kvh = place % a.n_kv, seq = place % width / a.n_kv;
+  const Span s = span_of(a, seq);
+  const int t0 = tile * tokens;
+  if (t0 >= s.rows) return;
+  const int t1 = t0 + tokens < s.rows ? t0 + tokens : s.rows;        // the block's rows of the sequence
+  const int lo_b = a.window > 0 && s.start + t0 - a.window + 1 > 0 ? s.start + t0 - a.window + 1 : 0;
+  const int pg_lo = lo_b / Q8_PAGE;
+  int pg_hi = (s.start + t1 - 1) / Q8_PAGE;
+  if (pg_hi >= a.max_pages) pg_hi = a.max_pages - 1;
+
+  int pos[CW], lo[CW], trow[CW], hig[CW];
+  bf16x8_t qf[CW][KS];
+#pragma unroll
+  for (int b = 0; b < CW; ++b) {
+    const int col = (wave * CW + b) * 32 + (lane & 31);
+    const int t = t0 + col / a.group;
+    const bool real = t < t1 && col < tokens * a.group;
+    trow[b] = real ? t : -1;
+    hig[b] = col % a.group;
+    pos[b] = real ? s.start + t : -1;
+    lo[b] = a.window > 0 && pos[b] - a.window + 1 > 0 ? pos[b] - a.window + 1 : 0;
+    const bf16_t* src = a.q + (size_t)(s.row0 + (real ? t : t0)) * a.ldq + (size_t)(kvh * a.group + hig[b]) * HD;
+#pragma unroll
+    for (int k = 0; k < KS; ++k) {
+      uint4 u = *(const uint4*)(src + k * 16 + half * 8);
+      u = real ? make_uint4(u.x ^ a.flip, u.y ^ a.flip, u.z ^ a.flip, u.w ^ a.flip) : make_uint4(0, 0, 0, 0);
+      qf[b][k] = __builtin_bit_cast(bf16x8_t, u);
+    }
+  }
+  // the positions that the wave's columns span
+  const int wc0 = wave * CW * 32;
+  const int wt0 = t0 + wc0 / a.group;
+  int wt1 = t0 + (wc0 + CW * 32 - 1) / a.group;
+  wt1 = wt1 < t1 - 1 ? wt1 : t1 - 1;
+  const bool wave_real = wt0 < t1 && wc0 < tokens * a.group;
+  const int w_min = s.start + wt0, w_max = s.start + wt1;
+  const int w_lo_min = a.window > 0 && w_min - a.window + 1 > 0 ? w_min - a.window + 1 : 0;
+  const int w_lo_max = a.window > 0 && w_max - a.window + 1 > 0 ? w_max - a.window + 1 : 0;
+
+  f32x16_t o[CW][DT];
+  float m[CW], l[CW];
+#pragma unroll
+  for (int b = 0; b < CW; ++b) {
+    m[b] = -INFINITY;
+    l[b] = 0.f;
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+      for (int v = 0; v < 16; ++v) o[b][d][v] = 0.f;
+  }
+
+  const int32_t* table = a.page_table + (size_t)s.slot * a.max_pages;
+  const size_t head = (size_t)kvh * q8_head_bytes(HD);
+  uint4 rk[NPC], rv[NPC], rvs[NPC];
+  uint32_t rks[NPC];
+  bool r_ok = false;
+  auto fetch = [&](int pg) {
+    const int id = table[pg];
+    r_ok = id >= 0 && id < a.n_pages;
+    const uint8_t* p = a.cache + (size_t)(r_ok ? id : 0) * a.page_stride + head;
+#pragma unroll
+    for (int i = 0; i < NPC; ++i) {
+      int c = tid + i * 256;
+      if (NPC * 256 != 4 * HD && c >= 4 * HD) c = 0;
+      rk[i] = *(const uint4*)(p + c * 16);
+      rv[i] = *(const uint4*)(p + Q8_PAGE * HD + c * 16);
+      rks[i] = p[2 * Q8_PAGE * HD + (c & 15) * 4 + (c >> 4) / PIECES];
+      rvs[i] = *(const uint4*)(p + 2 * Q8_PAGE * HD + 64 + ((c >> 4) & 3) * 16);
+    }
+  };
+  auto stage = [&](char* lds, int key0) {
+    const bool tail = key0 + Q8_PAGE > s.len;
+#pragma unroll
+    for (int i = 0; i < NPC; ++i) {
+      const int c = tid + i * 256;
+      if (NPC * 256 != 4 * HD && c >= 4 * HD) break;
+      // keys: piece p of token 16 t + (c % 16)
+      const int tp = c >> 4, t = tp / PIECES, p = tp % PIECES, token = 16 * t + (c & 15);
+      const float ksc = q8_scale(rks[i]);
+      *(bf16x8_t*)(lds + ((2 * p) * Q8_PAGE + token) * 16) = eight(rk[i].x, rk[i].y, ksc);
+      *(bf16x8_t*)(lds + ((2 * p + 1) * Q8_PAGE + token) * 16) = eight(rk[i].z, rk[i].w, ksc);
+      // values: element d, tokens 16 t + 4 g + r
+      const int g = (c >> 4) & 3, d = (c >> 6) * 16 + (c & 15);
+      char* dst = lds + LDS_K + ((g & 1) * (DT * 32) + d) * 16 + (g >> 1) * 8;
+#pragma unroll
+      for (int t4 = 0; t4 < 4; ++t4) {
+        uint32_t w = t4 == 0 ? rv[i].x : (t4 == 1 ? rv[i].y : (t4 == 2 ? rv[i].z : rv[i].w));
+        uint32_t sc = t4 == 0 ? rvs[i].x : (t4 == 1 ? rvs[i].y : (t4 == 2 ? rvs[i].z : rvs[i].w));
+        if (tail) {          // tokens that the sequence does not hold: zeros, with a power that leaves them zeros
+          const int left = s.len - key0 - 16 * t4 - 4 * g;
+          w = first_bytes(w, left);
+          sc = first_bytes(sc, left);
+        }
+        // two of a word's four have one power each: convert the pair with either and keep the half that is meant
+        const uint32_t a0 = pair_of<false>(w, q8_scale(sc & 255u)), a1 = pair_of<false>(w, q8_scale((sc >> 8) & 255u));
+        const uint32_t b0 = pair_of<true>(w, q8_scale((sc >> 16) & 255u)), b1 = pair_of<true>(w, q8_scale(sc >> 24));
+        *(uint2*)(dst + t4 * (2 * DT * 32 * 16)) = make_uint2((a0 & 0xffffu) | (a1 & 0xffff0000u), (b0 & 0xffffu) | (b1 & 0xffff0000u));
+      }
+    }
+  };
+
+  constexpr int LDS_PAGE = LDS_K + LDS_V;
+  bool ok = false;
+  if (pg_lo <= pg_hi) {
+    fetch(pg_lo);
+    stage(pf_lds, pg_lo * Q8_PAGE);
+    ok = r_ok;
+  }
+  __syncthreads();
+  for (int pg = pg_lo; pg <= pg_hi; ++pg) {
+    if (pg < pg_hi) fetch(pg + 1);
+    const int key0 = pg * Q8_PAGE;
+    const char* lds = pf_lds + ((pg - pg_lo) & 1) * LDS_PAGE;
+    if (ok && wave_real && key0 <= w_max && key0 + Q8_PAGE - 1 >= w_lo_min) {
+      f32x16_t sc[CW][2];
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt) {
+#pragma unroll
+        for (int b = 0; b < CW; ++b)
+#pragma unroll
+          for (int v = 0; v < 16; ++v) sc[b][kt][v] = 0.f;
+#pragma unroll
+        for (int k = 0; k < KS; ++k) {
+          const bf16x8_t kf = *(const bf16x8_t*)(lds + ((2 * k + half) * Q8_PAGE + kt * 32 + (lane & 31)) * 16);
+#pragma unroll
+          for (int b = 0; b < CW; ++b) sc[b][kt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, qf[b][k], sc[b][kt], 0, 0, 0);
+        }
+      }
+      // element v of sc[b][kt] is key  key0 + 32 kt + 8 (v / 4) + 4 half + v % 4  of the lane's column
+      const bool mask = key0 + Q8_PAGE - 1 > w_min || key0 < w_lo_max;
+      bf16x8_t pf[CW][4];
+#pragma unroll
+      for (int b = 0; b < CW; ++b) {
+        if (mask) {
+#pragma unroll
+          for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+            for (int v = 0; v < 16; ++v) {
+              const int key = key0 + kt * 32 + 8 * (v >> 2) + 4 * half + (v & 3);
+              sc[b][kt][v] = key <= pos[b] && key >= lo[b] ? sc[b][kt][v] : -INFINITY;
+            }
+        }
+        float mx = -INFINITY;
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+          for (int v = 0; v < 16; ++v) mx = fmaxf(mx, sc[b][kt][v]);
+        mx = fmaxf(mx, __shfl_xor(mx, 32, WAVE));
+        const float m_new = fmaxf(m[b], mx);
+        const float off = m_new == -INFINITY ? 0.f : -m_new * a.scale_log2e;
+        if (__any(m_new != m[b])) {
+          const float keep = m[b] == -INFINITY ? 0.f : fast_exp2(fmaf(m[b], a.scale_log2e, off));
+          l[b] *= keep;
+#pragma unroll
+          for (int d = 0; d < DT; ++d)
+#pragma unroll
+            for (int v = 0; v < 16; ++v) o[b][d][v] *= keep;
+          m[b] = m_new;
+        }
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+          for (int v = 0; v < 16; ++v) {
+            const float e = fast_exp2(fmaf(sc[b][kt][v], a.scale_log2e, off));
+            l[b] += e;
+            pf[b][2 * kt + (v >> 3)][v & 7] = (__bf16)e;
+          }
+      }
+      // element e of pf[b][t] is key  16 t + 8 (e / 4) + 4 half + e % 4: the values lie in LDS in that order
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int d = 0; d < DT; ++d) {
+          const bf16x8_t vf = *(const bf16x8_t*)(lds + LDS_K + ((t * 2 + half) * (DT * 32) + d * 32 + (lane & 31)) * 16);
+#pragma unroll
+          for (int b = 0; b < CW; ++b) o[b][d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, pf[b][t], o[b][d], 0, 0, 0);
+        }
+    }
+    if (pg < pg_hi) {
+      stage(pf_lds + ((pg - pg_lo + 1) & 1) * LDS_PAGE, key0 + Q8_PAGE);
+      ok = r_ok;
+    }
+    __syncthreads();
+  }
+#pragma unroll
+  for (int b = 0; b < CW; ++b) {
+    l[b] += __shfl_xor(l[b], 32, WAVE);
+    if (trow[b] < 0) continue;
+    const float inv = l[b] == 0.f ? 0.f : 1.0f / l[b];
+    bf16_t* dst = a.out + (size_t)(s.row0 + trow[b]) * a.ldo + (size_t)(kvh * a.group + hig[b]) * HD;
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+      for (int qd = 0; qd < 4; ++qd) {
+        const int e = d * 32 + 8 * qd + 4 * half;
+        if (e < HD) Elem<bf16_t>::store4(dst + e, o[b][d][4 * qd] * inv, o[b][d][4 * qd + 1] * inv, o[b][d][4 * qd + 2] * inv, o[b][d][4 * qd + 3] * inv);
+      }
+  }
+}
+
+// ---------------------------------------------------------------------------------------------------------------------
+// What a launch looks like, from sizes that the host knows.  max_q_len and max_kv_len bound the sequences' rows and
+// lengths (a recorded launch passes the context's).
+struct Plan {
+  int tiled, nc, waves, chunks, splits, fill;
+};
+static Plan plan_of(int n_seq, int n_heads, int n_kv, int max_q_len, int max_kv_len, int window) {
+  Plan p = {};
+  const int group = n_heads / n_kv;
+  const long long cols = (long long)max_q_len * group;
+  p.tiled = cols > 64;
+  if (p.tiled) return p;
+  p.nc = cols <= 16 ? 1 : (cols <= 32 ? 2 : 4);
+  if (p.nc > NC_MOST) p.nc = NC_MOST;
+  p.chunks = (int)((cols + 16 * p.nc - 1) / (16 * p.nc));
+  // the waves of a block must find room in LDS for their results: columns x (head + 2) floats each
+  p.waves = HD <= 64 ? 8 : 4;
+  while (p.waves > 1 && p.waves * 16 * p.nc * (HD + 2) * 4 > 128 * 1024) p.waves /= 2;
+  int pages = (max_kv_len + Q8_PAGE - 1) / Q8_PAGE;
+  if (window > 0) {
+    const int seen = (window + max_q_len + Q8_PAGE - 2) / Q8_PAGE + 1;
+    if (seen < pages) pages = seen;
+  }
+  const long long pairs = (long long)n_seq * n_kv * p.chunks;
+  const int target = 512;
+  p.fill = pairs >= target ? 1 : (int)((target + pairs - 1) / pairs);
+  const int by_wave = (pages + p.waves - 1) / p.waves, by_16 = (pages + 16 * p.waves - 1) / (16 * p.waves);
+  p.splits = p.fill < by_wave ? p.fill : by_wave;
+  if (p.splits < by_16) p.splits = by_16;
+  if (p.splits < 1) p.splits = 1;
+  return p;
+}
+
+extern "C" int dlgo_attention_q8_head_dim() { return HD; }
+
+// floats of scratch that a launch needs (0: none)
+extern "C" long long dlgo_attention_q8_scratch(int n_rows, int n_seq, int n_heads, int n_kv, int max_q_len, int max_kv_len, int window) {
+  if (n_rows <= 0 || n_seq <= 0 || n_kv <= 0 || n_heads < n_kv || max_q_len <= 0 || max_kv_len <= 0) return 0;
+  const Plan p = plan_of(n_seq, n_heads, n_kv, max_q_len, max_kv_len, window);
+  return p.tiled || p.splits <= 1 ? 0 : (long long)n_rows * n_heads * p.splits * PART_ROW;
+}
+
+template <int NC, int WAVES>
+static hipError_t launch_decode(const AttnQ8& a, dim3 grid, hipStream_t stream) {
+  const int lds = WAVES * 16 * NC * (HD + 2) * 4;
+  hipError_t e = hipSuccess;
+  if (lds > 64 * 1024) e = hipFuncSetAttribute((const void*)attn_decode_kernel<NC, WAVES>, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+  if (e == hipSuccess) hipLaunchKernelGGL((attn_decode_kernel<NC, WAVES>), grid, dim3(WAVES * WAVE), lds, stream, a);
+  return e;
+}
+template <int NC>
+static hipError_t launch_decode_waves(const AttnQ8& a, dim3 grid, hipStream_t stream) {
+  switch (a.waves) {
+    case 8: if constexpr (8 * 16 * NC * (HD + 2) * 4 <= 128 * 1024) return launch_decode<NC, 8>(a, grid, stream); else return hipErrorInvalidValue;
+    case 4: if constexpr (4 * 16 * NC * (HD + 2) * 4 <= 128 * 1024) return launch_decode<NC, 4>(a, grid, stream); else return hipErrorInvalidValue;
+    case 2: if constexpr (HD > 64) return launch_decode<NC, 2>(a, grid, stream); else return hipErrorInvalidValue;
+    case 1: if constexpr (HD > 128) return launch_decode<NC, 1>(a, grid, stream); else return hipErrorInvalidValue;
+  }
+  return hipErrorInvalidValue;
+}
+
+extern "C" const char* dlgo_attention_q8(const void* q, int ldq, void* out, int ldo, int n_rows, int n_seq, int n_heads, int n_kv, int head_dim,
+                                         const int32_t* cu_q, const int32_t* start_pos, const int32_t* slots, const int32_t* page_table,
+                                         int n_slots, int max_pages, const void* cache, long long page_stride, int n_pages, int max_q_len,
+                                         int max_kv_len, int window, float scale, float* part, long long part_elems, hipStream_t stream) {
+  DLGO_REQUIRE(head_dim == HD, "attention_q8: this library is built for a head size of %d, not %d", HD, head_dim);
+  DLGO_REQUIRE(n_rows >= 0 && n_seq >= 0 && n_kv > 0 && n_heads >= n_kv && n_heads % n_kv == 0, "attention_q8: %d heads over %d kv heads", n_heads, n_kv);
+  DLGO_REQUIRE(n_heads / n_kv <= 128, "attention_q8: at most 128 heads share a kv head, not %d", n_heads / n_kv);
+  if (n_rows == 0 || n_seq == 0 || max_q_len == 0) return nullptr;
+  DLGO_REQUIRE(max_q_len > 0 && max_kv_len > 0 && n_slots > 0 && max_pages > 0 && n_pages > 0, "attention_q8: bad bounds");
+  DLGO_REQUIRE(scale - scale == 0.f && scale != 0.f, "attention_q8: the scale must be finite and not zero");
+  DLGO_REQUIRE(((uintptr_t)q & 15) == 0 && ldq % 8 == 0 && ldq >= n_heads * HD && ((uintptr_t)out & 7) == 0 && ldo % 4 == 0 && ldo >= n_heads * HD,
+               "attention_q8: query rows must be 16-byte aligned, result rows 8-byte aligned (strides %d and %d)", ldq, ldo);
+  DLGO_REQUIRE(((uintptr_t)cache & 15) == 0 && page_stride % 16 == 0 && page_stride >= n_kv * q8_head_bytes(HD),
+               "attention_q8: pages %lld bytes apart (16-byte aligned pages of at least %lld bytes are needed)", page_stride, n_kv * q8_head_bytes(HD));
+  DLGO_REQUIRE(n_seq <= 65535, "attention_q8: at most 65535 sequences");
+  if (max_kv_len > max_pages * (long long)Q8_PAGE) max_kv_len = max_pages * Q8_PAGE;
+  const Plan p = plan_of(n_seq, n_heads, n_kv, max_q_len, max_kv_len, window);
+  AttnQ8 a = {(const bf16_t*)q, (bf16_t*)out, part, cu_q, start_pos, slots, page_table, (const uint8_t*)cache, page_stride, ldq, ldo, n_rows, n_seq,
+              n_heads, n_kv, n_heads / n_kv, n_slots, max_pages, n_pages, window > 0 ? window : 0,
+              (scale < 0 ? -scale : scale) * 1.44269504088896341f, scale < 0 ? 0x80008000u : 0u, p.splits, p.fill, p.waves};
+  hipError_t e = hipSuccess;
+  if (p.tiled) {
+    constexpr int CW = HD <= 64 ? 2 : 1;
+    const int columns = PF_WAVES * 32 * CW, tokens = columns / a.group;
+    const int n_tiles = (max_q_len + tokens - 1) / tokens;
+    const long long blocks = (long long)n_tiles * n_seq * n_kv;
+    DLGO_REQUIRE(blocks < (1ll << 31), "attention_q8: too many rows at once");
+    const int lds = 2 * (LDS_K + LDS_V);
+    if (lds > 64 * 1024) e = hipFuncSetAttribute((const void*)attn_prefill_kernel<CW>, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+    if (e == hipSuccess) hipLaunchKernelGGL(attn_prefill_kernel<CW>, dim3((unsigned)blocks), dim3(PF_WAVES * WAVE), lds, stream, a, tokens, n_tiles);
+  } else {
+    DLGO_REQUIRE(p.splits <= 65535, "attention_q8: sequences of %d tokens are too long", max_kv_len);
+    const long long need = p.splits > 1 ? (long long)n_rows * n_heads * p.splits * PART_ROW : 0;
+    DLGO_REQUIRE(need == 0 || (part && part_elems >= need && ((uintptr_t)part & 15) == 0), "attention_q8: scratch of %lld floats is needed, %lld given", need, part ? part_elems : 0ll);
+    const dim3 grid((unsigned)(n_kv * p.chunks), (unsigned)n_seq, (unsigned)p.splits);
+    e = hipErrorInvalidValue;
+    if (p.nc == 1) e = launch_decode_waves<1>(a, grid, stream);
+    if constexpr (NC_MOST >= 2) if (p.nc == 2) e = launch_decode_waves<2>(a, grid, stream);
+    if constexpr (NC_MOST >= 4) if (p.nc == 4) e = launch_decode_waves<4>(a, grid, stream);
+    if (e == hipSuccess && p.splits > 1) {
+      DLGO_LAUNCH_CHECK("attention_q8");
+      hipLaunchKernelGGL(attn_combine_kernel, dim3((unsigned)(max_q_len * n_heads), (unsigned)n_seq), dim3(WAVE), 0, stream, a);
+    }
+  }
+  DLGO_REQUIRE(e == hipSuccess, "attention_q8: %s", hipGetErrorString(e));
+  DLGO_LAUNCH_CHECK("attention_q8");
+  return nullptr;
+}

@@ -1,0 +1,355 @@
+// Rotation of a step's queries and keys, fused with the write of keys and values into the 8-bit cache (q8_page.h).
+//
+// For a token's key (rotated) or value x of one head:  e = the least integer with max|x| <= 448 * 2^e (at least -126),
+//   byte_d = e4m3(x_d * 2^-e), to nearest, ties to even;  scale = e + 127.
+// The multiplication is exact, so an element is rounded once, from float32: off by at most 2^-4 of itself (half a step
+// of e4m3's 3 bits), or 2^-10 * 2^e below e4m3's smallest normal number.  computerex/dlgo keeps keys and values in
+// float32 (memory/kvcache.go:5-9); its weights' 8-bit blocks carry a scale each (quant/dequant.go), as tokens do here.
+//
+// Bound by memory: a row is read once (the second read of a partner piece hits the cache), queries are written in
+// bfloat16, keys and values in 8 bits.
+#include "q8_page.h"
+// everything here is float32 arithmetic whatever the storage type: no approximation can be named (exact_begin.h)
+#include "exact_begin.h"
+
+struct RopeQ8 {
+  const bf16_t* qkv;
+  bf16_t* q_out;
+  uint8_t* cache;
+  const float* cos_t;
+  const float* sin_t;
+  const int32_t* positions;
+  const int32_t* tok_seq;
+  const int32_t* slots;
+  const int32_t* page_table;
+  long long page_stride;
+  int ld, ldq, n_tokens, n_heads, n_kv, hd, rot, interleaved, table_rows, n_seq, n_slots, max_pages, n_pages;
+};
+
+static __device__ __forceinline__ void load8(const bf16_t* p, float* f) {
+  const uint4 u = *(const uint4*)p;
+  f[0] = __uint_as_float(u.x << 16); f[1] = __uint_as_float(u.x & 0xffff0000u);
+  f[2] = __uint_as_float(u.y << 16); f[3] = __uint_as_float(u.y & 0xffff0000u);
+  f[4] = __uint_as_float(u.z << 16); f[5] = __uint_as_float(u.z & 0xffff0000u);
+  f[6] = __uint_as_float(u.w << 16); f[7] = __uint_as_float(u.w & 0xffff0000u);
+}
+
+// Eight elements of a head from element d0 on, rotated.  PIECES: pairs lie in this piece (interleaved) or are this piece
+// and the one half a rotated width away, all 16-byte aligned; else element by element.
+template <bool PIECES>
+static __device__ __forceinline__ void rotated8(const RopeQ8& a, const bf16_t* head, int pos, int d0, float* y) {
+  const int half = a.rot / 2;
+  // a position beyond the table is the caller's mistake: it must not become a read out of bounds
+  const size_t at = (size_t)(pos < 0 ? 0 : (pos < a.table_rows ? pos : a.table_rows - 1)) * half;
+  if constexpr (PIECES) {
+    load8(head + d0, y);
+    if (!a.cos_t || d0 >= a.rot) return;
+    float c[8], s[8], x[8];
+    if (a.interleaved) {
+      *(float4*)c = *(const float4*)(a.cos_t + at + d0 / 2);
+      *(float4*)s = *(const float4*)(a.sin_t + at + d0 / 2);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float x0 = y[2 * i], x1 = y[2 * i + 1];
+        y[2 * i] = rotated_lo(x0, x1, c[i], s[i]);
+        y[2 * i + 1] = rotated_hi(x0, x1, c[i], s[i]);
+      }
+      return;
+    }
+    const bool low = d0 < half;
+    const int i0 = low ? d0 : d0 - half;
+    load8(head + (low ? d0 + half : d0 - half), x);
+#pragma unroll
+    for (int e = 0; e < 8; e += 4) {
+      *(float4*)(c + e) = *(const float4*)(a.cos_t + at + i0 + e);
+      *(float4*)(s + e) = *(const float4*)(a.sin_t + at + i0 + e);
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) y[e] = low ? rotated_lo(y[e], x[e], c[e], s[e]) : rotated_hi(x[e], y[e], c[e], s[e]);
+  } else {
+#pragma unroll 1
+    for (int e = 0; e < 8; ++e) {
+      const int d = d0 + e;
+      float v = bf16_to_f32(head[d]);
+      if (a.cos_t && d < a.rot) {
+        const int i = a.interleaved ? d / 2 : (d < half ? d : d - half);
+        const bool low = a.interleaved ? (d & 1) == 0 : d < half;
+        const float o = bf16_to_f32(head[a.interleaved ? (d ^ 1) : (low ? d + half : d - half)]);
+        const float c = a.cos_t[at + i], s = a.sin_t[at + i];
+        v = low ? rotated_lo(v, o, c, s) : rotated_hi(o, v, c, s);
+      }
+      y[e] = v;
+    }
+  }
+}
+
+template <bool PIECES>
+static __device__ __forceinline__ void plain8(const bf16_t* p, float* y) {
+  if constexpr (PIECES) {
+    load8(p, y);
+  } else {
+#pragma unroll 1
+    for (int e = 0; e < 8; ++e) y[e] = bf16_to_f32(p[e]);
+  }
+}
+
+static __device__ __forceinline__ uint32_t top_bits(const float* y) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const uint32_t b = __float_as_uint(y[e]) & 0x7fffffffu;
+    m = b > m ? b : m;
+  }
+  return m;
+}
+
+// the least e with (the float of these bits) <= 448 * 2^e = 1.75 * 2^(8 + e), not below -126
+static __device__ __forceinline__ int power_for(uint32_t top) {
+  const int e = (int)(top >> 23) - 127 - 8 + ((top & 0x7fffffu) > 0x600000u ? 1 : 0);
+  return e < -126 ? -126 : e;
+}
+
+static __device__ __forceinline__ uint2 to_e4m3(const float* y, int power) {
+  const float f = __uint_as_float((uint32_t)(127 - power) << 23);          // 2^-power: power is -126 to 121
+  int lo = 0, hi = 0;
+  lo = __builtin_amdgcn_cvt_pk_fp8_f32(y[0] * f, y[1] * f, lo, false);
+  lo = __builtin_amdgcn_cvt_pk_fp8_f32(y[2] * f, y[3] * f, lo, true);
+  hi = __builtin_amdgcn_cvt_pk_fp8_f32(y[4] * f, y[5] * f, hi, false);
+  hi = __builtin_amdgcn_cvt_pk_fp8_f32(y[6] * f, y[7] * f, hi, true);
+  return make_uint2((uint32_t)lo, (uint32_t)hi);
+}
+
+// Where row t's token lies: its page's offset in the cache (-1 if there is no such page: nothing is written) and its
+// place in the page.
+static __device__ __forceinline__ long long page_of(const RopeQ8& a, int t, int pos) {
+  const int seq = a.tok_seq[t];
+  if (seq < 0 || seq >= a.n_seq || pos < 0 || pos / Q8_PAGE >= a.max_pages) return -1;
+  const int slot = a.slots[seq];
+  if (slot < 0 || slot >= a.n_slots) return -1;
+  const int page = a.page_table[(size_t)slot * a.max_pages + pos / Q8_PAGE];
+  return page < 0 || page >= a.n_pages ? -1 : (long long)page * a.page_stride;
+}
+
+// The queries: a thread takes a piece of eight elements and, where its pairs lie in another piece, that one too (the
+// thread of the higher piece then has nothing to do), so that q_out may be the queries' own place in qkv.
+template <bool PIECES>
+static __device__ __forceinline__ void queries(const RopeQ8& a, long long idx) {
+  const int per_head = a.hd / 8, per_row = a.n_heads * per_head;
+  if (idx >= (long long)a.n_tokens * per_row) return;
+  const int t = (int)(idx / per_row), c = (int)(idx % per_row), d0 = (c % per_head) * 8;
+  const bf16_t* head = a.qkv + (size_t)t * a.ld + (size_t)(c / per_head) * a.hd;
+  bf16_t* dst = a.q_out + (size_t)t * a.ldq + (size_t)(c / per_head) * a.hd;
+  const int pos = a.positions[t];
+  if constexpr (PIECES) {
+    const bool far = a.cos_t && !a.interleaved && d0 < a.rot;
+    const int half = a.rot / 2;
+    if (far && d0 >= half) return;
+    float y[8], z[8];
+    rotated8<true>(a, head, pos, d0, y);
+    if (far) rotated8<true>(a, head, pos, d0 + half, z);
+    Elem<bf16_t>::store4(dst + d0, y[0], y[1], y[2], y[3]);
+    Elem<bf16_t>::store4(dst + d0 + 4, y[4], y[5], y[6], y[7]);
+    if (far) {
+      Elem<bf16_t>::store4(dst + d0 + half, z[0], z[1], z[2], z[3]);
+      Elem<bf16_t>::store4(dst + d0 + half + 4, z[4], z[5], z[6], z[7]);
+    }
+  } else if (d0 == 0) {      // widths that no model of a usual shape has: a thread takes a whole head, pair by pair
+    const int half = a.rot / 2;
+    const size_t at = (size_t)(pos < 0 ? 0 : (pos < a.table_rows ? pos : a.table_rows - 1)) * half;
+#pragma unroll 1
+    for (int i = 0; i < half; ++i) {
+      const int i0 = a.interleaved ? 2 * i : i, i1 = a.interleaved ? 2 * i + 1 : i + half;
+      float x0 = bf16_to_f32(head[i0]), x1 = bf16_to_f32(head[i1]);
+      if (a.cos_t) {
+        const float c_ = a.cos_t[at + i], s_ = a.sin_t[at + i];
+        const float y0 = rotated_lo(x0, x1, c_, s_), y1 = rotated_hi(x0, x1, c_, s_);
+        x0 = y0;
+        x1 = y1;
+      }
+      dst[i0] = f32_to_bf16(x0);
+      dst[i1] = f32_to_bf16(x1);
+    }
+#pragma unroll 1
+    for (int i = a.rot; i < a.hd; ++i) dst[i] = head[i];
+  }
+}
+
+// `lanes` (a power of two, at least hd / 8) neighbouring threads share a token's key and value of one head, a piece of
+// eight elements each.
+template <bool PIECES>
+static __device__ __forceinline__ void key_and_value(const RopeQ8& a, int t, int kvh, int piece, int lanes, int pos, uint2* kb, uint2* vb,
+                                                     int* ks, int* vs) {
+  float k[8], v[8];
+  const int d0 = piece * 8;
+  uint32_t kt = 0, vt = 0;
+  if (d0 < a.hd) {
+    const bf16_t* row = a.qkv + (size_t)t * a.ld;
+    rotated8<PIECES>(a, row + (size_t)(a.n_heads + kvh) * a.hd, pos, d0, k);
+    plain8<PIECES>(row + (size_t)(a.n_heads + a.n_kv + kvh) * a.hd + d0, v);
+    kt = top_bits(k);
+    vt = top_bits(v);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) k[e] = v[e] = 0.f;
+  }
+  for (int o = lanes >> 1; o > 0; o >>= 1) {
+    const uint32_t k2 = (uint32_t)__shfl_xor((int)kt, o, WAVE), v2 = (uint32_t)__shfl_xor((int)vt, o, WAVE);
+    kt = k2 > kt ? k2 : kt;
+    vt = v2 > vt ? v2 : vt;
+  }
+  const bool finite = kt < 0x7f800000u && vt < 0x7f800000u;
+  const int ke = power_for(kt), ve = power_for(vt);
+  *kb = finite ? to_e4m3(k, ke) : make_uint2(0, 0);
+  *vb = finite ? to_e4m3(v, ve) : make_uint2(0, 0);
+  *ks = finite ? ke + 127 : Q8_NAN;
+  *vs = finite ? ve + 127 : 127;
+}
+
+// Few rows: no two of them need lie in one page, so a thread stores what it has where it goes (values byte by byte).
+template <bool PIECES>
+__global__ __launch_bounds__(256) void rope_kv_q8_rows_kernel(RopeQ8 a, int kv_blocks, int lanes) {
+  if ((int)blockIdx.x >= kv_blocks) {
+    queries<PIECES>(a, (long long)((int)blockIdx.x - kv_blocks) * 256 + threadIdx.x);
+    return;
+  }
+  const long long unit = ((long long)blockIdx.x * 256 + threadIdx.x) / lanes;
+  const int piece = threadIdx.x % lanes;
+  const long long units = (long long)a.n_tokens * a.n_kv;
+  const bool real = unit < units;
+  const int t = real ? (int)(unit / a.n_kv) : 0, kvh = real ? (int)(unit % a.n_kv) : 0;
+  const int pos = a.positions[t];
+  uint2 kb, vb;
+  int ks, vs;
+  key_and_value<PIECES>(a, t, kvh, piece, lanes, pos, &kb, &vb, &ks, &vs);
+  const long long off = page_of(a, t, pos);
+  if (!real || off < 0 || piece * 8 >= a.hd) return;
+  uint8_t* head = a.cache + off + (size_t)kvh * q8_head_bytes(a.hd);
+  const int in = pos % Q8_PAGE, t16 = in >> 4, i = in & 15, g = i >> 2, r = i & 3;
+  *(uint2*)(head + (t16 * (a.hd / 16) + piece / 2) * 256 + i * 16 + (piece & 1) * 8) = kb;
+  uint8_t* val = head + Q8_PAGE * a.hd + ((piece / 2 * 4 + g) * 16 + (piece & 1) * 8) * 16 + 4 * t16 + r;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) val[e * 16] = (uint8_t)((e < 4 ? vb.x : vb.y) >> (8 * (e & 3)));
+  if (piece == 0) {
+    uint8_t* scales = head + 2 * Q8_PAGE * a.hd;
+    scales[4 * i + t16] = (uint8_t)ks;
+    scales[64 + 16 * g + 4 * t16 + r] = (uint8_t)vs;
+  }
+}
+
+// Many rows: a block takes 64 consecutive rows of the step and one kv head, brings keys and values together in LDS, and
+// stores with its lanes in the order of the page: 16 tokens of a keys' piece are 256 bytes in a row, and four tokens of a
+// value's element one word, where four neighbouring rows are neighbouring tokens of a page (elsewhere byte by byte).
+template <bool PIECES>
+__global__ __launch_bounds__(256) void rope_kv_q8_tiles_kernel(RopeQ8 a, int kv_blocks, int lanes) {
+  extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+  if ((int)blockIdx.x >= kv_blocks) {
+    queries<PIECES>(a, (long long)((int)blockIdx.x - kv_blocks) * 256 + threadIdx.x);
+    return;
+  }
+  __shared__ long long at[64];        // each row's page in the cache, -1 where there is none
+  __shared__ int in_page[64];
+  const int stride = a.hd + 16;       // rows 16 bytes apart in the banks
+  uint8_t* kt = lds;
+  uint8_t* vt = lds + 64 * stride;
+  const int kvh = blockIdx.x % a.n_kv, t0 = (blockIdx.x / a.n_kv) * 64;
+  const int n = a.n_tokens - t0 < 64 ? a.n_tokens - t0 : 64;
+  if (threadIdx.x < 64) {
+    const int t = t0 + ((int)threadIdx.x < n ? (int)threadIdx.x : n - 1);
+    const int pos = a.positions[t];
+    at[threadIdx.x] = (int)threadIdx.x < n ? page_of(a, t, pos) : -1;
+    in_page[threadIdx.x] = pos & (Q8_PAGE - 1);
+  }
+  __syncthreads();
+  const size_t head = (size_t)kvh * q8_head_bytes(a.hd);
+  const int piece = threadIdx.x % lanes;
+  for (int j0 = 0; j0 < 64; j0 += 256 / lanes) {        // whole waves take part in the shuffles
+    const int j = j0 + threadIdx.x / lanes;
+    const int t = t0 + (j < n ? j : n - 1);
+    uint2 kb, vb;
+    int ks, vs;
+    key_and_value<PIECES>(a, t, kvh, piece, lanes, a.positions[t], &kb, &vb, &ks, &vs);
+    if (j >= 64 || piece * 8 >= a.hd) continue;
+    *(uint2*)(kt + j * stride + piece * 8) = kb;
+    *(uint2*)(vt + j * stride + piece * 8) = vb;
+    if (piece == 0 && at[j] >= 0) {
+      uint8_t* scales = a.cache + at[j] + head + 2 * Q8_PAGE * a.hd;
+      const int in = in_page[j], t16 = in >> 4, i = in & 15;
+      scales[4 * i + t16] = (uint8_t)ks;
+      scales[64 + 16 * (i >> 2) + 4 * t16 + (i & 3)] = (uint8_t)vs;
+    }
+  }
+  __syncthreads();
+  const int pieces = a.hd / 16;
+  for (int c = threadIdx.x; c < 64 * pieces; c += 256) {
+    const int j = c & 63, p = c >> 6;
+    if (at[j] < 0) continue;
+    const int in = in_page[j];
+    *(uint4*)(a.cache + at[j] + head + ((in >> 4) * pieces + p) * 256 + (in & 15) * 16) = *(const uint4*)(kt + j * stride + p * 16);
+  }
+  // four rows of a word: q = which of the four words 16 rows apart, so that 64 lanes write 256 bytes in a row
+  const int lead = 3 & -in_page[0];   // rows before the first one whose place in its page is a multiple of four
+  for (int c = threadIdx.x; c < 64 * (a.hd / 4); c += 256) {
+    const int q = c & 3, d = (c >> 2) % a.hd, g = (c >> 2) / a.hd;       // g: 0 .. 3
+    // 16 groups of four rows from row `lead` on, and the rows left over at both ends (lead of them before, 4 - lead after)
+    const int j = lead + 16 * q + 4 * g;
+    const bool whole = j + 3 < n && at[j] >= 0 && (in_page[j] & 3) == 0 && at[j + 3] == at[j] && at[j + 1] == at[j] && at[j + 2] == at[j] &&
+                       in_page[j + 1] == in_page[j] + 1 && in_page[j + 2] == in_page[j] + 2 && in_page[j + 3] == in_page[j] + 3;
+    const uint8_t* src = vt + d;
+    uint8_t* page = a.cache + head + Q8_PAGE * a.hd + (d & ~15) * 64 + (d & 15) * 16;
+    if (whole) {
+      const int in = in_page[j];
+      const uint32_t w = src[j * stride] | (src[(j + 1) * stride] << 8) | (src[(j + 2) * stride] << 16) | ((uint32_t)src[(j + 3) * stride] << 24);
+      *(uint32_t*)(page + at[j] + ((in >> 2) & 3) * 256 + (in >> 4) * 4) = w;
+      continue;
+    }
+    for (int m = 0; m < 4; ++m) {
+      const int jm = (j + m) & 63;            // the last group's rows past the tile are the first ones, before `lead`
+      if (jm >= n || at[jm] < 0) continue;
+      const int in = in_page[jm];
+      page[at[jm] + ((in >> 2) & 3) * 256 + (in >> 4) * 4 + (in & 3)] = src[jm * stride];
+    }
+  }
+}
+
+extern "C" const char* dlgo_rope_kv_q8(const void* qkv, int ld, void* q_out, int ldq, int n_tokens, int n_heads, int n_kv, int hd,
+                                       int rot, int interleaved, const float* cos_t, const float* sin_t, int table_rows,
+                                       const int32_t* positions, const int32_t* tok_seq, const int32_t* slots, int n_seq,
+                                       const int32_t* page_table, int n_slots, int max_pages, void* cache, long long page_stride,
+                                       int n_pages, int write_kv, hipStream_t stream) {
+  DLGO_REQUIRE(n_tokens >= 0 && n_heads > 0 && n_kv >= 0 && hd >= 16 && hd % 16 == 0 && hd <= 256,
+               "rope_kv_q8: %d rows, %d query and %d kv heads of size %d (head sizes come in steps of 16, up to 256)", n_tokens, n_heads, n_kv, hd);
+  DLGO_REQUIRE(rot >= 0 && rot <= hd && rot % 2 == 0, "rope_kv_q8: rotated width %d must be even and at most the head size %d", rot, hd);
+  DLGO_REQUIRE(ld >= (n_heads + (write_kv ? 2 * n_kv : 0)) * hd && ldq >= n_heads * hd, "rope_kv_q8: row strides %d and %d are shorter than the heads they hold", ld, ldq);
+  DLGO_REQUIRE((cos_t == nullptr) == (sin_t == nullptr), "rope_kv_q8: cos and sin tables come together");
+  DLGO_REQUIRE(cos_t == nullptr || table_rows > 0, "rope_kv_q8: empty rotation table");
+  DLGO_REQUIRE(!write_kv || (n_kv > 0 && cache && page_table && slots && tok_seq && max_pages > 0 && n_slots > 0 && n_seq > 0 && n_pages > 0),
+               "rope_kv_q8: cache arguments missing");
+  DLGO_REQUIRE(!write_kv || (((uintptr_t)cache & 15) == 0 && page_stride % 16 == 0 && page_stride >= n_kv * q8_head_bytes(hd)),
+               "rope_kv_q8: pages %lld bytes apart (16-byte aligned pages of at least %lld bytes are needed)", page_stride, n_kv * q8_head_bytes(hd));
+  if (n_tokens == 0) return nullptr;
+  RopeQ8 a = {(const bf16_t*)qkv, (bf16_t*)q_out, (uint8_t*)cache, cos_t, sin_t, positions, tok_seq, slots, page_table,
+              page_stride, ld, ldq, n_tokens, n_heads, n_kv, hd, rot, interleaved, table_rows, n_seq, n_slots, max_pages, n_pages};
+  const bool pieces = rot % (interleaved ? 8 : 16) == 0 && ld % 8 == 0 && ldq % 8 == 0 && ((uintptr_t)qkv & 15) == 0 && ((uintptr_t)q_out & 15) == 0 &&
+                      (!cos_t || (((uintptr_t)cos_t & 15) == 0 && ((uintptr_t)sin_t & 15) == 0));
+  int lanes = 2;
+  while (lanes * 8 < hd) lanes *= 2;
+  // a block of the many-rows kernel takes 64 rows of a head: from 128 rows on it stores whole lines where the other
+  // stores single bytes, below there are too few of its blocks
+  const bool tiles = n_tokens >= 128;
+  const long long kv_blocks = !write_kv ? 0 : tiles ? (long long)((n_tokens + 63) / 64) * n_kv : ((long long)n_tokens * n_kv * lanes + 255) / 256;
+  const long long q_blocks = ((long long)n_tokens * n_heads * (hd / 8) + 255) / 256;
+  DLGO_REQUIRE(kv_blocks + q_blocks < (1ll << 31), "rope_kv_q8: too many rows at once");
+  const dim3 grid((unsigned)(kv_blocks + q_blocks));
+  const int lds = 2 * 64 * (hd + 16);
+  if (tiles) {
+    if (pieces) hipLaunchKernelGGL(rope_kv_q8_tiles_kernel<true>, grid, dim3(256), lds, stream, a, (int)kv_blocks, lanes);
+    else hipLaunchKernelGGL(rope_kv_q8_tiles_kernel<false>, grid, dim3(256), lds, stream, a, (int)kv_blocks, lanes);
+  } else {
+    if (pieces) hipLaunchKernelGGL(rope_kv_q8_rows_kernel<true>, grid, dim3(256), 0, stream, a, (int)kv_blocks, lanes);
+    else hipLaunchKernelGGL(rope_kv_q8_rows_kernel<false>, grid, dim3(256), 0, stream, a, (int)kv_blocks, lanes);
+  }
+  DLGO_LAUNCH_CHECK("rope_kv_q8");
+  return nullptr;
+}
+
+#include "exact_end.h"

@@ -86,7 +86,8 @@ def _lib(module: str, defines=()):
     if lib is None:
         lib = build.load(module, defines)
         for name in ("dlgo_embed", "dlgo_copy_rows", "dlgo_rmsnorm", "dlgo_rope_kv", "dlgo_gemm", "dlgo_gemm_accum_norm", "dlgo_gemm_parts", "dlgo_gemm_rows", "dlgo_gemm_rmsnorm", "dlgo_gemm_rows_leave_parts", "dlgo_gemm_rows_scaled", "dlgo_gemm_tile_leave", "dlgo_gemm_tile_scaled", "dlgo_attention_rows",
-                     "dlgo_attention_prefill", "dlgo_attention_prefill_f32", "dlgo_attention_decode", "dlgo_attention_decode_f32", "dlgo_argmax", "dlgo_sample", "dlgo_bias_add", "dlgo_head_rmsnorm"):
+                     "dlgo_attention_prefill", "dlgo_attention_prefill_f32", "dlgo_attention_decode", "dlgo_attention_decode_f32", "dlgo_argmax", "dlgo_sample", "dlgo_bias_add", "dlgo_head_rmsnorm",
+                     "dlgo_rope_kv_q8", "dlgo_attention_q8", "dlgo_verify_drafts"):
             if hasattr(lib, name):
                 getattr(lib, name).restype = ctypes.c_char_p
         _libs[key] = lib
@@ -705,6 +706,140 @@ def attention(q: torch.Tensor, out: torch.Tensor, n_heads: int, n_kv: int, head_
     return out
 
 
+Q8_MAX_HEAD_DIM = 256      # head sizes of the 8-bit cache: multiples of 16 up to this one
+
+
+def q8_page_bytes(n_kv: int, head_dim: int) -> int:
+    """Bytes of one layer's part of a page of the 8-bit cache: for each kv head 64 tokens' keys and values in a byte an
+    element, and a byte for the power of two of each token's key and value (csrc/q8_page.h)."""
+    return n_kv * 2 * PAGE * (head_dim + 1)
+
+
+def _q8_cache(name: str, cache: torch.Tensor, page_stride: int, n_kv: int, head_dim: int) -> int:
+    """How many whole pages a cache tensor holds (the kernels touch no page beyond)."""
+    _need(cache, f"{name}: cache", torch.uint8, 1)
+    page = q8_page_bytes(n_kv, head_dim)
+    if head_dim % 16 or not 16 <= head_dim <= Q8_MAX_HEAD_DIM:
+        raise KernelError(f"{name}: the 8-bit cache takes head sizes in steps of 16, up to {Q8_MAX_HEAD_DIM}, not {head_dim}")
+    if not cache.is_contiguous() or page_stride < page or cache.numel() < page:
+        raise KernelError(f"{name}: a cache of {cache.numel()} bytes with pages {page_stride} bytes apart does not hold pages of {page} bytes")
+    return min((cache.numel() - page) // page_stride + 1, 2 ** 31 - 1)
+
+
+def _same_device(name: str, first: torch.Tensor, *others: Optional[torch.Tensor]) -> None:
+    """Everything on one device, and that device the current one: the launches go to its current stream."""
+    for t in others:
+        if t is not None and t.device != first.device:
+            raise KernelError(f"{name}: tensors on {first.device} and {t.device}")
+    if first.device.index != torch.cuda.current_device():
+        raise KernelError(f"{name}: tensors on {first.device}, the current device is cuda:{torch.cuda.current_device()}")
+
+
+def rope_kv_q8(qkv: torch.Tensor, q_out: torch.Tensor, n_heads: int, n_kv: int, head_dim: int, rot: int, interleaved: bool,
+               cos: Optional[torch.Tensor], sin: Optional[torch.Tensor], positions: torch.Tensor,
+               tok_seq: Optional[torch.Tensor], slots: Optional[torch.Tensor], page_table: Optional[torch.Tensor],
+               cache: Optional[torch.Tensor], page_stride: int, write_kv: bool = True) -> None:
+    """rope_kv() for the 8-bit cache: the query heads of qkv [T, (H+2KV)*hd] (bfloat16) rotated into q_out [T, H*hd], which
+    may be their own place in qkv; the key heads rotated and, with the values, stored in 8 bits in the page of each token
+    (cache: uint8, from the first byte of this layer's part of page 0 on; page_stride in bytes).  positions [T], tok_seq
+    [T] (each row's index into slots) and slots are int32.  A token's key (value) of a head is stored as e4m3 numbers times the least power of
+    two (from 2^-126 on) that brings its largest magnitude within 448; each element is rounded once, from float32.  A token whose key
+    or value is not finite is marked as a whole, and every row that sees it becomes NaN in that kv head's queries' results.
+    Rows whose position has no page (a hole in the table, a page the cache does not hold) store nothing.  Positions must
+    lie inside the rotation tables.  write_kv=False: queries only."""
+    _need(qkv, "rope_kv_q8: qkv rows", torch.bfloat16, 2)
+    _need(q_out, "rope_kv_q8: query rows", torch.bfloat16, 2)
+    _need(positions, "rope_kv_q8: positions", torch.int32, 1)
+    t = qkv.shape[0]
+    if head_dim % 16 or not 16 <= head_dim <= Q8_MAX_HEAD_DIM:
+        raise KernelError(f"rope_kv_q8: the 8-bit cache takes head sizes in steps of 16, up to {Q8_MAX_HEAD_DIM}, not {head_dim}")
+    if n_heads < 1 or n_kv < 0 or (write_kv and n_kv < 1):
+        raise KernelError(f"rope_kv_q8: {n_heads} query and {n_kv} kv heads")
+    if positions.shape[0] != t or not positions.is_contiguous():
+        raise KernelError("rope_kv_q8: one position per row, in a row in memory")
+    if qkv.shape[1] < (n_heads + (2 * n_kv if write_kv else 0)) * head_dim or q_out.shape[0] != t or q_out.shape[1] != n_heads * head_dim:
+        raise KernelError(f"rope_kv_q8: rows {tuple(qkv.shape)} and query rows {tuple(q_out.shape)} do not fit {n_heads} query and {n_kv} kv heads of {head_dim}")
+    table_rows = 0
+    if (cos is None) != (sin is None):
+        raise KernelError("rope_kv_q8: cos and sin tables come together")
+    if cos is not None:
+        _need(cos, "rope_kv_q8: cos table", torch.float32, 2)
+        _need(sin, "rope_kv_q8: sin table", torch.float32, 2)
+        if cos.shape != sin.shape or cos.shape[1] != rot // 2 or not cos.is_contiguous() or not sin.is_contiguous():
+            raise KernelError(f"rope_kv_q8: tables {tuple(cos.shape)} do not fit a rotated width of {rot}")
+        table_rows = cos.shape[0]
+    n_pages = max_pages = n_slots = n_seq = 0
+    if write_kv:
+        for what, v, dims in (("token->sequence", tok_seq, 1), ("slots", slots, 1), ("page table", page_table, 2)):
+            _need(v, f"rope_kv_q8: {what}", torch.int32, dims)
+            if not v.is_contiguous():
+                raise KernelError(f"rope_kv_q8: {what} must be contiguous")
+        if tok_seq.shape[0] != t:
+            raise KernelError("rope_kv_q8: one sequence index per row")
+        n_pages = _q8_cache("rope_kv_q8", cache, page_stride, n_kv, head_dim)
+        n_slots, max_pages = page_table.shape
+        n_seq = slots.shape[0]
+    _same_device("rope_kv_q8", qkv, q_out, positions, cos, sin, *((tok_seq, slots, page_table, cache) if write_kv else ()))
+    if t == 0:
+        return
+    _check(_lib("kv_q8").dlgo_rope_kv_q8(_ptr(qkv), _rows(qkv, "rope_kv_q8: qkv rows"), _ptr(q_out), _rows(q_out, "rope_kv_q8: query rows"),
+                                         t, n_heads, n_kv, head_dim, rot, int(interleaved), _ptr(cos), _ptr(sin), table_rows,
+                                         _ptr(positions), _ptr(tok_seq), _ptr(slots), n_seq, _ptr(page_table), n_slots, max_pages,
+                                         _ptr(cache), ctypes.c_longlong(page_stride), n_pages, int(write_kv), _stream()))
+
+
+def attention_q8(q: torch.Tensor, out: torch.Tensor, n_heads: int, n_kv: int, head_dim: int, cu_q: torch.Tensor,
+                 start_pos: torch.Tensor, slots: Optional[torch.Tensor], page_table: torch.Tensor, cache: torch.Tensor,
+                 page_stride: int, max_q_len: int, max_kv_len: int, window: int = 0, scale: Optional[float] = None,
+                 scratch=None) -> torch.Tensor:
+    """Attention of a step's (rotated) query rows q [T, H*hd] over the 8-bit cache that rope_kv_q8() writes, which holds
+    the step's own tokens already; out [T, H*hd], both bfloat16.
+
+    cu_q [n_seq + 1], start_pos [n_seq], slots [n_seq]: int32 on the device.  Sequence i brings rows cu_q[i] to cu_q[i+1]
+    (none, one, a few drafted tokens, a prompt), at positions from start_pos[i] on, and its pages are row slots[i] of
+    page_table (row i if slots is None).  A row sees the keys up to its own position, with window > 0 the last `window`
+    of them.  Rows behind the last sequence's are left as they were.  max_q_len and max_kv_len (host) bound the
+    rows a sequence brings and the tokens it holds afterwards: a captured step passes what it allows for; rows and
+    tokens beyond the bounds are left out or slow, never out of bounds.  scratch(n) returns a float32 buffer of at least n elements for what
+    several blocks find of a row (allocated here if not given).  A row that finds no page at all is zeros."""
+    _need(q, "attention_q8: query rows", torch.bfloat16, 2)
+    _need(out, "attention_q8: output", torch.bfloat16, 2)
+    for what, v, dims in (("row offsets", cu_q, 1), ("start positions", start_pos, 1), ("slots", slots, 1), ("page table", page_table, 2)):
+        if v is None and what == "slots":
+            continue
+        _need(v, f"attention_q8: {what}", torch.int32, dims)
+        if not v.is_contiguous():
+            raise KernelError(f"attention_q8: {what} must be contiguous")
+    n_pages = _q8_cache("attention_q8", cache, page_stride, n_kv, head_dim)
+    t, n_seq = q.shape[0], start_pos.shape[0]
+    if n_kv < 1 or n_heads % n_kv or q.shape[1] != n_heads * head_dim or out.shape != q.shape:
+        raise KernelError(f"attention_q8: query rows {tuple(q.shape)} and output {tuple(out.shape)} do not fit {n_heads} heads of {head_dim} over {n_kv} kv heads")
+    if cu_q.shape[0] != n_seq + 1 or (slots is not None and slots.shape[0] != n_seq) or (slots is None and page_table.shape[0] < n_seq):
+        raise KernelError("attention_q8: row offsets, start positions and slots do not fit each other")
+    if max_q_len < 0 or max_kv_len < 0 or window < 0:
+        raise KernelError("attention_q8: bounds and window must not be negative")
+    if scale is None:
+        scale = 1.0 / math.sqrt(head_dim)
+    _same_device("attention_q8", q, out, cu_q, start_pos, slots, page_table, cache)
+    if t == 0 or n_seq == 0 or max_q_len == 0:
+        return out
+    max_q_len = min(int(max_q_len), t)
+    max_kv_len = max(1, min(int(max_kv_len), page_table.shape[1] * PAGE))
+    lib = _lib("attention_q8", (("HEAD_DIM", head_dim),))
+    lib.dlgo_attention_q8_scratch.restype = ctypes.c_longlong
+    need = lib.dlgo_attention_q8_scratch(t, n_seq, n_heads, n_kv, max_q_len, max_kv_len, int(window))
+    part = None
+    if need:
+        part = scratch(need) if scratch is not None else torch.empty(need, dtype=torch.float32, device=q.device)
+        _need(part, "attention_q8: scratch", torch.float32, 1)
+    _check(lib.dlgo_attention_q8(_ptr(q), _rows(q, "attention_q8: query rows"), _ptr(out), _rows(out, "attention_q8: output"), t, n_seq,
+                                 n_heads, n_kv, head_dim, _ptr(cu_q), _ptr(start_pos), _ptr(slots), _ptr(page_table),
+                                 page_table.shape[0], page_table.shape[1], _ptr(cache), ctypes.c_longlong(page_stride), n_pages,
+                                 max_q_len, max_kv_len, int(window), ctypes.c_float(scale), _ptr(part),
+                                 ctypes.c_longlong(part.numel() if part is not None else 0), _stream()))
+    return out
+
+
 _argmax_scratch: dict = {}
 
 
@@ -767,6 +902,60 @@ def sample(logits: torch.Tensor, work: torch.Tensor, temperature: torch.Tensor, 
     return out
 
 
+def verify_drafts(logits: torch.Tensor, draft_tokens: torch.Tensor, cu_drafts: torch.Tensor, temperature: torch.Tensor,
+                  uniform: torch.Tensor, accepted: torch.Tensor, token: torch.Tensor, max_drafts: int,
+                  draft_logits: Optional[torch.Tensor] = None, probs: Optional[torch.Tensor] = None, scratch=None) -> None:
+    """How many of each sequence's drafted tokens the target model keeps, and the token that follows them.
+
+    Sequence i drafted the tokens cu_drafts[i] to cu_drafts[i+1] of draft_tokens (int32, D in all; none is allowed, more
+    than max_drafts are not looked at) and
+    brings one row of the target's float32 logits [D + n, V] for the place of each draft and one for the place after them,
+    from row cu_drafts[i] + i on; uniform [D + n] has a number in [0, 1) for each of those rows.  temperature [n]; 0 is
+    greedy.  draft_logits [D, V]: the logits that the drafts were drawn from (at the same temperature); None: the drafts
+    are certain of their tokens (looked up, or a greedy draft model's).
+
+    With p = softmax(logits / T) and q = softmax(draft_logits / T) (or one for the drafted token), draft j is kept while
+    uniform_j * q(token_j) < p(token_j); accepted[i] (int32) counts the kept ones, token[i] (int32) is drawn from max(p - q, 0)
+    of the first refused draft's row, or from p of the last row, as the first index whose running sum exceeds the
+    sequence's last uniform number times the whole.  Greedy: a draft is kept if it is the row's maximum (lowest index), and the token is
+    the maximum.  Sums are 64-bit, in an order that only the shapes decide.  A logit of -inf or NaN has no weight.  A token
+    outside the vocabulary is refused.  probs [D] (float32, optional): p(token_j) for every draft.  scratch(n) returns a uint8 buffer of at least n
+    bytes (allocated here if not given)."""
+    _need(logits, "verify_drafts: logits", torch.float32, 2)
+    n, v = temperature.shape[0], logits.shape[1]
+    d = draft_tokens.shape[0]
+    for what, x, dt, size in (("draft tokens", draft_tokens, torch.int32, d), ("draft offsets", cu_drafts, torch.int32, n + 1),
+                              ("temperature", temperature, torch.float32, n), ("uniform numbers", uniform, torch.float32, d + n),
+                              ("accepted", accepted, torch.int32, n), ("token", token, torch.int32, n), ("probs", probs, torch.float32, d)):
+        if x is None and what == "probs":
+            continue
+        _need(x, f"verify_drafts: {what}", dt, 1)
+        if x.shape[0] != size or not x.is_contiguous():
+            raise KernelError(f"verify_drafts: {what} has shape {tuple(x.shape)}, {size} entries in a row are needed ({n} sequences, {d} drafts)")
+    if logits.shape[0] != d + n or v < 1:
+        raise KernelError(f"verify_drafts: {n} sequences with {d} drafts need {d + n} rows of logits, found {tuple(logits.shape)}")
+    if draft_logits is not None:
+        _need(draft_logits, "verify_drafts: draft logits", torch.float32, 2)
+        if tuple(draft_logits.shape) != (d, v):
+            raise KernelError(f"verify_drafts: draft logits {tuple(draft_logits.shape)}, expected {(d, v)}")
+    if max_drafts < 0:
+        raise KernelError("verify_drafts: max_drafts must not be negative")
+    _same_device("verify_drafts", logits, draft_tokens, cu_drafts, temperature, uniform, accepted, token, draft_logits, probs)
+    if n == 0:
+        return
+    model_drafts = draft_logits is not None and d > 0
+    lib = _lib("verify")
+    lib.dlgo_verify_drafts_scratch.restype = ctypes.c_longlong
+    need = lib.dlgo_verify_drafts_scratch(n, d, v, int(model_drafts))
+    work = scratch(need) if scratch is not None else torch.empty(need, dtype=torch.uint8, device=logits.device)
+    _need(work, "verify_drafts: scratch", torch.uint8, 1)
+    _check(lib.dlgo_verify_drafts(_ptr(logits), ctypes.c_longlong(_rows(logits, "verify_drafts: logits")), _ptr(draft_tokens),
+                                  _ptr(draft_logits if model_drafts else None),
+                                  ctypes.c_longlong(_rows(draft_logits, "verify_drafts: draft logits") if model_drafts else 0),
+                                  _ptr(cu_drafts), _ptr(temperature), _ptr(uniform), n, d, v, min(int(max_drafts), d), _ptr(accepted),
+                                  _ptr(token), _ptr(probs), _ptr(work), ctypes.c_longlong(work.numel()), _stream()))
+
+
 # ---------------------------------------------------------------------------
 # Timing the launches one by one (what computerex/dlgo's gpu_timing_main.go:73-119 does for its operations): inside a
 # `with Timings() as t:` block every face above that launches something is bracketed by two events on the current
@@ -825,6 +1014,6 @@ def _timed(fn):
 
 
 for _name in ("embed", "copy_rows", "rmsnorm", "bias_add", "head_rmsnorm", "gemm_accum_then_norm", "gemm_runs", "gemm", "gemm_rmsnorm",
-              "gemm_accum_leave_norm", "gemm_scaled", "rope_kv", "attention", "argmax", "sample"):
+              "gemm_accum_leave_norm", "gemm_scaled", "rope_kv", "attention", "argmax", "sample", "rope_kv_q8", "attention_q8", "verify_drafts"):
     globals()[_name] = _timed(globals()[_name])
 del _name
