@@ -40,13 +40,17 @@ struct AttnQ8 {
   int ldq, ldo, n_rows, n_seq, n_heads, n_kv, group, n_slots, max_pages, n_pages, window;
   float scale_log2e;             // not negative; `flip` is its sign
   uint32_t flip;
-  int splits, fill, waves;       // blocks that a sequence's pages may be dealt to: see splits_of
+  int splits, fill;              // blocks that a sequence's pages may be dealt to: see splits_of
 };
+
+// Waves of a block: four.  Eight leave room for one block a compute unit (a block's own start, its first trips to memory,
+// is then nobody's time to use): 64 sequences of 2,300 tokens 31.1 against 29.3 us, 16 sequences with drafts 21.6 against 18.7.
+#define WAVES 4
 
 // How many of the launch's blocks a sequence with n pages uses: enough to fill the chip (`fill`, known at the launch),
 // but not more than leave each wave a page, and so many that a wave has at most 16 pages.
 __device__ __forceinline__ int splits_of(const AttnQ8& a, int n) {
-  const int by_wave = (n + a.waves - 1) / a.waves, by_16 = (n + 16 * a.waves - 1) / (16 * a.waves);
+  const int by_wave = (n + WAVES - 1) / WAVES, by_16 = (n + 16 * WAVES - 1) / (16 * WAVES);
   int s = a.fill < by_wave ? a.fill : by_wave;
   if (s < by_16) s = by_16;
   return s < 1 ? 1 : (s > a.splits ? a.splits : s);
@@ -77,6 +81,19 @@ __device__ __forceinline__ Span span_of(const AttnQ8& a, int seq) {
 }
 
 __device__ __forceinline__ float fast_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// The maximum of a lane's value and that of the lane 32 (16) away.
+__device__ __forceinline__ float max_32(float x) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float max_16(float x) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+// Sums are rescaled only where a maximum has grown by more than 2^8 over the one that they stand for: a probability is
+// then at most 2^8, which costs float32 and bfloat16 none of their places.
+__device__ __forceinline__ bool has_grown(float mx, float m, float scale_log2e) { return (mx - m) * scale_log2e > 8.f; }
 
 typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2_t;
 template <bool HI> __device__ __forceinline__ uint32_t pair_of(uint32_t w, float scale) {
@@ -112,26 +129,37 @@ struct PageRegs {
   uint4 vs;             // the scales of the values of tokens 16 t + 4 (lane / 16) + r
 };
 
-static __device__ __forceinline__ void fetch_page(PageRegs& p, const uint8_t* head, int lane) {
+typedef __attribute__((ext_vector_type(4))) uint32_t u32x4_t;
+static __device__ __forceinline__ uint4 buffer16(__amdgpu_buffer_rsrc_t r, int at, int fixed) {
+  const u32x4_t v = __builtin_bit_cast(u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(r, at, fixed, 0));
+  return make_uint4(v.x, v.y, v.z, v.w);
+}
+
+// Asks for a page.  Through a buffer descriptor: what lies beyond `bytes` (all of it, if that is 0: no such page) comes
+// back as zeros without a trip to memory, so no load stands under a condition, and the loads of the next page stay in
+// flight while this one is used.
+static __device__ __forceinline__ void fetch_page(PageRegs& p, const uint8_t* head, int bytes, int lane) {
+  const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc((void*)head, 0, bytes, 0x00027000);
+  const int at = lane * 16;
 #pragma unroll
   for (int t = 0; t < 4; ++t)
 #pragma unroll
-    for (int j = 0; j < KLOADS; ++j) {
-      // lanes whose piece lies beyond the head read the page's first bytes instead and count as zero below
-      const bool ok = PIECES % 4 == 0 || 4 * j + (lane >> 4) < PIECES;
-      p.k[t][j] = *(const uint4*)(head + (ok ? (t * PIECES + 4 * j) * 256 + lane * 16 : 0));
-    }
+    for (int j = 0; j < KLOADS; ++j) p.k[t][j] = buffer16(r, at, (t * PIECES + 4 * j) * 256);
+  p.ks = (uint32_t)__builtin_amdgcn_raw_buffer_load_b32(r, (lane & 15) * 4, 2 * Q8_PAGE * HD, 0);
 #pragma unroll
-  for (int c = 0; c < PIECES; ++c) p.v[c] = *(const uint4*)(head + Q8_PAGE * HD + c * 1024 + lane * 16);
-  p.ks = *(const uint32_t*)(head + 2 * Q8_PAGE * HD + (lane & 15) * 4);
-  p.vs = *(const uint4*)(head + 2 * Q8_PAGE * HD + 64 + (lane >> 4) * 16);
+  for (int c = 0; c < PIECES; ++c) p.v[c] = buffer16(r, at, Q8_PAGE * HD + c * 1024);
+  p.vs = buffer16(r, (lane >> 4) * 16, 2 * Q8_PAGE * HD + 64);
 }
 
-template <int NC, int WAVES>
-__global__ __launch_bounds__(WAVES* WAVE) void attn_decode_kernel(AttnQ8 a) {
+// Waves a SIMD that the registers are to allow: two places for a page, the sums and the queries.
+#define EU(NC) ((NC) == 1 ? (HD <= 64 ? 3 : (HD <= 128 ? 2 : 1)) : ((NC) == 2 && HD <= 64 ? 2 : 1))
+
+template <int NC>
+__global__ __launch_bounds__(WAVES* WAVE) __attribute__((amdgpu_waves_per_eu(EU(NC)))) void attn_decode_kernel(AttnQ8 a) {
   constexpr int QK = 2 * KLOADS;                         // matrix instructions for the scores of 16 tokens
   extern __shared__ __attribute__((aligned(16))) float merge[];    // [WAVES][COLS][HD], then [WAVES][COLS] maxima and sums
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, n = lane & 15;
+  const int lane = threadIdx.x & 63, g = lane >> 4, n = lane & 15;
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);        // known to be the same in all lanes, as all that follows from it
   const int kvh = blockIdx.x % a.n_kv, chunk = blockIdx.x / a.n_kv, seq = blockIdx.y, split = blockIdx.z;
   const Span s = span_of(a, seq);
   const int cols = s.rows * a.group, col0 = chunk * COLS(NC);
@@ -142,14 +170,21 @@ __global__ __launch_bounds__(WAVES* WAVE) void attn_decode_kernel(AttnQ8 a) {
   const int pg0 = s.first_page + split * per;
   const int pg1 = pg0 + per < s.first_page + s.n_pages ? pg0 + per : s.first_page + s.n_pages;      // pages [pg0, pg1)
 
-  // this lane's column of each of the NC blocks of 16: a row of the step and a head
-  bf16x8_t qf[NC][QK];
+  // The numbers of the wave's first 64 pages, one a lane, asked for together with the queries: page k of the wave is
+  // first + k * WAVES.
+  const int32_t* table = a.page_table + (size_t)s.slot * a.max_pages;
+  const int turns = pg1 - pg0 > wave ? (pg1 - pg0 - wave + WAVES - 1) / WAVES : 0;
+  const int first = turns > 0 ? pg0 + wave : s.first_page;
+  int ids = table[first + (lane < turns ? lane : 0) * WAVES];
+
+  // this lane's column of each of the NC blocks of 16: a row of the step and a head (a column past the last reads the last)
+  uint4 qraw[NC][QK];
   int pos[NC], lo[NC];
 #pragma unroll
   for (int b = 0; b < NC; ++b) {
     const int col = col0 + 16 * b + n;
     const bool real = col < cols;
-    const int row = real ? col / a.group : 0, hig = real ? col % a.group : 0;
+    const int at = real ? col : cols - 1, row = at / a.group, hig = at % a.group;
     pos[b] = real ? s.start + row : -1;
     lo[b] = a.window > 0 && pos[b] - a.window + 1 > 0 ? pos[b] - a.window + 1 : 0;
     const bf16_t* src = a.q + (size_t)(s.row0 + row) * a.ldq + (size_t)(kvh * a.group + hig) * HD;
@@ -158,10 +193,7 @@ __global__ __launch_bounds__(WAVES* WAVE) void attn_decode_kernel(AttnQ8 a) {
 #pragma unroll
       for (int m = 0; m < 2; ++m) {
         const int piece = 4 * j + g;
-        uint4 u = *(const uint4*)(src + (piece < PIECES ? piece * 16 + m * 8 : 0));
-        if (!real || piece >= PIECES) u = make_uint4(0, 0, 0, 0);
-        else u = make_uint4(u.x ^ a.flip, u.y ^ a.flip, u.z ^ a.flip, u.w ^ a.flip);
-        qf[b][2 * j + m] = __builtin_bit_cast(bf16x8_t, u);
+        qraw[b][2 * j + m] = *(const uint4*)(src + (piece < PIECES ? piece * 16 + m * 8 : 0));
       }
   }
   f32x4_t o[NC][PIECES];
@@ -173,36 +205,22 @@ __global__ __launch_bounds__(WAVES* WAVE) void attn_decode_kernel(AttnQ8 a) {
 #pragma unroll
     for (int c = 0; c < PIECES; ++c) o[b][c] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
   }
-
-  const int32_t* table = a.page_table + (size_t)s.slot * a.max_pages;
-  const size_t head = (size_t)kvh * q8_head_bytes(HD);
-  // the numbers of this wave's pages, 64 at a time, one a lane
-  int ids = 0, ids_from = -1;
-  auto page_id = [&](int k) {                          // the wave's k-th page
-    const int from = k & ~63;
-    if (from != ids_from) {
-      const int pg = pg0 + wave + (from + lane) * WAVES;
-      ids = table[pg < pg1 ? pg : pg0];
-      ids_from = from;
-    }
-    return __builtin_amdgcn_readlane(ids, k & 63);
-  };
-  auto fetch = [&](PageRegs& p, int id) {
-    const bool ok = id >= 0 && id < a.n_pages;         // a hole reads page 0 and counts nothing
-    fetch_page(p, (const uint8_t*)uniform_ptr(a.cache + (size_t)(ok ? id : 0) * a.page_stride + head), lane);
-    return ok;
+  bf16x8_t qf[NC][QK];
+  auto queries = [&]() {
+#pragma unroll
+    for (int b = 0; b < NC; ++b)
+#pragma unroll
+      for (int j = 0; j < QK; ++j) {
+        // pieces beyond the head count as zero (the keys' lanes then hold bytes of the next piece, never NaN)
+        const bool ok = PIECES % 4 == 0 || 4 * (j / 2) + g < PIECES;
+        const uint4 u = qraw[b][j];
+        qf[b][j] = __builtin_bit_cast(bf16x8_t, ok ? make_uint4(u.x ^ a.flip, u.y ^ a.flip, u.z ^ a.flip, u.w ^ a.flip) : make_uint4(0, 0, 0, 0));
+      }
   };
 
-  const int turns = pg1 - pg0 > wave ? (pg1 - pg0 - wave + WAVES - 1) / WAVES : 0;
-  PageRegs cur;
-  bool cur_ok = false;
-  if (turns > 0) cur_ok = fetch(cur, page_id(0));
-  for (int k = 0; k < turns; ++k) {
-    PageRegs next;
-    bool next_ok = false;
-    if (k + 1 < turns) next_ok = fetch(next, page_id(k + 1));
-    if (cur_ok) {
-      const int key0 = (pg0 + wave + k * WAVES) * Q8_PAGE;
+  const uint8_t* head = a.cache + (size_t)kvh * q8_head_bytes(HD);
+
+  auto page = [&](PageRegs& cur, int key0) {
       f32x4_t sc[NC][4];
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
@@ -222,18 +240,10 @@ __global__ __launch_bounds__(WAVES* WAVE) void attn_decode_kernel(AttnQ8 a) {
         }
       }
       // element r of sc[b][t] is key  key0 + 16 t + 4 g + r  of column n
-      if (key0 + Q8_PAGE > s.len) {                    // tokens that the sequence does not hold: their bytes are anybody's
-#pragma unroll
-        for (int c = 0; c < PIECES; ++c) {
-          const int k0 = s.len - key0 - 4 * g;
-          cur.v[c] = make_uint4(first_bytes(cur.v[c].x, k0), first_bytes(cur.v[c].y, k0 - 16), first_bytes(cur.v[c].z, k0 - 32),
-                                first_bytes(cur.v[c].w, k0 - 48));
-        }
-      }
+      const bool mask = key0 + Q8_PAGE - 1 > s.start || a.window > 0;
       bf16x8_t pf[NC][2];
 #pragma unroll
       for (int b = 0; b < NC; ++b) {
-        const bool mask = key0 + Q8_PAGE - 1 > s.start || a.window > 0;
         if (mask) {
 #pragma unroll
           for (int t = 0; t < 4; ++t)
@@ -248,33 +258,43 @@ __global__ __launch_bounds__(WAVES* WAVE) void attn_decode_kernel(AttnQ8 a) {
         for (int t = 0; t < 4; ++t)
 #pragma unroll
           for (int r = 0; r < 4; ++r) mx = fmaxf(mx, sc[b][t][r]);
-        mx = fmaxf(mx, __shfl_xor(mx, 16, WAVE));
-        mx = fmaxf(mx, __shfl_xor(mx, 32, WAVE));
-        const float m_new = fmaxf(m[b], mx);
-        const float off = m_new == -INFINITY ? 0.f : -m_new * a.scale_log2e;
-        if (__any(m_new != m[b])) {
-          const float keep = m[b] == -INFINITY ? 0.f : fast_exp2(fmaf(m[b], a.scale_log2e, off));
+        mx = max_32(max_16(mx));
+        if (__any(has_grown(mx, m[b], a.scale_log2e))) {
+          const float m_new = fmaxf(m[b], mx);
+          const float keep = m[b] == -INFINITY ? 0.f : fast_exp2((m[b] - m_new) * a.scale_log2e);
           l[b] *= keep;
 #pragma unroll
           for (int c = 0; c < PIECES; ++c) o[b][c] *= keep;
           m[b] = m_new;
         }
+        const float off = m[b] == -INFINITY ? 0.f : -m[b] * a.scale_log2e;
         float p[16];
 #pragma unroll
         for (int t = 0; t < 4; ++t)
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            const float e = mask && sc[b][t][r] == -INFINITY ? 0.f : fast_exp2(fmaf(sc[b][t][r], a.scale_log2e, off));
+            const float e = fast_exp2(fmaf(sc[b][t][r], a.scale_log2e, off));       // 0 where the score is -inf
             l[b] += e;
             // the value's power of two goes into the probability: exact, and its own bits are at hand
             const uint32_t w = t == 0 ? cur.vs.x : (t == 1 ? cur.vs.y : (t == 2 ? cur.vs.z : cur.vs.w));
-            const float f = q8_scale((w >> (8 * r)) & 255u);
-            p[4 * t + r] = mask && sc[b][t][r] == -INFINITY ? 0.f : e * f;
+            p[4 * t + r] = e * q8_scale((w >> (8 * r)) & 255u);
           }
+        if (mask) {                                    // the power of a token that nobody sees may be anything
+#pragma unroll
+          for (int i = 0; i < 16; ++i) p[i] = sc[b][i >> 2][i & 3] == -INFINITY ? 0.f : p[i];
+        }
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
           for (int e = 0; e < 8; ++e) pf[b][h][e] = (__bf16)p[8 * h + e];
+      }
+      if (key0 + Q8_PAGE > s.len) {                    // tokens that the sequence does not hold: their bytes are anybody's
+#pragma unroll
+        for (int c = 0; c < PIECES; ++c) {
+          const int k0 = s.len - key0 - 4 * g;
+          cur.v[c] = make_uint4(first_bytes(cur.v[c].x, k0), first_bytes(cur.v[c].y, k0 - 16), first_bytes(cur.v[c].z, k0 - 32),
+                                first_bytes(cur.v[c].w, k0 - 48));
+        }
       }
 #pragma unroll
       for (int c = 0; c < PIECES; ++c) {
@@ -285,9 +305,32 @@ __global__ __launch_bounds__(WAVES* WAVE) void attn_decode_kernel(AttnQ8 a) {
           o[b][c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v1, pf[b][1], o[b][c], 0, 0, 0);
         }
       }
+  };
+
+  // two places in registers, one filling while the other is used
+  for (int k0 = 0; k0 < turns; k0 += 64) {
+    const int pg = first + k0 * WAVES;
+    const int here = turns - k0 < 64 ? turns - k0 : 64;
+    if (k0 > 0) ids = table[pg + (lane < here ? lane : 0) * WAVES];
+    bool real[2];
+    PageRegs regs[2];
+    auto fetch = [&](int k, int which) {
+      const int id = __builtin_amdgcn_readlane(ids, k < here ? k : 0);
+      real[which] = k < here && id >= 0 && id < a.n_pages;             // a hole counts nothing
+      fetch_page(regs[which], (const uint8_t*)uniform_ptr(head + (size_t)(real[which] ? id : 0) * a.page_stride),
+                 real[which] ? (int)q8_head_bytes(HD) : 0, lane);
+    };
+    fetch(0, 0);
+    if (k0 == 0) {
+      __builtin_amdgcn_sched_barrier(0);               // the queries are not waited for before the first page is asked for
+      queries();
     }
-    cur = next;
-    cur_ok = next_ok;
+    for (int k = 0; k < here; k += 2) {
+      fetch(k + 1, 1);
+      if (real[0]) page(regs[0], (pg + k * WAVES) * Q8_PAGE);
+      fetch(k + 2, 0);
+      if (real[1]) page(regs[1], (pg + (k + 1) * WAVES) * Q8_PAGE);
+    }
   }
 
   // the waves' results meet in LDS: element 4 g + r of o[b][c] is element 16 c + 4 g + r of the head, of column n
@@ -354,17 +397,31 @@ __global__ __launch_bounds__(WAVE) void attn_combine_kernel(AttnQ8 a) {
   const int per = (s.n_pages + used - 1) / used;
   const int filled = (s.n_pages + per - 1) / per;      // blocks that were given pages
   float M = -INFINITY;
-  for (int i = 0; i < filled; ++i) M = fmaxf(M, base[(size_t)i * PART_ROW + HD]);
+  for (int i = lane; i < filled; i += WAVE) M = fmaxf(M, base[(size_t)i * PART_ROW + HD]);
+  M = wave_max(M);
   constexpr int NE = (HD + WAVE - 1) / WAVE;
   float L = 0.f, acc[NE];
 #pragma unroll
   for (int e = 0; e < NE; ++e) acc[e] = 0.f;
-  for (int i = 0; i < filled; ++i) {
-    const float* p = base + (size_t)i * PART_ROW;
-    const float mm = p[HD], f = mm == -INFINITY ? 1.f : exp2f((mm - M) * a.scale_log2e);     // -inf: zeros, or NaN
-    L = fmaf(f, p[HD + 1], L);
+  // eight results at a time are asked for at once; what lies past the last is the last again, with no weight
+  for (int i0 = 0; i0 < filled; i0 += 8) {
+    float mm[8], ll[8], v[8][NE];
 #pragma unroll
-    for (int e = 0; e < NE; ++e) acc[e] = fmaf(f, p[e * WAVE + lane < HD ? e * WAVE + lane : 0], acc[e]);
+    for (int i = 0; i < 8; ++i) {
+      const float* p = base + (size_t)(i0 + i < filled ? i0 + i : filled - 1) * PART_ROW;
+      mm[i] = p[HD];
+      ll[i] = p[HD + 1];
+#pragma unroll
+      for (int e = 0; e < NE; ++e) v[i][e] = p[e * WAVE + lane < HD ? e * WAVE + lane : 0];
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (i0 + i < filled) {
+        const float f = mm[i] == -INFINITY ? 1.f : exp2f((mm[i] - M) * a.scale_log2e);       // -inf: zeros, or NaN
+        L = fmaf(f, ll[i], L);
+#pragma unroll
+        for (int e = 0; e < NE; ++e) acc[e] = fmaf(f, v[i][e], acc[e]);
+      }
   }
   const float inv = L == 0.f ? 0.f : 1.0f / L;
 #pragma unroll
@@ -379,226 +436,233 @@ __global__ __launch_bounds__(WAVE) void attn_combine_kernel(AttnQ8 a) {
 // of two: exact), the next page's bytes are on their way meanwhile, and the two places in LDS are used in turn, so that
 // a page costs one barrier.  Scores are kept transposed (keys x columns): a lane owns a column.
 #define PF_WAVES 4
+#define PF_EU (HD <= 128 ? 2 : 1)           // waves a SIMD that the registers are to allow
 #define DT ((HD + 31) / 32)                 // tiles of 32 elements of the result
 #define KS (HD / 16)                        // steps of 16 along the head
 #define LDS_K (Q8_PAGE * HD * 2)            // [element / 8][token][8 elements]
 #define LDS_V (4 * 2 * DT * 32 * 16)        // [t][h][element][8 tokens: 16 t + 8 a + 4 h + r]
-#define NPC ((4 * HD + 255) / 256)          // 16-byte pieces of a page's keys (of its values) a thread brings
 
-template <int CW>
-__global__ __launch_bounds__(PF_WAVES* WAVE) void attn_prefill_kernel(AttnQ8 a, int tokens, int n_tiles) {
+__global__ __launch_bounds__(PF_WAVES* WAVE) __attribute__((amdgpu_waves_per_eu(PF_EU))) void attn_prefill_kernel(AttnQ8 a, int tokens) {
   extern __shared__ __attribute__((aligned(16))) char pf_lds[];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5;
-  // Late tiles see more keys than early ones: tiles are dealt longest first, 256 blocks (one a compute unit) at a time,
-  // every other time in reverse, so that the blocks that share a unit add up to about the same number of pages.
+  const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  // Late tiles see more keys than early ones: every sequence's tiles are dealt from its last one on, 256 blocks (one a
+  // compute unit) at a time, every other time in reverse, so that the blocks that share a unit add up to about the same
+  // number of pages and the launch ends with short ones.
   const int total = gridDim.x, width = a.n_seq * a.n_kv;
   const int turn = blockIdx.x >> 8, in_turn = total - (turn << 8) < 256 ? total - (turn << 8) : 256;
   const int place = turn & 1 ? (turn << 8) + in_turn - 1 - (blockIdx.x & 255) : blockIdx.x;
-  const int tile = n_tiles - 1 - place / width, kvh = place % a.n_kv, seq = place % width / a.n_kv;
+  const int kvh = place % a.n_kv, seq = place % width / a.n_kv;
   const Span s = span_of(a, seq);
-  const int t0 = tile * tokens;
-  if (t0 >= s.rows) return;
+  const int tile = (s.rows + tokens - 1) / tokens - 1 - place / width, t0 = tile * tokens;
+  if (tile < 0) return;
   const int t1 = t0 + tokens < s.rows ? t0 + tokens : s.rows;        // the block's rows of the sequence
   const int lo_b = a.window > 0 && s.start + t0 - a.window + 1 > 0 ? s.start + t0 - a.window + 1 : 0;
   const int pg_lo = lo_b / Q8_PAGE;
   int pg_hi = (s.start + t1 - 1) / Q8_PAGE;
   if (pg_hi >= a.max_pages) pg_hi = a.max_pages - 1;
 
-  int pos[CW], lo[CW], trow[CW], hig[CW];
-  bf16x8_t qf[CW][KS];
+  // this lane's column: a row of the sequence and a head (one past the last reads the block's first row and counts nothing)
+  const int col = wave * 32 + (lane & 31), trow = t0 + col / a.group, hig = col % a.group;
+  const bool mine = trow < t1 && col < tokens * a.group;
+  const int pos = mine ? s.start + trow : -1;
+  const int lo = a.window > 0 && pos - a.window + 1 > 0 ? pos - a.window + 1 : 0;
+  bf16x8_t qf[KS];
+  {
+    const bf16_t* src = a.q + (size_t)(s.row0 + (mine ? trow : t0)) * a.ldq + (size_t)(kvh * a.group + hig) * HD + half * 8;
+    uint4 u[KS];
 #pragma unroll
-  for (int b = 0; b < CW; ++b) {
-    const int col = (wave * CW + b) * 32 + (lane & 31);
-    const int t = t0 + col / a.group;
-    const bool real = t < t1 && col < tokens * a.group;
-    trow[b] = real ? t : -1;
-    hig[b] = col % a.group;
-    pos[b] = real ? s.start + t : -1;
-    lo[b] = a.window > 0 && pos[b] - a.window + 1 > 0 ? pos[b] - a.window + 1 : 0;
-    const bf16_t* src = a.q + (size_t)(s.row0 + (real ? t : t0)) * a.ldq + (size_t)(kvh * a.group + hig[b]) * HD;
+    for (int k = 0; k < KS; ++k) u[k] = *(const uint4*)(src + k * 16);
 #pragma unroll
-    for (int k = 0; k < KS; ++k) {
-      uint4 u = *(const uint4*)(src + k * 16 + half * 8);
-      u = real ? make_uint4(u.x ^ a.flip, u.y ^ a.flip, u.z ^ a.flip, u.w ^ a.flip) : make_uint4(0, 0, 0, 0);
-      qf[b][k] = __builtin_bit_cast(bf16x8_t, u);
-    }
+    for (int k = 0; k < KS; ++k) qf[k] = __builtin_bit_cast(bf16x8_t, make_uint4(u[k].x ^ a.flip, u[k].y ^ a.flip, u[k].z ^ a.flip, u[k].w ^ a.flip));
   }
-  // the positions that the wave's columns span
-  const int wc0 = wave * CW * 32;
-  const int wt0 = t0 + wc0 / a.group;
-  int wt1 = t0 + (wc0 + CW * 32 - 1) / a.group;
-  wt1 = wt1 < t1 - 1 ? wt1 : t1 - 1;
-  const bool wave_real = wt0 < t1 && wc0 < tokens * a.group;
-  const int w_min = s.start + wt0, w_max = s.start + wt1;
-  const int w_lo_min = a.window > 0 && w_min - a.window + 1 > 0 ? w_min - a.window + 1 : 0;
-  const int w_lo_max = a.window > 0 && w_max - a.window + 1 > 0 ? w_max - a.window + 1 : 0;
+  // pages up to position all_see and from any_lo on are seen whole by every column of the wave: they need no mask; pages
+  // behind last_pos and before first_lo by none
+  const int c0 = wave * 32, c1 = c0 + 31 < tokens * a.group - 1 ? c0 + 31 : tokens * a.group - 1;
+  const int all_see = s.start + t0 + c0 / a.group;
+  const int last_pos = s.start + (t0 + c1 / a.group < t1 - 1 ? t0 + c1 / a.group : t1 - 1);
+  const int any_lo = a.window > 0 && last_pos - a.window + 1 > 0 ? last_pos - a.window + 1 : 0;
+  const int first_lo = a.window > 0 && all_see - a.window + 1 > 0 ? all_see - a.window + 1 : 0;
+  const bool some = c0 < tokens * a.group && t0 + c0 / a.group < t1;
 
-  f32x16_t o[CW][DT];
-  float m[CW], l[CW];
+  f32x16_t o[DT];
+  float m = -INFINITY, l = 0.f;
 #pragma unroll
-  for (int b = 0; b < CW; ++b) {
-    m[b] = -INFINITY;
-    l[b] = 0.f;
+  for (int d = 0; d < DT; ++d)
 #pragma unroll
-    for (int d = 0; d < DT; ++d)
-#pragma unroll
-      for (int v = 0; v < 16; ++v) o[b][d][v] = 0.f;
-  }
+    for (int v = 0; v < 16; ++v) o[d][v] = 0.f;
 
   const int32_t* table = a.page_table + (size_t)s.slot * a.max_pages;
-  const size_t head = (size_t)kvh * q8_head_bytes(HD);
-  uint4 rk[NPC], rv[NPC], rvs[NPC];
-  uint32_t rks[NPC];
-  bool r_ok = false;
-  auto fetch = [&](int pg) {
-    const int id = table[pg];
-    r_ok = id >= 0 && id < a.n_pages;
-    const uint8_t* p = a.cache + (size_t)(r_ok ? id : 0) * a.page_stride + head;
-#pragma unroll
-    for (int i = 0; i < NPC; ++i) {
-      int c = tid + i * 256;
-      if (NPC * 256 != 4 * HD && c >= 4 * HD) c = 0;
-      rk[i] = *(const uint4*)(p + c * 16);
-      rv[i] = *(const uint4*)(p + Q8_PAGE * HD + c * 16);
-      rks[i] = p[2 * Q8_PAGE * HD + (c & 15) * 4 + (c >> 4) / PIECES];
-      rvs[i] = *(const uint4*)(p + 2 * Q8_PAGE * HD + 64 + ((c >> 4) & 3) * 16);
-    }
+  const uint8_t* head = a.cache + (size_t)kvh * q8_head_bytes(HD);
+  // The 8 * HD pieces of a page, its keys' and then its values', are shared out over the threads: a wave's 64 are of one kind.
+  constexpr int THREADS = PF_WAVES * WAVE, NP = (8 * HD + THREADS - 1) / THREADS;
+  struct Raw {
+    uint4 piece[NP];
+    uint32_t ks;                             // the scales of the keys of tokens 16 t + (lane % 16)
+    uint4 vs;                                // the scales of the values of tokens 16 t + 4 (lane / 16) + r
+    int there;                               // whether there is such a page
   };
-  auto stage = [&](char* lds, int key0) {
-    const bool tail = key0 + Q8_PAGE > s.len;
+  int id = table[pg_lo <= pg_hi ? pg_lo : 0];            // the number of the page that is asked for next, known a page ahead
+  auto fetch = [&](Raw& x, int pg) {                     // pages are asked for in order
+    const int after = table[pg < pg_hi ? pg + 1 : pg_hi];
+    x.there = id >= 0 && id < a.n_pages;
+    const uint8_t* p = head + (size_t)(x.there ? id : 0) * a.page_stride;
+    x.ks = *(const uint32_t*)(p + 2 * Q8_PAGE * HD + (lane & 15) * 4);
+    x.vs = *(const uint4*)(p + 2 * Q8_PAGE * HD + 64 + (lane >> 4) * 16);
 #pragma unroll
-    for (int i = 0; i < NPC; ++i) {
-      const int c = tid + i * 256;
-      if (NPC * 256 != 4 * HD && c >= 4 * HD) break;
-      // keys: piece p of token 16 t + (c % 16)
-      const int tp = c >> 4, t = tp / PIECES, p = tp % PIECES, token = 16 * t + (c & 15);
-      const float ksc = q8_scale(rks[i]);
-      *(bf16x8_t*)(lds + ((2 * p) * Q8_PAGE + token) * 16) = eight(rk[i].x, rk[i].y, ksc);
-      *(bf16x8_t*)(lds + ((2 * p + 1) * Q8_PAGE + token) * 16) = eight(rk[i].z, rk[i].w, ksc);
-      // values: element d, tokens 16 t + 4 g + r
-      const int g = (c >> 4) & 3, d = (c >> 6) * 16 + (c & 15);
-      char* dst = lds + LDS_K + ((g & 1) * (DT * 32) + d) * 16 + (g >> 1) * 8;
+    for (int i = 0; i < NP; ++i) {
+      const int w0 = i * THREADS + wave * WAVE;
+      x.piece[i] = *(const uint4*)(p + ((i + 1) * THREADS <= 8 * HD || w0 < 8 * HD ? w0 * 16 : 0) + lane * 16);
+    }
+    id = after;
+  };
+  auto stage = [&](Raw& x, char* lds, int key0) {
+    // tokens that the sequence does not hold, or a page that is not there: zeros, with a power that leaves them zeros
+    const int left = x.there ? s.len - key0 : 0;
+    if (left < Q8_PAGE) {
+      const int n = left - 4 * (lane >> 4);
+      x.vs = make_uint4(first_bytes(x.vs.x, n), first_bytes(x.vs.y, n - 16), first_bytes(x.vs.z, n - 32), first_bytes(x.vs.w, n - 48));
 #pragma unroll
-      for (int t4 = 0; t4 < 4; ++t4) {
-        uint32_t w = t4 == 0 ? rv[i].x : (t4 == 1 ? rv[i].y : (t4 == 2 ? rv[i].z : rv[i].w));
-        uint32_t sc = t4 == 0 ? rvs[i].x : (t4 == 1 ? rvs[i].y : (t4 == 2 ? rvs[i].z : rvs[i].w));
-        if (tail) {          // tokens that the sequence does not hold: zeros, with a power that leaves them zeros
-          const int left = s.len - key0 - 16 * t4 - 4 * g;
-          w = first_bytes(w, left);
-          sc = first_bytes(sc, left);
+      for (int i = 0; i < NP; ++i)
+        if ((i + 1) * THREADS > 4 * HD && i * THREADS + wave * WAVE >= 4 * HD)
+          x.piece[i] = make_uint4(first_bytes(x.piece[i].x, n), first_bytes(x.piece[i].y, n - 16), first_bytes(x.piece[i].z, n - 32), first_bytes(x.piece[i].w, n - 48));
+    }
+#pragma unroll
+    for (int i = 0; i < NP; ++i) {
+      const int w0 = i * THREADS + wave * WAVE;
+      const uint4 u = x.piece[i];
+      if ((i + 1) * THREADS <= 4 * HD || w0 < 4 * HD) {
+        // piece p of token 16 t + (lane % 16)
+        const int tp = w0 / 16 + (lane >> 4), t = tp / PIECES, p = tp % PIECES, token = 16 * t + (lane & 15);
+        const float ksc = q8_scale((x.ks >> (8 * t)) & 255u);
+        *(bf16x8_t*)(lds + ((2 * p) * Q8_PAGE + token) * 16) = eight(u.x, u.y, ksc);
+        *(bf16x8_t*)(lds + ((2 * p + 1) * Q8_PAGE + token) * 16) = eight(u.z, u.w, ksc);
+      } else if ((i + 1) * THREADS <= 8 * HD || w0 < 8 * HD) {
+        // element d, tokens 16 t + 4 g + r
+        const int d = (w0 / 64 - HD / 16) * 16 + (lane & 15), g = lane >> 4;
+        char* dst = lds + LDS_K + ((g & 1) * (DT * 32) + d) * 16 + (g >> 1) * 8;
+#pragma unroll
+        for (int t4 = 0; t4 < 4; ++t4) {
+          const uint32_t w = t4 == 0 ? u.x : (t4 == 1 ? u.y : (t4 == 2 ? u.z : u.w));
+          const uint32_t sc = t4 == 0 ? x.vs.x : (t4 == 1 ? x.vs.y : (t4 == 2 ? x.vs.z : x.vs.w));
+          // each of a word's four has a power of its own: convert a pair with either and keep the half that is meant
+          const uint32_t a0 = pair_of<false>(w, q8_scale(sc & 255u)), a1 = pair_of<false>(w, q8_scale((sc >> 8) & 255u));
+          const uint32_t b0 = pair_of<true>(w, q8_scale((sc >> 16) & 255u)), b1 = pair_of<true>(w, q8_scale(sc >> 24));
+          *(uint2*)(dst + t4 * (2 * DT * 32 * 16)) = make_uint2((a0 & 0xffffu) | (a1 & 0xffff0000u), (b0 & 0xffffu) | (b1 & 0xffff0000u));
         }
-        // two of a word's four have one power each: convert the pair with either and keep the half that is meant
-        const uint32_t a0 = pair_of<false>(w, q8_scale(sc & 255u)), a1 = pair_of<false>(w, q8_scale((sc >> 8) & 255u));
-        const uint32_t b0 = pair_of<true>(w, q8_scale((sc >> 16) & 255u)), b1 = pair_of<true>(w, q8_scale(sc >> 24));
-        *(uint2*)(dst + t4 * (2 * DT * 32 * 16)) = make_uint2((a0 & 0xffffu) | (a1 & 0xffff0000u), (b0 & 0xffffu) | (b1 & 0xffff0000u));
       }
     }
   };
 
-  constexpr int LDS_PAGE = LDS_K + LDS_V;
-  bool ok = false;
-  if (pg_lo <= pg_hi) {
-    fetch(pg_lo);
-    stage(pf_lds, pg_lo * Q8_PAGE);
-    ok = r_ok;
-  }
-  __syncthreads();
-  for (int pg = pg_lo; pg <= pg_hi; ++pg) {
-    if (pg < pg_hi) fetch(pg + 1);
+  // One page: its bytes lie in LDS; the next page's are in `soon` (asked for a page ago) and go there after it, those of
+  // the page after that are asked for into `later`: a trip to memory takes longer than a page.
+  int ok = 0;
+  auto page = [&](int pg, Raw& soon, Raw& later) {
+    fetch(later, pg + 2);
     const int key0 = pg * Q8_PAGE;
-    const char* lds = pf_lds + ((pg - pg_lo) & 1) * LDS_PAGE;
-    if (ok && wave_real && key0 <= w_max && key0 + Q8_PAGE - 1 >= w_lo_min) {
-      f32x16_t sc[CW][2];
+    const char* lds = pf_lds + ((pg - pg_lo) & 1) * (LDS_K + LDS_V);
+    if (ok && some && key0 <= last_pos && key0 + Q8_PAGE > first_lo) {
+      f32x16_t sc[2];
 #pragma unroll
-      for (int kt = 0; kt < 2; ++kt) {
+      for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
-        for (int b = 0; b < CW; ++b)
+        for (int v = 0; v < 16; ++v) sc[kt][v] = 0.f;
+      // the operands of four steps are asked for together, and the two tiles of keys take turns: nothing waits for the
+      // instruction before it
 #pragma unroll
-          for (int v = 0; v < 16; ++v) sc[b][kt][v] = 0.f;
+      for (int k0 = 0; k0 < KS; k0 += 4) {
+        bf16x8_t kf[4][2];
 #pragma unroll
-        for (int k = 0; k < KS; ++k) {
-          const bf16x8_t kf = *(const bf16x8_t*)(lds + ((2 * k + half) * Q8_PAGE + kt * 32 + (lane & 31)) * 16);
+        for (int k = k0; k < KS && k < k0 + 4; ++k)
 #pragma unroll
-          for (int b = 0; b < CW; ++b) sc[b][kt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, qf[b][k], sc[b][kt], 0, 0, 0);
-        }
+          for (int kt = 0; kt < 2; ++kt) kf[k - k0][kt] = *(const bf16x8_t*)(lds + ((2 * k + half) * Q8_PAGE + kt * 32 + (lane & 31)) * 16);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int k = k0; k < KS && k < k0 + 4; ++k)
+#pragma unroll
+          for (int kt = 0; kt < 2; ++kt) sc[kt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[k - k0][kt], qf[k], sc[kt], 0, 0, 0);
       }
-      // element v of sc[b][kt] is key  key0 + 32 kt + 8 (v / 4) + 4 half + v % 4  of the lane's column
-      const bool mask = key0 + Q8_PAGE - 1 > w_min || key0 < w_lo_max;
-      bf16x8_t pf[CW][4];
-#pragma unroll
-      for (int b = 0; b < CW; ++b) {
-        if (mask) {
-#pragma unroll
-          for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-            for (int v = 0; v < 16; ++v) {
-              const int key = key0 + kt * 32 + 8 * (v >> 2) + 4 * half + (v & 3);
-              sc[b][kt][v] = key <= pos[b] && key >= lo[b] ? sc[b][kt][v] : -INFINITY;
-            }
-        }
-        float mx = -INFINITY;
-#pragma unroll
-        for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-          for (int v = 0; v < 16; ++v) mx = fmaxf(mx, sc[b][kt][v]);
-        mx = fmaxf(mx, __shfl_xor(mx, 32, WAVE));
-        const float m_new = fmaxf(m[b], mx);
-        const float off = m_new == -INFINITY ? 0.f : -m_new * a.scale_log2e;
-        if (__any(m_new != m[b])) {
-          const float keep = m[b] == -INFINITY ? 0.f : fast_exp2(fmaf(m[b], a.scale_log2e, off));
-          l[b] *= keep;
-#pragma unroll
-          for (int d = 0; d < DT; ++d)
-#pragma unroll
-            for (int v = 0; v < 16; ++v) o[b][d][v] *= keep;
-          m[b] = m_new;
-        }
+      // element v of sc[kt] is key  key0 + 32 kt + 8 (v / 4) + 4 half + v % 4  of the lane's column
+      if (key0 + Q8_PAGE - 1 > all_see || key0 < any_lo) {
 #pragma unroll
         for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
           for (int v = 0; v < 16; ++v) {
-            const float e = fast_exp2(fmaf(sc[b][kt][v], a.scale_log2e, off));
-            l[b] += e;
-            pf[b][2 * kt + (v >> 3)][v & 7] = (__bf16)e;
+            const int key = key0 + kt * 32 + 8 * (v >> 2) + 4 * half + (v & 3);
+            sc[kt][v] = key <= pos && key >= lo ? sc[kt][v] : -INFINITY;
           }
       }
-      // element e of pf[b][t] is key  16 t + 8 (e / 4) + 4 half + e % 4: the values lie in LDS in that order
+      float mx = -INFINITY;
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) mx = fmaxf(mx, sc[kt][v]);
+      mx = max_32(mx);
+      if (__any(has_grown(mx, m, a.scale_log2e))) {
+        const float m_new = fmaxf(m, mx);
+        const float keep = m == -INFINITY ? 0.f : fast_exp2((m - m_new) * a.scale_log2e);
+        l *= keep;
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+          for (int v = 0; v < 16; ++v) o[d][v] *= keep;
+        m = m_new;
+      }
+      const float off = m == -INFINITY ? 0.f : -m * a.scale_log2e;
+      bf16x8_t pf[4];
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) {
+          const float e = fast_exp2(fmaf(sc[kt][v], a.scale_log2e, off));
+          l += e;
+          pf[2 * kt + (v >> 3)][v & 7] = (__bf16)e;
+        }
+      // element e of pf[t] is key  16 t + 8 (e / 4) + 4 half + e % 4: the values lie in LDS in that order
 #pragma unroll
       for (int t = 0; t < 4; ++t)
 #pragma unroll
         for (int d = 0; d < DT; ++d) {
           const bf16x8_t vf = *(const bf16x8_t*)(lds + LDS_K + ((t * 2 + half) * (DT * 32) + d * 32 + (lane & 31)) * 16);
-#pragma unroll
-          for (int b = 0; b < CW; ++b) o[b][d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, pf[b][t], o[b][d], 0, 0, 0);
+          o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, pf[t], o[d], 0, 0, 0);
         }
     }
     if (pg < pg_hi) {
-      stage(pf_lds + ((pg - pg_lo + 1) & 1) * LDS_PAGE, key0 + Q8_PAGE);
-      ok = r_ok;
+      stage(soon, pf_lds + ((pg - pg_lo + 1) & 1) * (LDS_K + LDS_V), key0 + Q8_PAGE);
+      ok = soon.there;
     }
     __syncthreads();
+  };
+  if (pg_lo <= pg_hi) {                      // else the window begins behind the table: nothing to see
+    Raw x, y;
+    fetch(x, pg_lo);
+    fetch(y, pg_lo + 1);
+    stage(x, pf_lds, pg_lo * Q8_PAGE);
+    ok = x.there;
+    __syncthreads();
+    for (int pg = pg_lo; pg <= pg_hi; pg += 2) {
+      page(pg, y, x);
+      if (pg < pg_hi) page(pg + 1, x, y);
+    }
   }
+  l += __shfl_xor(l, 32, WAVE);
+  if (!mine) return;
+  const float inv = l == 0.f ? 0.f : 1.0f / l;
+  bf16_t* dst = a.out + (size_t)(s.row0 + trow) * a.ldo + (size_t)(kvh * a.group + hig) * HD;
 #pragma unroll
-  for (int b = 0; b < CW; ++b) {
-    l[b] += __shfl_xor(l[b], 32, WAVE);
-    if (trow[b] < 0) continue;
-    const float inv = l[b] == 0.f ? 0.f : 1.0f / l[b];
-    bf16_t* dst = a.out + (size_t)(s.row0 + trow[b]) * a.ldo + (size_t)(kvh * a.group + hig[b]) * HD;
+  for (int d = 0; d < DT; ++d)
 #pragma unroll
-    for (int d = 0; d < DT; ++d)
-#pragma unroll
-      for (int qd = 0; qd < 4; ++qd) {
-        const int e = d * 32 + 8 * qd + 4 * half;
-        if (e < HD) Elem<bf16_t>::store4(dst + e, o[b][d][4 * qd] * inv, o[b][d][4 * qd + 1] * inv, o[b][d][4 * qd + 2] * inv, o[b][d][4 * qd + 3] * inv);
-      }
-  }
+    for (int qd = 0; qd < 4; ++qd) {
+      const int e = d * 32 + 8 * qd + 4 * half;
+      if (e < HD) Elem<bf16_t>::store4(dst + e, o[d][4 * qd] * inv, o[d][4 * qd + 1] * inv, o[d][4 * qd + 2] * inv, o[d][4 * qd + 3] * inv);
+    }
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
 // What a launch looks like, from sizes that the host knows.  max_q_len and max_kv_len bound the sequences' rows and
 // lengths (a recorded launch passes the context's).
 struct Plan {
-  int tiled, nc, waves, chunks, splits, fill;
+  int tiled, nc, chunks, splits, fill;
 };
 static Plan plan_of(int n_seq, int n_heads, int n_kv, int max_q_len, int max_kv_len, int window) {
   Plan p = {};
@@ -609,9 +673,6 @@ static Plan plan_of(int n_seq, int n_heads, int n_kv, int max_q_len, int max_kv_
   p.nc = cols <= 16 ? 1 : (cols <= 32 ? 2 : 4);
   if (p.nc > NC_MOST) p.nc = NC_MOST;
   p.chunks = (int)((cols + 16 * p.nc - 1) / (16 * p.nc));
-  // the waves of a block must find room in LDS for their results: columns x (head + 2) floats each
-  p.waves = HD <= 64 ? 8 : 4;
-  while (p.waves > 1 && p.waves * 16 * p.nc * (HD + 2) * 4 > 128 * 1024) p.waves /= 2;
   int pages = (max_kv_len + Q8_PAGE - 1) / Q8_PAGE;
   if (window > 0) {
     const int seen = (window + max_q_len + Q8_PAGE - 2) / Q8_PAGE + 1;
@@ -620,7 +681,7 @@ static Plan plan_of(int n_seq, int n_heads, int n_kv, int max_q_len, int max_kv_
   const long long pairs = (long long)n_seq * n_kv * p.chunks;
   const int target = 512;
   p.fill = pairs >= target ? 1 : (int)((target + pairs - 1) / pairs);
-  const int by_wave = (pages + p.waves - 1) / p.waves, by_16 = (pages + 16 * p.waves - 1) / (16 * p.waves);
+  const int by_wave = (pages + WAVES - 1) / WAVES, by_16 = (pages + 16 * WAVES - 1) / (16 * WAVES);
   p.splits = p.fill < by_wave ? p.fill : by_wave;
   if (p.splits < by_16) p.splits = by_16;
   if (p.splits < 1) p.splits = 1;
@@ -636,23 +697,13 @@ extern "C" long long dlgo_attention_q8_scratch(int n_rows, int n_seq, int n_head
   return p.tiled || p.splits <= 1 ? 0 : (long long)n_rows * n_heads * p.splits * PART_ROW;
 }
 
-template <int NC, int WAVES>
-static hipError_t launch_decode(const AttnQ8& a, dim3 grid, hipStream_t stream) {
-  const int lds = WAVES * 16 * NC * (HD + 2) * 4;
-  hipError_t e = hipSuccess;
-  if (lds > 64 * 1024) e = hipFuncSetAttribute((const void*)attn_decode_kernel<NC, WAVES>, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
-  if (e == hipSuccess) hipLaunchKernelGGL((attn_decode_kernel<NC, WAVES>), grid, dim3(WAVES * WAVE), lds, stream, a);
-  return e;
-}
 template <int NC>
-static hipError_t launch_decode_waves(const AttnQ8& a, dim3 grid, hipStream_t stream) {
-  switch (a.waves) {
-    case 8: if constexpr (8 * 16 * NC * (HD + 2) * 4 <= 128 * 1024) return launch_decode<NC, 8>(a, grid, stream); else return hipErrorInvalidValue;
-    case 4: if constexpr (4 * 16 * NC * (HD + 2) * 4 <= 128 * 1024) return launch_decode<NC, 4>(a, grid, stream); else return hipErrorInvalidValue;
-    case 2: if constexpr (HD > 64) return launch_decode<NC, 2>(a, grid, stream); else return hipErrorInvalidValue;
-    case 1: if constexpr (HD > 128) return launch_decode<NC, 1>(a, grid, stream); else return hipErrorInvalidValue;
-  }
-  return hipErrorInvalidValue;
+static hipError_t launch_decode(const AttnQ8& a, dim3 grid, hipStream_t stream) {
+  const int lds = WAVES * COLS(NC) * (HD + 2) * 4;       // the waves' results
+  hipError_t e = hipSuccess;
+  if (lds > 64 * 1024) e = hipFuncSetAttribute((const void*)attn_decode_kernel<NC>, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+  if (e == hipSuccess) hipLaunchKernelGGL((attn_decode_kernel<NC>), grid, dim3(WAVES * WAVE), lds, stream, a);
+  return e;
 }
 
 extern "C" const char* dlgo_attention_q8(const void* q, int ldq, void* out, int ldo, int n_rows, int n_seq, int n_heads, int n_kv, int head_dim,
@@ -674,26 +725,24 @@ extern "C" const char* dlgo_attention_q8(const void* q, int ldq, void* out, int 
   const Plan p = plan_of(n_seq, n_heads, n_kv, max_q_len, max_kv_len, window);
   AttnQ8 a = {(const bf16_t*)q, (bf16_t*)out, part, cu_q, start_pos, slots, page_table, (const uint8_t*)cache, page_stride, ldq, ldo, n_rows, n_seq,
               n_heads, n_kv, n_heads / n_kv, n_slots, max_pages, n_pages, window > 0 ? window : 0,
-              (scale < 0 ? -scale : scale) * 1.44269504088896341f, scale < 0 ? 0x80008000u : 0u, p.splits, p.fill, p.waves};
+              (scale < 0 ? -scale : scale) * 1.44269504088896341f, scale < 0 ? 0x80008000u : 0u, p.splits, p.fill};
   hipError_t e = hipSuccess;
   if (p.tiled) {
-    constexpr int CW = HD <= 64 ? 2 : 1;
-    const int columns = PF_WAVES * 32 * CW, tokens = columns / a.group;
-    const int n_tiles = (max_q_len + tokens - 1) / tokens;
+    const int tokens = PF_WAVES * 32 / a.group, n_tiles = (max_q_len + tokens - 1) / tokens;
     const long long blocks = (long long)n_tiles * n_seq * n_kv;
     DLGO_REQUIRE(blocks < (1ll << 31), "attention_q8: too many rows at once");
     const int lds = 2 * (LDS_K + LDS_V);
-    if (lds > 64 * 1024) e = hipFuncSetAttribute((const void*)attn_prefill_kernel<CW>, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
-    if (e == hipSuccess) hipLaunchKernelGGL(attn_prefill_kernel<CW>, dim3((unsigned)blocks), dim3(PF_WAVES * WAVE), lds, stream, a, tokens, n_tiles);
+    if (lds > 64 * 1024) e = hipFuncSetAttribute((const void*)attn_prefill_kernel, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+    if (e == hipSuccess) hipLaunchKernelGGL(attn_prefill_kernel, dim3((unsigned)blocks), dim3(PF_WAVES * WAVE), lds, stream, a, tokens);
   } else {
     DLGO_REQUIRE(p.splits <= 65535, "attention_q8: sequences of %d tokens are too long", max_kv_len);
     const long long need = p.splits > 1 ? (long long)n_rows * n_heads * p.splits * PART_ROW : 0;
     DLGO_REQUIRE(need == 0 || (part && part_elems >= need && ((uintptr_t)part & 15) == 0), "attention_q8: scratch of %lld floats is needed, %lld given", need, part ? part_elems : 0ll);
     const dim3 grid((unsigned)(n_kv * p.chunks), (unsigned)n_seq, (unsigned)p.splits);
     e = hipErrorInvalidValue;
-    if (p.nc == 1) e = launch_decode_waves<1>(a, grid, stream);
-    if constexpr (NC_MOST >= 2) if (p.nc == 2) e = launch_decode_waves<2>(a, grid, stream);
-    if constexpr (NC_MOST >= 4) if (p.nc == 4) e = launch_decode_waves<4>(a, grid, stream);
+    if (p.nc == 1) e = launch_decode<1>(a, grid, stream);
+    if constexpr (NC_MOST >= 2) if (p.nc == 2) e = launch_decode<2>(a, grid, stream);
+    if constexpr (NC_MOST >= 4) if (p.nc == 4) e = launch_decode<4>(a, grid, stream);
     if (e == hipSuccess && p.splits > 1) {
       DLGO_LAUNCH_CHECK("attention_q8");
       hipLaunchKernelGGL(attn_combine_kernel, dim3((unsigned)(max_q_len * n_heads), (unsigned)n_seq), dim3(WAVE), 0, stream, a);
