@@ -21,11 +21,12 @@
 #define CHUNK 4096                       // elements of a row that a block takes, 16 a thread
 #define THREADS 256
 #define PER (CHUNK / THREADS)
+#define LOG2E 1.44269504088896340736
 
 struct Piece16 {
-  double sum;                            // of exp((x - max) / T) over the block's elements
+  double sum;                            // of exp((x - max) / T) over the part's elements (not where T = 0)
   float max;
-  int arg;                               // lowest index of the maximum, -1 if nothing was a number
+  int arg;                               // T = 0: lowest index of the maximum, -1 if nothing was a number; else 0
 };
 struct Choice {                          // what the first block of a sequence found, for the last kernel
   int accepted, row, draft_row, drawn;   // draft_row: -1 where nothing is taken away; drawn: the token if it is settled
@@ -49,33 +50,31 @@ struct Verify {
   Choice* choice;                        // [sequences]
   long long ldl, ldd;
   int n, d, vocab, parts, most;
+  int run, judge_run;                    // parts of a row that a block of the first (second) kernel takes in turn
 };
 
-// exp(x) for x <= 0 (or NaN, which counts as nothing): Cody and Waite's reduction to |r| <= ln 2 / 2 and the Taylor series
-// to r^12, whose remainder is below 2 * 10^-16 of the result.
-__device__ __forceinline__ double exp_neg(double x) {
-  x = fmax(x, -800.0);
-  const double k = rint(x * 1.4426950408889634074);
-  double r = fma(k, -0x1.62e42fee00000p-1, x);           // ln 2 in two parts, the first with 21 zero bits at its end
-  r = fma(k, -0x1.a39ef35793c76p-33, r);
-  double p = 1.0 / 479001600.0;
-  p = fma(p, r, 1.0 / 39916800.0);
-  p = fma(p, r, 1.0 / 3628800.0);
-  p = fma(p, r, 1.0 / 362880.0);
-  p = fma(p, r, 1.0 / 40320.0);
-  p = fma(p, r, 1.0 / 5040.0);
-  p = fma(p, r, 1.0 / 720.0);
-  p = fma(p, r, 1.0 / 120.0);
-  p = fma(p, r, 1.0 / 24.0);
-  p = fma(p, r, 1.0 / 6.0);
-  p = fma(p, r, 0.5);
-  p = fma(p, r, 1.0);
-  p = fma(p, r, 1.0);
-  return ldexp(p, (int)k);
+// 2^y for y <= 0: y is taken apart into a whole number (the addition of 1.5 * 2^52 leaves it in the sum's low bits) and a
+// rest of at most a half, whose power is the polynomial of degree 8 through the nine Chebyshev nodes of [-1/2, 1/2]: off
+// by at most 1.07 * 10^-12 of itself.  Below 2^-1000 (-inf and NaN among it) it is 2^-1000.
+__device__ __forceinline__ double exp2_neg(double y) {
+  y = fmax(y, -1000.0);
+  const double shifted = y + 0x1.8p52;
+  const double f = y - (shifted - 0x1.8p52);
+  double p = fma(1.3255224878668817e-06, f, 1.5310079402249296e-05);
+  p = fma(p, f, 0.00015403455852453838);
+  p = fma(p, f, 0.0013333450568000645);
+  p = fma(p, f, 0.009618129159402558);
+  p = fma(p, f, 0.05550410941205933);
+  p = fma(p, f, 0.2402265069581299);
+  p = fma(p, f, 0.6931471805459335);
+  p = fma(p, f, 1.0);
+  return __builtin_ldexp(p, (int)(uint32_t)__double_as_longlong(shifted));
 }
-// the weight of x in a row whose maximum is m: 1 for the maximum itself, infinite or not
-__device__ __forceinline__ double weight(float x, float m, double inv_t) {
-  return x == m ? 1.0 : exp_neg(((double)x - (double)m) * inv_t);
+// The weight exp((x - m) / T) of a logit in a row whose maximum is m, c = log2 e / T: 1 for the maximum itself, infinite or
+// not, and nothing at all for what lies 2^-1000 below it, -inf and NaN among it.
+__device__ __forceinline__ double weight(float x, float m, double c) {
+  const double y = ((double)x - (double)m) * c;
+  return x == m ? 1.0 : (y > -1000.0 ? exp2_neg(y) : 0.0);
 }
 
 __device__ __forceinline__ double wave_sum64(double v) {
@@ -83,7 +82,17 @@ __device__ __forceinline__ double wave_sum64(double v) {
   for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, WAVE);
   return v;
 }
-__device__ __forceinline__ void take_max(float& m, int& at, float m2, int at2) {
+// the sum over the lanes up to this one
+__device__ __forceinline__ double wave_running64(double v) {
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int o = 1; o < WAVE; o <<= 1) {
+    const double u = __shfl_up(v, o, WAVE);
+    if (lane >= o) v += u;
+  }
+  return v;
+}
+__device__ __forceinline__ void take_max(float& m, int& at, float m2, int at2) {        // the lowest index of equals
   if (at2 >= 0 && (at < 0 || m2 > m || (m2 == m && at2 < at))) {
     m = m2;
     at = at2;
@@ -98,36 +107,37 @@ __device__ __forceinline__ void wave_max_at(float& m, int& at) {
   }
 }
 
-// Sixteen elements of a row, four runs of four a thread (element 4 * (256 k + thread) + e of the block's part), with
-// nothing (NaN) past the row's end.
-__device__ __forceinline__ void load16(const float* row, int first, int vocab, float (&x)[PER]) {
-  const bool aligned = ((uintptr_t)row & 15) == 0;
-#pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    const int i = first + (k * THREADS + (int)threadIdx.x) * 4;
-    if (aligned && i + 3 < vocab) {
-      *(float4*)(x + 4 * k) = *(const float4*)(row + i);
-    } else {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) x[4 * k + e] = i + e < vocab ? row[i + e] : __uint_as_float(0x7fc00000u);
-    }
-  }
-}
+// four floats in a row in memory, at any float's address
+struct __attribute__((packed, aligned(4))) Four {
+  float x, y, z, w;
+};
 
-// Sixteen consecutive elements from `first` on.
-__device__ __forceinline__ void load_run(const float* row, int first, int vocab, float (&x)[PER]) {
-  const bool aligned = ((uintptr_t)row & 15) == 0;
+// Sixteen elements of a row, nothing (NaN) past the row's end: element k is `first` + at(k).  No load stands under a lane's
+// condition: a part that reaches past the end reads the last element in place of what is not there.
+template <typename At>
+__device__ __forceinline__ void load_part(const float* row, int first, int vocab, float (&x)[PER], At at) {
+  if (first + CHUNK <= vocab) {
 #pragma unroll
-  for (int k = 0; k < PER; k += 4) {
-    const int i = first + k;
-    if (aligned && i + 3 < vocab) {
-      *(float4*)(x + k) = *(const float4*)(row + i);
-    } else {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) x[k + e] = i + e < vocab ? row[i + e] : __uint_as_float(0x7fc00000u);
+    for (int k = 0; k < PER; k += 4) {
+      const Four f = *(const Four*)(row + first + at(k));
+      x[k] = f.x;
+      x[k + 1] = f.y;
+      x[k + 2] = f.z;
+      x[k + 3] = f.w;
     }
+  } else {
+#pragma unroll
+    for (int k = 0; k < PER; ++k) {
+      const int i = first + at(k);
+      x[k] = row[i < vocab ? i : vocab - 1];
+    }
+#pragma unroll
+    for (int k = 0; k < PER; ++k) x[k] = first + at(k) < vocab ? x[k] : __uint_as_float(0x7fc00000u);
   }
 }
+// four runs of four a thread: what 64 lanes load is 1 KB in a row
+__device__ __forceinline__ int in_runs(int k) { return ((k >> 2) * THREADS + (int)threadIdx.x) * 4 + (k & 3); }
+__device__ __forceinline__ void load16(const float* row, int first, int vocab, float (&x)[PER]) { load_part(row, first, vocab, x, in_runs); }
 
 // A sequence's drafts [c0, c1) whatever the numbers on the device are.
 __device__ __forceinline__ void drafts_of(const Verify& a, int seq, int& c0, int& c1) {
@@ -138,216 +148,264 @@ __device__ __forceinline__ void drafts_of(const Verify& a, int seq, int& c0, int
   if (c1 - c0 > a.most) c1 = c0 + a.most;
 }
 
-// grid: rows * parts.  Maximum, its index and the sum of a part of a row.
+__device__ __forceinline__ float max_of(const float (&x)[PER]) {
+  float m = -INFINITY;
+#pragma unroll
+  for (int k = 0; k < PER; ++k) m = fmaxf(m, x[k]);
+  return m;
+}
+
+// grid: rows * ceil(parts / run).  Maximum and sum (T = 0: its index) of `run` parts of a row one after the other, the next
+// one's elements on their way while this one's are summed.  A wave's sum stands on the wave's own maximum; one barrier a
+// part brings the four together.
 __global__ __launch_bounds__(THREADS) void verify_rows_kernel(Verify a) {
-  __shared__ float ms[THREADS / WAVE];
-  __shared__ int as[THREADS / WAVE];
-  __shared__ double ss[THREADS / WAVE];
-  const int row = blockIdx.x / a.parts, part = blockIdx.x % a.parts, wave = threadIdx.x / WAVE;
+  constexpr int NWV = THREADS / WAVE;
+  __shared__ float ms[2][NWV];
+  __shared__ int as[2][NWV];
+  __shared__ double ss[2][NWV];
+  const int runs = (a.parts + a.run - 1) / a.run;
+  const int row = blockIdx.x / runs, part0 = blockIdx.x % runs * a.run, wave = threadIdx.x / WAVE;
+  const int part1 = part0 + a.run < a.parts ? part0 + a.run : a.parts;
   const bool target = row < a.d + a.n;
   const int at_row = target ? row : row - (a.d + a.n);
-  float x[PER];
-  load16(target ? a.logits + at_row * a.ldl : a.drafts + at_row * a.ldd, part * CHUNK, a.vocab, x);
-  // the row's sequence: how many of the others begin no later
+  const float* src = target ? a.logits + at_row * a.ldl : a.drafts + at_row * a.ldd;
+  float x[PER], y[PER];
+  load16(src, part0 * CHUNK, a.vocab, x);
+  // the row's sequence: how many of the others begin no later (every wave counts for itself)
   int before = 0;
-  for (int i0 = 1; i0 < a.n; i0 += THREADS) {
-    const int i = i0 + (int)threadIdx.x;
-    before += __syncthreads_count(i < a.n && a.cu[i < a.n ? i : 0] + (target ? i : 0) <= at_row);
+  for (int i0 = 1; i0 < a.n; i0 += WAVE) {
+    const int i = i0 + ((int)threadIdx.x & 63);
+    before += __popcll(__ballot(i < a.n && a.cu[i < a.n ? i : 0] + (target ? i : 0) <= at_row));
   }
   const float t = a.temperature[before];
   const bool greedy = !(t > 0.f);
-  float m = -INFINITY;
-  int at = -1;
+  const double c = greedy ? 1.0 : LOG2E / (double)t;
+  auto one = [&](int part, float (&v)[PER], float (&next)[PER]) {
+    if (part + 1 < part1) load16(src, (part + 1) * CHUNK, a.vocab, next);
+    const int odd = part & 1;
+    float m = max_of(v);
+    int at = 0;
+    double s = 0.0;
+    if (greedy) {
+      at = -1;
 #pragma unroll
-  for (int k = 0; k < 4; ++k)
+      for (int k = PER - 1; k >= 0; --k)                      // the first of equals stays
+        if (v[k] == m) at = part * CHUNK + in_runs(k);
+      wave_max_at(m, at);
+    } else {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const float v = x[4 * k + e];
-      const bool more = v == v && (at < 0 || v > m);        // indices grow: the first of equals stays
-      m = more ? v : m;
-      at = more ? part * CHUNK + (k * THREADS + (int)threadIdx.x) * 4 + e : at;
+      for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, WAVE));
+      if (m < INFINITY) {
+        // what is -inf or NaN counts 2^-1000 here: nothing beside the maximum's 1
+        const double mc = -(double)m * c;
+#pragma unroll
+        for (int k = 0; k < PER; ++k) s += exp2_neg(fma((double)v[k], c, mc));
+      } else {
+#pragma unroll
+        for (int k = 0; k < PER; ++k) s += v[k] == m ? 1.0 : 0.0;
+      }
+      s = wave_sum64(s);
     }
-  wave_max_at(m, at);
-  if ((threadIdx.x & 63) == 0) {
-    ms[wave] = m;
-    as[wave] = at;
-  }
-  __syncthreads();
-  m = ms[0];
-  at = as[0];
+    if ((threadIdx.x & 63) == 0) {
+      ms[odd][wave] = m;
+      as[odd][wave] = at;
+      ss[odd][wave] = s;
+    }
+    __syncthreads();                       // the other place is written a part later, when everybody has read this one
+    if (threadIdx.x == 0) {
+      Piece16 p;
+      p.max = ms[odd][0];
+      p.arg = as[odd][0];
 #pragma unroll
-  for (int w = 1; w < THREADS / WAVE; ++w) take_max(m, at, ms[w], as[w]);
-  double s = 0.0;
-  if (!greedy) {
-    const double inv_t = 1.0 / (double)t;
+      for (int w = 1; w < NWV; ++w) {
+        if (greedy) take_max(p.max, p.arg, ms[odd][w], as[odd][w]);
+        else p.max = fmaxf(p.max, ms[odd][w]);
+      }
+      p.sum = 0.0;
+      if (!greedy) {
 #pragma unroll
-    for (int k = 0; k < PER; ++k) s += x[k] == x[k] ? weight(x[k], m, inv_t) : 0.0;
-    s = wave_sum64(s);
-    if ((threadIdx.x & 63) == 0) ss[wave] = s;
-    __syncthreads();
-    s = ss[0];
-#pragma unroll
-    for (int w = 1; w < THREADS / WAVE; ++w) s += ss[w];
-  }
-  if (threadIdx.x == 0) {
-    Piece16 p;
-    p.sum = s;
-    p.max = m;
-    p.arg = at;
-    a.pieces[(size_t)row * a.parts + part] = p;
+        for (int w = 0; w < NWV; ++w) p.sum += ss[odd][w] * weight(ms[odd][w], p.max, c);
+      }
+      a.pieces[(size_t)row * a.parts + part] = p;
+    }
+  };
+  for (int part = part0; part < part1; part += 2) {
+    one(part, x, y);
+    if (part + 1 < part1) one(part + 1, y, x);
   }
 }
 
-// A whole row from its parts, by one wave: maximum, its index, sum.
-__device__ __forceinline__ void whole_row(const Verify& a, int row, double inv_t, float& m, int& at, double& sum) {
-  const Piece16* p = a.pieces + (size_t)row * a.parts;
-  const int lane = threadIdx.x & 63;
-  m = -INFINITY;
-  at = -1;
-  for (int i = lane; i < a.parts; i += WAVE) take_max(m, at, p[i].max, p[i].arg);
-  wave_max_at(m, at);
-  sum = 0.0;
-  for (int i = lane; i < a.parts; i += WAVE)
-    if (p[i].arg >= 0) sum += p[i].sum * weight(p[i].max, m, inv_t);
-  sum = wave_sum64(sum);
-}
-
-struct Judged {       // a row's maxima and inverse sums, and whether its draft is kept
-  double tinv, dinv;
-  float tmax, dmax;
-  int arg, keep;
+struct Whole {        // a row from its parts: 1 / sum, maximum, its index
+  double inv;
+  float max;
+  int arg;
 };
 
-// grid (parts, sequences).  Every block of a sequence judges its drafts (a few hundred numbers that the first kernel
-// left) and sums the weights of its part of the row that the next token comes from.
+// grid (ceil(parts / judge_run), sequences).  Every block of a sequence judges its drafts (from a few hundred numbers that
+// the first kernel left, eight lanes a row) and sums the weights of its parts of the row that the next token comes from.
 __global__ __launch_bounds__(THREADS) void verify_judge_kernel(Verify a) {
   extern __shared__ __attribute__((aligned(16))) char lds[];
-  Judged* rows = (Judged*)lds;             // [most + 1]
+  Whole* rows = (Whole*)lds;               // [most + 1] of the target, [most] of the drafts
   __shared__ double ss[THREADS / WAVE];
-  const int part = blockIdx.x, seq = blockIdx.y, wave = threadIdx.x / WAVE, lane = threadIdx.x & 63;
+  const int part0 = blockIdx.x * a.judge_run, seq = blockIdx.y, wave = threadIdx.x / WAVE, lane = threadIdx.x & 63;
+  const int part1 = part0 + a.judge_run < a.parts ? part0 + a.judge_run : a.parts;
   int c0, c1;
   drafts_of(a, seq, c0, c1);
   const int d = c1 - c0;
   const float t = a.temperature[seq];
   const bool greedy = !(t > 0.f);
-  const double inv_t = greedy ? 1.0 : 1.0 / (double)t;
-  for (int j = wave; j <= d; j += THREADS / WAVE) {
-    const int row = c0 + seq + j;
-    Judged r;
-    double sum, dsum = 1.0;
-    int darg;
-    whole_row(a, row, inv_t, r.tmax, r.arg, sum);
-    r.tinv = 1.0 / sum;
-    r.dmax = 0.f;
-    r.dinv = 0.0;
-    r.keep = 0;
-    if (j < d) {
-      const int tok = a.tokens[c0 + j];
-      const bool in = tok >= 0 && tok < a.vocab;
-      double p = 0.0, q = 1.0;
-      if (greedy) {
-        p = in && tok == r.arg ? 1.0 : 0.0;
-        r.keep = p > 0.0;
-      } else {
-        const float x = a.logits[row * a.ldl + (in ? tok : 0)];
-        p = in && x == x ? weight(x, r.tmax, inv_t) * r.tinv : 0.0;
-        if (a.drafts) {
-          whole_row(a, a.d + a.n + c0 + j, inv_t, r.dmax, darg, dsum);
-          r.dinv = 1.0 / dsum;
-          const float y = a.drafts[(c0 + j) * a.ldd + (in ? tok : 0)];
-          q = in && y == y ? weight(y, r.dmax, inv_t) * r.dinv : 0.0;
-        }
-        r.keep = (double)a.uniform[row] * q < p;
-      }
-      if (part == 0 && lane == 0 && a.probs) a.probs[c0 + j] = (float)p;
+  const double c = greedy ? 1.0 : LOG2E / (double)t;
+  // a lane for each draft (every wave judges all of them): its token and the two logits
+  auto logits_of = [&](int j, bool& in, float& x, float& y) {
+    const int tok = a.tokens[c0 + j];
+    in = tok >= 0 && tok < a.vocab;
+    x = a.logits[(c0 + seq + j) * a.ldl + (in ? tok : 0)];
+    y = a.drafts ? a.drafts[(c0 + j) * a.ldd + (in ? tok : 0)] : 0.f;
+  };
+  bool in0 = false;
+  float x0 = 0.f, y0 = 0.f;
+  if (lane < d) logits_of(lane, in0, x0, y0);
+  const int n_rows = d + 1 + (a.drafts && !greedy ? d : 0), sub = threadIdx.x & 7;
+  for (int q0 = 0; q0 < n_rows; q0 += THREADS / 8) {
+    const int q = q0 + (int)threadIdx.x / 8, qc = q < n_rows ? q : n_rows - 1;
+    const Piece16* p = a.pieces + (size_t)(qc <= d ? c0 + seq + qc : a.d + a.n + c0 + qc - d - 1) * a.parts;
+    Whole w;
+    w.max = -INFINITY;
+    w.arg = -1;
+    for (int i = sub; i < a.parts; i += 8) take_max(w.max, w.arg, p[i].max, p[i].arg);
+#pragma unroll
+    for (int o = 4; o > 0; o >>= 1) {
+      const float m2 = __shfl_xor(w.max, o, WAVE);
+      const int at2 = __shfl_xor(w.arg, o, WAVE);
+      take_max(w.max, w.arg, m2, at2);
     }
-    if (lane == 0) rows[j] = r;
+    double sum = 0.0;
+    for (int i = sub; i < a.parts; i += 8) sum += p[i].sum * weight(p[i].max, w.max, c);
+#pragma unroll
+    for (int o = 4; o > 0; o >>= 1) sum += __shfl_xor(sum, o, WAVE);
+    w.inv = 1.0 / sum;
+    if (sub == 0 && q < n_rows) rows[q] = w;
   }
   __syncthreads();
-  int kept = 0;
-  while (kept < d && rows[kept].keep) ++kept;
-  const Judged r = rows[kept];
+  int kept = d;
+  for (int j0 = 0; j0 < d && kept == d; j0 += WAVE) {
+    const int j = j0 + lane;
+    if (j0 > 0 && j < d) logits_of(j, in0, x0, y0);
+    bool keep = true;
+    if (j < d) {
+      double p, q = 1.0;
+      if (greedy) {
+        p = in0 && a.tokens[c0 + j] == rows[j].arg ? 1.0 : 0.0;
+        keep = p > 0.0;
+      } else {
+        p = in0 ? weight(x0, rows[j].max, c) * rows[j].inv : 0.0;
+        if (a.drafts) q = in0 ? weight(y0, rows[d + 1 + j].max, c) * rows[d + 1 + j].inv : 0.0;
+        keep = (double)a.uniform[c0 + seq + j] * q < p;
+      }
+      if (part0 == 0 && wave == 0 && a.probs) a.probs[c0 + j] = (float)p;
+    }
+    const unsigned long long refused = __ballot(!keep);
+    if (refused) kept = j0 + __builtin_ctzll(refused);
+  }
+  if (part0 == 0 && wave == 0 && a.probs)             // the drafts behind the first 64 and a refused one have a probability too
+    for (int j = (kept / WAVE + 1) * WAVE + lane; kept < d && j < d; j += WAVE) {
+      logits_of(j, in0, x0, y0);
+      a.probs[c0 + j] = !in0 ? 0.f : greedy ? (a.tokens[c0 + j] == rows[j].arg ? 1.f : 0.f) : (float)(weight(x0, rows[j].max, c) * rows[j].inv);
+    }
   const bool refused = kept < d;
+  const Whole r = rows[kept], less = rows[refused && a.drafts && !greedy ? d + 1 + kept : kept];
   const int row = c0 + seq + kept;
-  Choice c;
-  c.accepted = kept;
-  c.row = row;
-  c.draft_row = refused && !greedy && a.drafts ? c0 + kept : -1;
-  c.without = refused && !greedy && !a.drafts ? a.tokens[c0 + kept] : -1;
-  c.drawn = greedy ? (r.arg < 0 ? 0 : r.arg) : -1;
-  c.tmax = r.tmax;
-  c.dmax = r.dmax;
-  c.tinv = r.tinv;
-  c.dinv = r.dinv;
-  if (part == 0 && threadIdx.x == 0) a.choice[seq] = c;
+  Choice ch;
+  ch.accepted = kept;
+  ch.row = row;
+  ch.draft_row = refused && !greedy && a.drafts ? c0 + kept : -1;
+  ch.without = refused && !greedy && !a.drafts ? a.tokens[c0 + kept] : -1;
+  ch.drawn = greedy ? (r.arg < 0 ? 0 : r.arg) : -1;
+  ch.tmax = r.max;
+  ch.dmax = less.max;
+  ch.tinv = r.inv;
+  ch.dinv = less.inv;
+  if (part0 == 0 && threadIdx.x == 0) a.choice[seq] = ch;
   if (greedy) return;
-  double s = 0.0;
   if (!refused) {                          // the whole row: its parts' sums are known
-    const Piece16 p = a.pieces[(size_t)row * a.parts + part];
-    s = p.arg >= 0 ? p.sum * weight(p.max, r.tmax, inv_t) * r.tinv : 0.0;
-  } else {
+    const int part = part0 + (int)threadIdx.x;
+    if (part < part1) {
+      const Piece16 p = a.pieces[(size_t)row * a.parts + part];
+      a.mass[(size_t)seq * a.parts + part] = p.sum * weight(p.max, r.max, c) * r.inv;
+    }
+    return;
+  }
+  const float* src = a.logits + row * a.ldl;
+  const float* src2 = a.drafts ? a.drafts + (long long)ch.draft_row * a.ldd : src;
+  for (int part = part0; part < part1; ++part) {
     float x[PER], y[PER];
-    load16(a.logits + row * a.ldl, part * CHUNK, a.vocab, x);
-    if (a.drafts) load16(a.drafts + (long long)c.draft_row * a.ldd, part * CHUNK, a.vocab, y);
+    load16(src, part * CHUNK, a.vocab, x);
+    load16(src2, part * CHUNK, a.vocab, y);
+    double s = 0.0;
 #pragma unroll
     for (int k = 0; k < PER; ++k) {
-      double w = x[k] == x[k] ? weight(x[k], r.tmax, inv_t) * r.tinv : 0.0;
-      if (a.drafts) w -= y[k] == y[k] ? weight(y[k], r.dmax, inv_t) * r.dinv : 0.0;
-      else if (part * CHUNK + ((k >> 2) * THREADS + (int)threadIdx.x) * 4 + (k & 3) == c.without) w = 0.0;
+      double w = weight(x[k], r.max, c) * r.inv;
+      if (a.drafts) w -= weight(y[k], less.max, c) * less.inv;
+      else if (part * CHUNK + in_runs(k) == ch.without) w = 0.0;
       s += fmax(w, 0.0);
     }
     s = wave_sum64(s);
+    if (part > part0) __syncthreads();     // the part before has been read
     if (lane == 0) ss[wave] = s;
     __syncthreads();
-    s = ss[0];
+    if (threadIdx.x == 0) {
+      s = ss[0];
 #pragma unroll
-    for (int w = 1; w < THREADS / WAVE; ++w) s += ss[w];
+      for (int w = 1; w < THREADS / WAVE; ++w) s += ss[w];
+      a.mass[(size_t)seq * a.parts + part] = s;
+    }
   }
-  if (threadIdx.x == 0) a.mass[(size_t)seq * a.parts + part] = s;
 }
 
 // grid (sequences).  The part whose running sum passes the target, then the element in it.
 __global__ __launch_bounds__(THREADS) void verify_draw_kernel(Verify a) {
-  __shared__ double run[THREADS];
+  __shared__ double wave_run[THREADS / WAVE];
   __shared__ int found;
-  const int seq = blockIdx.x;
-  const Choice c = a.choice[seq];
-  if (threadIdx.x == 0) a.accepted[seq] = c.accepted;
-  if (c.drawn >= 0) {
-    if (threadIdx.x == 0) a.token[seq] = c.drawn;
-    return;
-  }
+  const int seq = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x / WAVE;
+  const Choice ch = a.choice[seq];
+  const float t = a.temperature[seq];
+  const double own = a.mass[(size_t)seq * a.parts + (lane < a.parts ? lane : 0)];      // of the first 64 parts
   int c0, c1;
   drafts_of(a, seq, c0, c1);
-  const double inv_t = 1.0 / (double)a.temperature[seq];
+  const double u = (double)a.uniform[c1 + seq];
+  if (threadIdx.x == 0) {
+    a.accepted[seq] = ch.accepted;
+    found = a.vocab;
+  }
+  if (ch.drawn >= 0) {
+    if (threadIdx.x == 0) a.token[seq] = ch.drawn;
+    return;
+  }
+  const double c = LOG2E / (double)t;
   // every wave by itself: the parts' masses one a lane, their running sums
-  const int lane = threadIdx.x & 63;
-  const Piece16* p = a.pieces + (size_t)c.row * a.parts;
-  auto total_of = [&](bool plain) {
+  const Piece16* p = a.pieces + (size_t)ch.row * a.parts;
+  bool plain = false;
+  auto mass_of = [&](int i) {              // of part i, whose number is the lane's modulo 64
+    if (plain) return i < a.parts ? p[i].sum * weight(p[i].max, ch.tmax, c) * ch.tinv : 0.0;
+    return i < a.parts ? (i < WAVE ? own : a.mass[(size_t)seq * a.parts + i]) : 0.0;
+  };
+  auto total_of = [&]() {
     double v = 0.0;
-    for (int i = lane; i < a.parts; i += WAVE)
-      v += plain ? (p[i].arg >= 0 ? p[i].sum * weight(p[i].max, c.tmax, inv_t) * c.tinv : 0.0) : a.mass[(size_t)seq * a.parts + i];
+    for (int i = lane; i < a.parts; i += WAVE) v += mass_of(i);
     return wave_sum64(v);
   };
-  double total = total_of(false);
-  const bool plain = !(total > 0.0);       // nothing is left beside the draft's distribution: the target's own
-  if (plain) total = total_of(true);
-  const double target = (double)a.uniform[c1 + seq] * total;
+  double total = total_of();
+  if (!(total > 0.0)) {                    // nothing is left beside the draft's distribution: the target's own
+    plain = true;
+    total = total_of();
+  }
+  const double target = u * total;
   int part = -1, last_part = 0;
   double before = 0.0, last_before = 0.0, sum_so_far = 0.0;
   for (int i0 = 0; i0 < a.parts && part < 0; i0 += WAVE) {
-    const int i = i0 + lane;
-    double v = 0.0;
-    if (i < a.parts) v = plain ? (p[i].arg >= 0 ? p[i].sum * weight(p[i].max, c.tmax, inv_t) * c.tinv : 0.0) : a.mass[(size_t)seq * a.parts + i];
-    double incl = v;
-#pragma unroll
-    for (int o = 1; o < WAVE; o <<= 1) {
-      const double u = __shfl_up(incl, o, WAVE);
-      if (lane >= o) incl += u;
-    }
-    incl += sum_so_far;
-    const double excl = incl - v;
-    const unsigned long long over = __ballot(i < a.parts && v > 0.0 && incl > target), some = __ballot(v > 0.0);
+    const double v = mass_of(i0 + lane);
+    const double incl = wave_running64(v) + sum_so_far, excl = incl - v;
+    const unsigned long long over = __ballot(v > 0.0 && incl > target), some = __ballot(v > 0.0);
     if (some) {
       const int at = 63 - __builtin_clzll(some);
       last_part = i0 + at;
@@ -364,35 +422,31 @@ __global__ __launch_bounds__(THREADS) void verify_draw_kernel(Verify a) {
     part = last_part;
     before = last_before;
   }
-  if (threadIdx.x == 0) found = a.vocab;
-  __syncthreads();
-  const int first = part * CHUNK + (int)threadIdx.x * PER;         // consecutive elements a thread, for the running sum
-  const float* row = a.logits + (long long)c.row * a.ldl;
-  const bool less = !plain && c.draft_row >= 0;
+  const int first = part * CHUNK + (int)threadIdx.x * PER;
+  const bool less = !plain && ch.draft_row >= 0;
   float x[PER], y[PER];
-  load_run(row, first, a.vocab, x);
-  if (less) load_run(a.drafts + (long long)c.draft_row * a.ldd, first, a.vocab, y);
+  auto consecutive = [](int k) { return (int)threadIdx.x * PER + k; };      // a thread's sixteen lie in a row, for the running sum
+  load_part(a.logits + (long long)ch.row * a.ldl, part * CHUNK, a.vocab, x, consecutive);
+  if (less) load_part(a.drafts + (long long)ch.draft_row * a.ldd, part * CHUNK, a.vocab, y, consecutive);
   double w[PER], sum = 0.0;
   int last = -1;
 #pragma unroll
   for (int k = 0; k < PER; ++k) {
     const int i = first + k;
-    double v = x[k] == x[k] ? weight(x[k], c.tmax, inv_t) * c.tinv : 0.0;
-    if (less) v -= y[k] == y[k] ? weight(y[k], c.dmax, inv_t) * c.dinv : 0.0;
-    if (!plain && i == c.without) v = 0.0;
+    double v = weight(x[k], ch.tmax, c) * ch.tinv;
+    if (less) v -= weight(y[k], ch.dmax, c) * ch.dinv;
+    if (!plain && i == ch.without) v = 0.0;
     w[k] = fmax(v, 0.0);
     if (w[k] > 0.0) last = i;
     sum += w[k];
   }
-  run[threadIdx.x] = sum;
+  const double run = wave_running64(sum);
+  if (lane == WAVE - 1) wave_run[wave] = run;
   __syncthreads();
-  for (int o = 1; o < THREADS; o <<= 1) {          // running sums over the threads
-    const double v = (int)threadIdx.x >= o ? run[threadIdx.x - o] : 0.0;
-    __syncthreads();
-    run[threadIdx.x] += v;
-    __syncthreads();
-  }
-  double at = before + (threadIdx.x > 0 ? run[threadIdx.x - 1] : 0.0);
+  double at = before + (run - sum);
+#pragma unroll
+  for (int i = 0; i < THREADS / WAVE; ++i)
+    if (i < wave) at += wave_run[i];
   int hit = a.vocab;
 #pragma unroll
   for (int k = 0; k < PER; ++k) {
@@ -436,14 +490,17 @@ extern "C" const char* dlgo_verify_drafts(const float* logits, long long ldl, co
   DLGO_REQUIRE(scratch && scratch_bytes >= need && ((uintptr_t)scratch & 15) == 0, "verify_drafts: %lld bytes of scratch are needed, %lld given", need, scratch ? scratch_bytes : 0ll);
   DLGO_REQUIRE(rows * parts < (1ll << 31) && n <= 65535, "verify_drafts: too many rows at once");
   char* at = (char*)scratch;
-  Verify a = {logits, drafts, tokens, cu, temperature, uniform, accepted, token, probs, (Piece16*)at, nullptr, nullptr, ldl, ldd, n, d, vocab, (int)parts, most};
+  Verify a = {logits, drafts, tokens, cu, temperature, uniform, accepted, token, probs, (Piece16*)at, nullptr, nullptr, ldl, ldd, n, d, vocab, (int)parts, most, 1, 1};
   at += round16(rows * parts * (long long)sizeof(Piece16));
   a.mass = (double*)at;
   at += round16(n * parts * 8);
   a.choice = (Choice*)at;
-  hipLaunchKernelGGL(verify_rows_kernel, dim3((unsigned)(rows * parts)), dim3(THREADS), 0, stream, a);
+  // with many blocks a unit each takes several parts in turn; with few every part is a block of its own
+  a.run = rows * parts >= 8192 ? 4 : 1;
+  hipLaunchKernelGGL(verify_rows_kernel, dim3((unsigned)(rows * ((parts + a.run - 1) / a.run))), dim3(THREADS), 0, stream, a);
   DLGO_LAUNCH_CHECK("verify_drafts");
-  hipLaunchKernelGGL(verify_judge_kernel, dim3((unsigned)parts, (unsigned)n), dim3(THREADS), (most + 1) * (int)sizeof(Judged), stream, a);
+  a.judge_run = n * parts >= 1024 ? 2 : 1;
+  hipLaunchKernelGGL(verify_judge_kernel, dim3((unsigned)((parts + a.judge_run - 1) / a.judge_run), (unsigned)n), dim3(THREADS), (2 * most + 1) * (int)sizeof(Whole), stream, a);
   DLGO_LAUNCH_CHECK("verify_drafts");
   hipLaunchKernelGGL(verify_draw_kernel, dim3((unsigned)n), dim3(THREADS), 0, stream, a);
   DLGO_LAUNCH_CHECK("verify_drafts");
