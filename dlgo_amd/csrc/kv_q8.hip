@@ -34,6 +34,10 @@ static __device__ __forceinline__ void load8(const bf16_t* p, float* f) {
   f[6] = __uint_as_float(u.w << 16); f[7] = __uint_as_float(u.w & 0xffff0000u);
 }
 
+static __device__ __forceinline__ void store8(bf16_t* p, const float* f) {
+  *(uint4*)p = make_uint4(Elem<bf16_t>::pair(f[0], f[1]), Elem<bf16_t>::pair(f[2], f[3]), Elem<bf16_t>::pair(f[4], f[5]), Elem<bf16_t>::pair(f[6], f[7]));
+}
+
 // Eight elements of a head from element d0 on, rotated.  PIECES: pairs lie in this piece (interleaved) or are this piece
 // and the one half a rotated width away, all 16-byte aligned; else element by element.
 template <bool PIECES>
@@ -130,67 +134,148 @@ static __device__ __forceinline__ long long page_of(const RopeQ8& a, int t, int 
   return page < 0 || page >= a.n_pages ? -1 : (long long)page * a.page_stride;
 }
 
-// The queries: a thread takes a piece of eight elements and, where its pairs lie in another piece, that one too (the
-// thread of the higher piece then has nothing to do), so that q_out may be the queries' own place in qkv.
+// The queries.  A thread takes a piece of eight elements, or the two pieces whose elements are each other's partners, of
+// QH heads of a row: the angles are read once for all of them, and their loads are asked for together.  It writes only
+// what it has read, so q_out may be the queries' own place in qkv.
+#define QH 4
+struct QueryUnits {
+  int far, per_head, groups;      // pairs of pieces half a rotated width apart; units a head; groups of QH heads
+};
+static __host__ __device__ __forceinline__ QueryUnits query_units(int n_heads, int hd, int rot, bool pieces, bool rotates, bool interleaved) {
+  QueryUnits u;
+  u.far = rotates && !interleaved ? rot / 16 : 0;
+  u.per_head = pieces ? u.far + (hd - 16 * u.far) / 8 : 1;
+  u.groups = (n_heads + QH - 1) / QH;
+  return u;
+}
 template <bool PIECES>
 static __device__ __forceinline__ void queries(const RopeQ8& a, long long idx) {
-  const int per_head = a.hd / 8, per_row = a.n_heads * per_head;
+  const QueryUnits u = query_units(a.n_heads, a.hd, a.rot, PIECES, a.cos_t != nullptr, a.interleaved != 0);
+  const int per_row = u.groups * u.per_head;
   if (idx >= (long long)a.n_tokens * per_row) return;
-  const int t = (int)(idx / per_row), c = (int)(idx % per_row), d0 = (c % per_head) * 8;
-  const bf16_t* head = a.qkv + (size_t)t * a.ld + (size_t)(c / per_head) * a.hd;
-  bf16_t* dst = a.q_out + (size_t)t * a.ldq + (size_t)(c / per_head) * a.hd;
-  const int pos = a.positions[t];
+  const int t = (int)(idx / per_row), c = (int)(idx % per_row), h0 = c / u.per_head * QH, unit = c % u.per_head;
+  const int heads = a.n_heads - h0 < QH ? a.n_heads - h0 : QH;
+  const bf16_t* src = a.qkv + (size_t)t * a.ld + (size_t)h0 * a.hd;
+  bf16_t* dst = a.q_out + (size_t)t * a.ldq + (size_t)h0 * a.hd;
+  const int half = a.rot / 2, pos = a.positions[t];
+  const size_t at = (size_t)(pos < 0 ? 0 : (pos < a.table_rows ? pos : a.table_rows - 1)) * half;
   if constexpr (PIECES) {
-    const bool far = a.cos_t && !a.interleaved && d0 < a.rot;
-    const int half = a.rot / 2;
-    if (far && d0 >= half) return;
-    float y[8], z[8];
-    rotated8<true>(a, head, pos, d0, y);
-    if (far) rotated8<true>(a, head, pos, d0 + half, z);
-    Elem<bf16_t>::store4(dst + d0, y[0], y[1], y[2], y[3]);
-    Elem<bf16_t>::store4(dst + d0 + 4, y[4], y[5], y[6], y[7]);
-    if (far) {
-      Elem<bf16_t>::store4(dst + d0 + half, z[0], z[1], z[2], z[3]);
-      Elem<bf16_t>::store4(dst + d0 + half + 4, z[4], z[5], z[6], z[7]);
+    const bool far = unit < u.far;
+    const int d0 = far ? unit * 8 : 16 * u.far + (unit - u.far) * 8, d1 = far ? d0 + half : d0;
+    uint4 lo[QH], hi[QH];
+#pragma unroll
+    for (int h = 0; h < QH; ++h) {                       // a head past the last: the last again
+      const bf16_t* p = src + (size_t)(h < heads ? h : heads - 1) * a.hd;
+      lo[h] = *(const uint4*)(p + d0);
+      hi[h] = *(const uint4*)(p + d1);
     }
-  } else if (d0 == 0) {      // widths that no model of a usual shape has: a thread takes a whole head, pair by pair
-    const int half = a.rot / 2;
-    const size_t at = (size_t)(pos < 0 ? 0 : (pos < a.table_rows ? pos : a.table_rows - 1)) * half;
-#pragma unroll 1
-    for (int i = 0; i < half; ++i) {
-      const int i0 = a.interleaved ? 2 * i : i, i1 = a.interleaved ? 2 * i + 1 : i + half;
-      float x0 = bf16_to_f32(head[i0]), x1 = bf16_to_f32(head[i1]);
-      if (a.cos_t) {
-        const float c_ = a.cos_t[at + i], s_ = a.sin_t[at + i];
-        const float y0 = rotated_lo(x0, x1, c_, s_), y1 = rotated_hi(x0, x1, c_, s_);
-        x0 = y0;
-        x1 = y1;
+    const bool turns = a.cos_t && d0 < a.rot;
+    float cs[8], sn[8];
+    if (turns) {
+      const size_t i0 = at + (far ? d0 : d0 / 2);
+#pragma unroll
+      for (int e = 0; e < 8; e += 4) {                   // interleaved pairs have four angles a piece
+        *(float4*)(cs + e) = *(const float4*)(a.cos_t + i0 + (far ? e : 0));
+        *(float4*)(sn + e) = *(const float4*)(a.sin_t + i0 + (far ? e : 0));
       }
-      dst[i0] = f32_to_bf16(x0);
-      dst[i1] = f32_to_bf16(x1);
     }
+#pragma unroll
+    for (int h = 0; h < QH; ++h) {
+      if (h >= heads) break;
+      float x[8], y[8];
+      load8((const bf16_t*)&lo[h], x);
+      load8((const bf16_t*)&hi[h], y);
+      if (turns && far) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float x0 = x[e], x1 = y[e];
+          x[e] = rotated_lo(x0, x1, cs[e], sn[e]);
+          y[e] = rotated_hi(x0, x1, cs[e], sn[e]);
+        }
+      } else if (turns) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float x0 = x[2 * i], x1 = x[2 * i + 1];
+          x[2 * i] = rotated_lo(x0, x1, cs[i], sn[i]);
+          x[2 * i + 1] = rotated_hi(x0, x1, cs[i], sn[i]);
+        }
+      }
+      store8(dst + (size_t)h * a.hd + d0, x);
+      if (far) store8(dst + (size_t)h * a.hd + d1, y);
+    }
+  } else {      // widths that no model of a usual shape has: a thread takes whole heads, pair by pair
 #pragma unroll 1
-    for (int i = a.rot; i < a.hd; ++i) dst[i] = head[i];
+    for (int h = 0; h < heads; ++h) {
+      const bf16_t* head = src + (size_t)h * a.hd;
+      bf16_t* out = dst + (size_t)h * a.hd;
+#pragma unroll 1
+      for (int i = 0; i < half; ++i) {
+        const int i0 = a.interleaved ? 2 * i : i, i1 = a.interleaved ? 2 * i + 1 : i + half;
+        float x0 = bf16_to_f32(head[i0]), x1 = bf16_to_f32(head[i1]);
+        if (a.cos_t) {
+          const float c_ = a.cos_t[at + i], s_ = a.sin_t[at + i];
+          const float y0 = rotated_lo(x0, x1, c_, s_), y1 = rotated_hi(x0, x1, c_, s_);
+          x0 = y0;
+          x1 = y1;
+        }
+        out[i0] = f32_to_bf16(x0);
+        out[i1] = f32_to_bf16(x1);
+      }
+#pragma unroll 1
+      for (int i = a.rot; i < a.hd; ++i) out[i] = head[i];
+    }
   }
 }
 
-// `lanes` (a power of two, at least hd / 8) neighbouring threads share a token's key and value of one head, a piece of
-// eight elements each.
-template <bool PIECES>
+// `lanes` (a power of two, at least hd / (8 N)) neighbouring threads share a token's key and value of one head, N pieces of
+// eight elements each: with N = 2 piece p and piece p + hd / 16, which are each other's partners where the whole head is
+// rotated in halves (half the loads); with N = 1 piece p (a shorter way for a launch of few rows: 8 tokens 5.6 -> 4.5 us).
+template <bool PIECES, int N>
 static __device__ __forceinline__ void key_and_value(const RopeQ8& a, int t, int kvh, int piece, int lanes, int pos, uint2* kb, uint2* vb,
                                                      int* ks, int* vs) {
-  float k[8], v[8];
-  const int d0 = piece * 8;
+  float k[N][8], v[N][8];
   uint32_t kt = 0, vt = 0;
-  if (d0 < a.hd) {
+  const int d0 = piece * 8, d1 = d0 + a.hd / 2;
+  if (d0 < a.hd / N) {
     const bf16_t* row = a.qkv + (size_t)t * a.ld;
-    rotated8<PIECES>(a, row + (size_t)(a.n_heads + kvh) * a.hd, pos, d0, k);
-    plain8<PIECES>(row + (size_t)(a.n_heads + a.n_kv + kvh) * a.hd + d0, v);
-    kt = top_bits(k);
-    vt = top_bits(v);
+    const bf16_t* key = row + (size_t)(a.n_heads + kvh) * a.hd;
+    const bf16_t* val = row + (size_t)(a.n_heads + a.n_kv + kvh) * a.hd;
+    if (N == 2 && PIECES && a.cos_t && !a.interleaved && a.rot == a.hd) {
+      load8(key + d0, k[0]);
+      load8(key + d1, k[N - 1]);
+      plain8<PIECES>(val + d0, v[0]);
+      plain8<PIECES>(val + d1, v[N - 1]);
+      const size_t at = (size_t)(pos < 0 ? 0 : (pos < a.table_rows ? pos : a.table_rows - 1)) * (a.hd / 2) + d0;
+      float c[8], s[8];
+#pragma unroll
+      for (int e = 0; e < 8; e += 4) {
+        *(float4*)(c + e) = *(const float4*)(a.cos_t + at + e);
+        *(float4*)(s + e) = *(const float4*)(a.sin_t + at + e);
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float x0 = k[0][e], x1 = k[N - 1][e];
+        k[0][e] = rotated_lo(x0, x1, c[e], s[e]);
+        k[N - 1][e] = rotated_hi(x0, x1, c[e], s[e]);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        rotated8<PIECES>(a, key, pos, i ? d1 : d0, k[i]);
+        plain8<PIECES>(val + (i ? d1 : d0), v[i]);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const uint32_t k1 = top_bits(k[i]), v1 = top_bits(v[i]);
+      kt = k1 > kt ? k1 : kt;
+      vt = v1 > vt ? v1 : vt;
+    }
   } else {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) k[e] = v[e] = 0.f;
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) k[i][e] = v[i][e] = 0.f;
   }
   for (int o = lanes >> 1; o > 0; o >>= 1) {
     const uint32_t k2 = (uint32_t)__shfl_xor((int)kt, o, WAVE), v2 = (uint32_t)__shfl_xor((int)vt, o, WAVE);
@@ -199,8 +284,11 @@ static __device__ __forceinline__ void key_and_value(const RopeQ8& a, int t, int
   }
   const bool finite = kt < 0x7f800000u && vt < 0x7f800000u;
   const int ke = power_for(kt), ve = power_for(vt);
-  *kb = finite ? to_e4m3(k, ke) : make_uint2(0, 0);
-  *vb = finite ? to_e4m3(v, ve) : make_uint2(0, 0);
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    kb[i] = finite ? to_e4m3(k[i], ke) : make_uint2(0, 0);
+    vb[i] = finite ? to_e4m3(v[i], ve) : make_uint2(0, 0);
+  }
   *ks = finite ? ke + 127 : Q8_NAN;
   *vs = finite ? ve + 127 : 127;
 }
@@ -218,17 +306,17 @@ __global__ __launch_bounds__(256) void rope_kv_q8_rows_kernel(RopeQ8 a, int kv_b
   const bool real = unit < units;
   const int t = real ? (int)(unit / a.n_kv) : 0, kvh = real ? (int)(unit % a.n_kv) : 0;
   const int pos = a.positions[t];
-  uint2 kb, vb;
+  uint2 kb[1], vb[1];
   int ks, vs;
-  key_and_value<PIECES>(a, t, kvh, piece, lanes, pos, &kb, &vb, &ks, &vs);
   const long long off = page_of(a, t, pos);
+  key_and_value<PIECES, 1>(a, t, kvh, piece, lanes, pos, kb, vb, &ks, &vs);
   if (!real || off < 0 || piece * 8 >= a.hd) return;
   uint8_t* head = a.cache + off + (size_t)kvh * q8_head_bytes(a.hd);
   const int in = pos % Q8_PAGE, t16 = in >> 4, i = in & 15, g = i >> 2, r = i & 3;
-  *(uint2*)(head + (t16 * (a.hd / 16) + piece / 2) * 256 + i * 16 + (piece & 1) * 8) = kb;
+  *(uint2*)(head + (t16 * (a.hd / 16) + piece / 2) * 256 + i * 16 + (piece & 1) * 8) = kb[0];
   uint8_t* val = head + Q8_PAGE * a.hd + ((piece / 2 * 4 + g) * 16 + (piece & 1) * 8) * 16 + 4 * t16 + r;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) val[e * 16] = (uint8_t)((e < 4 ? vb.x : vb.y) >> (8 * (e & 3)));
+  for (int e = 0; e < 8; ++e) val[e * 16] = (uint8_t)((e < 4 ? vb[0].x : vb[0].y) >> (8 * (e & 3)));
   if (piece == 0) {
     uint8_t* scales = head + 2 * Q8_PAGE * a.hd;
     scales[4 * i + t16] = (uint8_t)ks;
@@ -248,6 +336,7 @@ __global__ __launch_bounds__(256) void rope_kv_q8_tiles_kernel(RopeQ8 a, int kv_
   }
   __shared__ long long at[64];        // each row's page in the cache, -1 where there is none
   __shared__ int in_page[64];
+  __shared__ long long group[16];
   const int stride = a.hd + 16;       // rows 16 bytes apart in the banks
   uint8_t* kt = lds;
   uint8_t* vt = lds + 64 * stride;
@@ -260,17 +349,28 @@ __global__ __launch_bounds__(256) void rope_kv_q8_tiles_kernel(RopeQ8 a, int kv_
     in_page[threadIdx.x] = pos & (Q8_PAGE - 1);
   }
   __syncthreads();
+  // where the word of each group of four rows goes that are four tokens of one word (for element 0), -1 for the others
+  const int lead = 3 & -in_page[0];
+  if (threadIdx.x < 16) {
+    const int j = lead + 4 * (int)threadIdx.x;
+    const bool whole = j + 3 < n && at[j] >= 0 && (in_page[j] & 3) == 0 && at[j + 3] == at[j] && at[j + 1] == at[j] && at[j + 2] == at[j] &&
+                       in_page[j + 1] == in_page[j] + 1 && in_page[j + 2] == in_page[j] + 2 && in_page[j + 3] == in_page[j] + 3;
+    group[threadIdx.x] = whole ? at[j] + Q8_PAGE * a.hd + ((in_page[j] >> 2) & 3) * 256 + (in_page[j] >> 4) * 4 : -1;
+  }
   const size_t head = (size_t)kvh * q8_head_bytes(a.hd);
   const int piece = threadIdx.x % lanes;
   for (int j0 = 0; j0 < 64; j0 += 256 / lanes) {        // whole waves take part in the shuffles
     const int j = j0 + threadIdx.x / lanes;
     const int t = t0 + (j < n ? j : n - 1);
-    uint2 kb, vb;
+    uint2 kb[2], vb[2];
     int ks, vs;
-    key_and_value<PIECES>(a, t, kvh, piece, lanes, a.positions[t], &kb, &vb, &ks, &vs);
-    if (j >= 64 || piece * 8 >= a.hd) continue;
-    *(uint2*)(kt + j * stride + piece * 8) = kb;
-    *(uint2*)(vt + j * stride + piece * 8) = vb;
+    key_and_value<PIECES, 2>(a, t, kvh, piece, lanes, a.positions[t], kb, vb, &ks, &vs);
+    if (j >= 64 || piece * 16 >= a.hd) continue;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      *(uint2*)(kt + j * stride + piece * 8 + h * (a.hd / 2)) = kb[h];
+      *(uint2*)(vt + j * stride + piece * 8 + h * (a.hd / 2)) = vb[h];
+    }
     if (piece == 0 && at[j] >= 0) {
       uint8_t* scales = a.cache + at[j] + head + 2 * Q8_PAGE * a.hd;
       const int in = in_page[j], t16 = in >> 4, i = in & 15;
@@ -279,34 +379,33 @@ __global__ __launch_bounds__(256) void rope_kv_q8_tiles_kernel(RopeQ8 a, int kv_
     }
   }
   __syncthreads();
-  const int pieces = a.hd / 16;
-  for (int c = threadIdx.x; c < 64 * pieces; c += 256) {
-    const int j = c & 63, p = c >> 6;
-    if (at[j] < 0) continue;
-    const int in = in_page[j];
-    *(uint4*)(a.cache + at[j] + head + ((in >> 4) * pieces + p) * 256 + (in & 15) * 16) = *(const uint4*)(kt + j * stride + p * 16);
+  {
+    const int j = threadIdx.x & 63, pieces = a.hd / 16;
+    if (at[j] >= 0) {
+      uint8_t* page = a.cache + at[j] + head + (in_page[j] >> 4) * pieces * 256 + (in_page[j] & 15) * 16;
+      for (int p = threadIdx.x >> 6; p < pieces; p += 4) *(uint4*)(page + p * 256) = *(const uint4*)(kt + j * stride + p * 16);
+    }
   }
-  // four rows of a word: q = which of the four words 16 rows apart, so that 64 lanes write 256 bytes in a row
-  const int lead = 3 & -in_page[0];   // rows before the first one whose place in its page is a multiple of four
-  for (int c = threadIdx.x; c < 64 * (a.hd / 4); c += 256) {
-    const int q = c & 3, d = (c >> 2) % a.hd, g = (c >> 2) / a.hd;       // g: 0 .. 3
-    // 16 groups of four rows from row `lead` on, and the rows left over at both ends (lead of them before, 4 - lead after)
+  // 16 groups of four rows from the first row on whose place in its page is a multiple of four; the rows left over at both
+  // ends are the sixteenth.  A thread's groups are 16 rows apart from its neighbours', so that 64 lanes write 256 bytes in a row.
+  const int q = threadIdx.x & 3;
+  for (int g = 0; g < 4; ++g) {
     const int j = lead + 16 * q + 4 * g;
-    const bool whole = j + 3 < n && at[j] >= 0 && (in_page[j] & 3) == 0 && at[j + 3] == at[j] && at[j + 1] == at[j] && at[j + 2] == at[j] &&
-                       in_page[j + 1] == in_page[j] + 1 && in_page[j + 2] == in_page[j] + 2 && in_page[j + 3] == in_page[j] + 3;
-    const uint8_t* src = vt + d;
-    uint8_t* page = a.cache + head + Q8_PAGE * a.hd + (d & ~15) * 64 + (d & 15) * 16;
-    if (whole) {
-      const int in = in_page[j];
-      const uint32_t w = src[j * stride] | (src[(j + 1) * stride] << 8) | (src[(j + 2) * stride] << 16) | ((uint32_t)src[(j + 3) * stride] << 24);
-      *(uint32_t*)(page + at[j] + ((in >> 2) & 3) * 256 + (in >> 4) * 4) = w;
+    const long long to = group[4 * q + g];
+    if (to >= 0) {
+      uint8_t* page = a.cache + to + head;
+      for (int d = threadIdx.x >> 2; d < a.hd; d += 64) {
+        const uint8_t* src = vt + d + j * stride;
+        *(uint32_t*)(page + (d & ~15) * 64 + (d & 15) * 16) = src[0] | (src[stride] << 8) | (src[2 * stride] << 16) | ((uint32_t)src[3 * stride] << 24);
+      }
       continue;
     }
     for (int m = 0; m < 4; ++m) {
       const int jm = (j + m) & 63;            // the last group's rows past the tile are the first ones, before `lead`
       if (jm >= n || at[jm] < 0) continue;
       const int in = in_page[jm];
-      page[at[jm] + ((in >> 2) & 3) * 256 + (in >> 4) * 4 + (in & 3)] = src[jm * stride];
+      uint8_t* page = a.cache + at[jm] + head + Q8_PAGE * a.hd + ((in >> 2) & 3) * 256 + (in >> 4) * 4 + (in & 3);
+      for (int d = threadIdx.x >> 2; d < a.hd; d += 64) page[(d & ~15) * 64 + (d & 15) * 16] = vt[d + jm * stride];
     }
   }
 }
@@ -331,13 +430,15 @@ extern "C" const char* dlgo_rope_kv_q8(const void* qkv, int ld, void* q_out, int
               page_stride, ld, ldq, n_tokens, n_heads, n_kv, hd, rot, interleaved, table_rows, n_seq, n_slots, max_pages, n_pages};
   const bool pieces = rot % (interleaved ? 8 : 16) == 0 && ld % 8 == 0 && ldq % 8 == 0 && ((uintptr_t)qkv & 15) == 0 && ((uintptr_t)q_out & 15) == 0 &&
                       (!cos_t || (((uintptr_t)cos_t & 15) == 0 && ((uintptr_t)sin_t & 15) == 0));
-  int lanes = 2;
-  while (lanes * 8 < hd) lanes *= 2;
-  // a block of the many-rows kernel takes 64 rows of a head: from 128 rows on it stores whole lines where the other
-  // stores single bytes, below there are too few of its blocks
-  const bool tiles = n_tokens >= 128;
+  // The many-rows kernel stores whole lines where the other stores single bytes, but its blocks are long: it is faster from
+  // 512 rows of a prompt on (32 heads of 64 over 8: 128 rows 4.9 against 4.8 us, 512 rows 5.1 against 5.6, 1,024 6.0
+  // against 7.2, 17,408 rows of 24 heads of 128: 69 us).
+  const bool tiles = n_tokens >= 512;
+  int lanes = 1;
+  while (lanes * (tiles ? 16 : 8) < hd) lanes *= 2;
   const long long kv_blocks = !write_kv ? 0 : tiles ? (long long)((n_tokens + 63) / 64) * n_kv : ((long long)n_tokens * n_kv * lanes + 255) / 256;
-  const long long q_blocks = ((long long)n_tokens * n_heads * (hd / 8) + 255) / 256;
+  const QueryUnits u = query_units(n_heads, hd, rot, pieces, cos_t != nullptr, interleaved != 0);
+  const long long q_blocks = ((long long)n_tokens * u.groups * u.per_head + 255) / 256;
   DLGO_REQUIRE(kv_blocks + q_blocks < (1ll << 31), "rope_kv_q8: too many rows at once");
   const dim3 grid((unsigned)(kv_blocks + q_blocks));
   const int lds = 2 * 64 * (hd + 16);

@@ -717,13 +717,14 @@ def q8_page_bytes(n_kv: int, head_dim: int) -> int:
 
 def _q8_cache(name: str, cache: torch.Tensor, page_stride: int, n_kv: int, head_dim: int) -> int:
     """How many whole pages a cache tensor holds (the kernels touch no page beyond)."""
-    _need(cache, f"{name}: cache", torch.uint8, 1)
-    page = q8_page_bytes(n_kv, head_dim)
+    if not isinstance(cache, torch.Tensor) or cache.dtype is not torch.uint8 or cache.dim() != 1 or not cache.is_cuda:
+        _need(cache, f"{name}: cache", torch.uint8, 1)
     if head_dim % 16 or not 16 <= head_dim <= Q8_MAX_HEAD_DIM:
         raise KernelError(f"{name}: the 8-bit cache takes head sizes in steps of 16, up to {Q8_MAX_HEAD_DIM}, not {head_dim}")
-    if not cache.is_contiguous() or page_stride < page or cache.numel() < page:
-        raise KernelError(f"{name}: a cache of {cache.numel()} bytes with pages {page_stride} bytes apart does not hold pages of {page} bytes")
-    return min((cache.numel() - page) // page_stride + 1, 2 ** 31 - 1)
+    page, size = n_kv * 2 * PAGE * (head_dim + 1), cache.numel()
+    if page_stride < page or size < page or not cache.is_contiguous():
+        raise KernelError(f"{name}: a cache of {size} bytes with pages {page_stride} bytes apart does not hold pages of {page} bytes")
+    return min((size - page) // page_stride + 1, 2 ** 31 - 1)
 
 
 def _same_device(name: str, first: torch.Tensor, *others: Optional[torch.Tensor]) -> None:
@@ -735,18 +736,21 @@ def _same_device(name: str, first: torch.Tensor, *others: Optional[torch.Tensor]
         raise KernelError(f"{name}: tensors on {first.device}, the current device is cuda:{torch.cuda.current_device()}")
 
 
-def rope_kv_q8(qkv: torch.Tensor, q_out: torch.Tensor, n_heads: int, n_kv: int, head_dim: int, rot: int, interleaved: bool,
-               cos: Optional[torch.Tensor], sin: Optional[torch.Tensor], positions: torch.Tensor,
-               tok_seq: Optional[torch.Tensor], slots: Optional[torch.Tensor], page_table: Optional[torch.Tensor],
-               cache: Optional[torch.Tensor], page_stride: int, write_kv: bool = True) -> None:
-    """rope_kv() for the 8-bit cache: the query heads of qkv [T, (H+2KV)*hd] (bfloat16) rotated into q_out [T, H*hd], which
-    may be their own place in qkv; the key heads rotated and, with the values, stored in 8 bits in the page of each token
-    (cache: uint8, from the first byte of this layer's part of page 0 on; page_stride in bytes).  positions [T], tok_seq
-    [T] (each row's index into slots) and slots are int32.  A token's key (value) of a head is stored as e4m3 numbers times the least power of
-    two (from 2^-126 on) that brings its largest magnitude within 448; each element is rounded once, from float32.  A token whose key
-    or value is not finite is marked as a whole, and every row that sees it becomes NaN in that kv head's queries' results.
-    Rows whose position has no page (a hole in the table, a page the cache does not hold) store nothing.  Positions must
-    lie inside the rotation tables.  write_kv=False: queries only."""
+_BF16, _F32, _I32, _U8 = torch.bfloat16, torch.float32, torch.int32, torch.uint8
+
+
+def _current_device() -> int:
+    return _raw_device() if _raw_device is not None else torch.cuda.current_device()
+
+
+def _is_vector(t: torch.Tensor, n: int, dev: int, dtype: torch.dtype = _I32) -> bool:
+    """n elements of dtype in a row in memory, on device `dev`."""
+    return t.dtype is dtype and t.numel() == n and t.get_device() == dev and t.is_contiguous()
+
+
+def _rope_kv_q8_check(qkv, q_out, n_heads, n_kv, head_dim, rot, cos, sin, positions, tok_seq, slots, page_table, cache, write_kv):
+    """What rope_kv_q8() needs of its arguments, one after the other; returns (rows of the rotation tables, rows and
+    width of the page table, sequences)."""
     _need(qkv, "rope_kv_q8: qkv rows", torch.bfloat16, 2)
     _need(q_out, "rope_kv_q8: query rows", torch.bfloat16, 2)
     _need(positions, "rope_kv_q8: positions", torch.int32, 1)
@@ -768,7 +772,7 @@ def rope_kv_q8(qkv: torch.Tensor, q_out: torch.Tensor, n_heads: int, n_kv: int, 
         if cos.shape != sin.shape or cos.shape[1] != rot // 2 or not cos.is_contiguous() or not sin.is_contiguous():
             raise KernelError(f"rope_kv_q8: tables {tuple(cos.shape)} do not fit a rotated width of {rot}")
         table_rows = cos.shape[0]
-    n_pages = max_pages = n_slots = n_seq = 0
+    max_pages = n_slots = n_seq = 0
     if write_kv:
         for what, v, dims in (("token->sequence", tok_seq, 1), ("slots", slots, 1), ("page table", page_table, 2)):
             _need(v, f"rope_kv_q8: {what}", torch.int32, dims)
@@ -776,16 +780,83 @@ def rope_kv_q8(qkv: torch.Tensor, q_out: torch.Tensor, n_heads: int, n_kv: int, 
                 raise KernelError(f"rope_kv_q8: {what} must be contiguous")
         if tok_seq.shape[0] != t:
             raise KernelError("rope_kv_q8: one sequence index per row")
-        n_pages = _q8_cache("rope_kv_q8", cache, page_stride, n_kv, head_dim)
+        _need(cache, "rope_kv_q8: cache", torch.uint8, 1)
         n_slots, max_pages = page_table.shape
         n_seq = slots.shape[0]
     _same_device("rope_kv_q8", qkv, q_out, positions, cos, sin, *((tok_seq, slots, page_table, cache) if write_kv else ()))
+    return table_rows, n_slots, max_pages, n_seq
+
+
+def rope_kv_q8(qkv: torch.Tensor, q_out: torch.Tensor, n_heads: int, n_kv: int, head_dim: int, rot: int, interleaved: bool,
+               cos: Optional[torch.Tensor], sin: Optional[torch.Tensor], positions: torch.Tensor,
+               tok_seq: Optional[torch.Tensor], slots: Optional[torch.Tensor], page_table: Optional[torch.Tensor],
+               cache: Optional[torch.Tensor], page_stride: int, write_kv: bool = True) -> None:
+    """rope_kv() for the 8-bit cache: the query heads of qkv [T, (H+2KV)*hd] (bfloat16) rotated into q_out [T, H*hd], which
+    may be their own place in qkv; the key heads rotated and, with the values, stored in 8 bits in the page of each token
+    (cache: uint8, from the first byte of this layer's part of page 0 on; page_stride in bytes).  positions [T], tok_seq
+    [T] (each row's index into slots) and slots are int32.  A token's key (value) of a head is stored as e4m3 numbers times the least power of
+    two (from 2^-126 on) that brings its largest magnitude within 448; each element is rounded once, from float32.  A token whose key
+    or value is not finite is marked as a whole, and every row that sees it becomes NaN in that kv head's queries' results.
+    Rows whose position has no page (a hole in the table, a page the cache does not hold) store nothing.  Positions must
+    lie inside the rotation tables.  write_kv=False: queries only."""
+    # the usual call is told by one look at each tensor; any other goes through the checks that can say what is wrong
+    n_pages = max_pages = n_slots = n_seq = 0
+    try:
+        dev = qkv.get_device()
+        t, width = qkv.shape
+        table_rows, half = cos.shape
+        plain = (dev >= 0 and dev == _current_device() and n_heads > 0 and n_kv > 0 and head_dim > 0 and qkv.dtype is _BF16 and q_out.dtype is _BF16
+                 and q_out.shape == (t, n_heads * head_dim) and q_out.get_device() == dev
+                 and width >= (n_heads + (2 * n_kv if write_kv else 0)) * head_dim and _is_vector(positions, t, dev)
+                 and half * 2 == rot and sin.shape == cos.shape and _is_vector(cos, table_rows * half, dev, _F32) and _is_vector(sin, table_rows * half, dev, _F32))
+        if plain and write_kv:
+            n_slots, max_pages = page_table.shape
+            n_seq = slots.numel()
+            plain = (_is_vector(tok_seq, t, dev) and _is_vector(slots, n_seq, dev) and _is_vector(page_table, n_slots * max_pages, dev)
+                     and cache.get_device() == dev)
+    except (AttributeError, TypeError, ValueError):        # something that is no tensor, or has other dimensions
+        plain = False
+    if not plain:
+        table_rows, n_slots, max_pages, n_seq = _rope_kv_q8_check(qkv, q_out, n_heads, n_kv, head_dim, rot, cos, sin, positions, tok_seq,
+                                                                  slots, page_table, cache, write_kv)
+        t = qkv.shape[0]
+    if write_kv:
+        n_pages = _q8_cache("rope_kv_q8", cache, page_stride, n_kv, head_dim)
     if t == 0:
         return
     _check(_lib("kv_q8").dlgo_rope_kv_q8(_ptr(qkv), _rows(qkv, "rope_kv_q8: qkv rows"), _ptr(q_out), _rows(q_out, "rope_kv_q8: query rows"),
                                          t, n_heads, n_kv, head_dim, rot, int(interleaved), _ptr(cos), _ptr(sin), table_rows,
                                          _ptr(positions), _ptr(tok_seq), _ptr(slots), n_seq, _ptr(page_table), n_slots, max_pages,
                                          _ptr(cache), ctypes.c_longlong(page_stride), n_pages, int(write_kv), _stream()))
+
+
+def _attention_q8_check(q, out, n_heads, n_kv, head_dim, cu_q, start_pos, slots, page_table, cache, page_stride, max_q_len, max_kv_len, window):
+    """What attention_q8() needs of its arguments, one after the other."""
+    _need(q, "attention_q8: query rows", torch.bfloat16, 2)
+    _need(out, "attention_q8: output", torch.bfloat16, 2)
+    for what, v, dims in (("row offsets", cu_q, 1), ("start positions", start_pos, 1), ("slots", slots, 1), ("page table", page_table, 2)):
+        if v is None and what == "slots":
+            continue
+        _need(v, f"attention_q8: {what}", torch.int32, dims)
+        if not v.is_contiguous():
+            raise KernelError(f"attention_q8: {what} must be contiguous")
+    _q8_cache("attention_q8", cache, page_stride, n_kv, head_dim)
+    t, n_seq = q.shape[0], start_pos.shape[0]
+    if n_kv < 1 or n_heads % n_kv or q.shape[1] != n_heads * head_dim or out.shape != q.shape:
+        raise KernelError(f"attention_q8: query rows {tuple(q.shape)} and output {tuple(out.shape)} do not fit {n_heads} heads of {head_dim} over {n_kv} kv heads")
+    if cu_q.shape[0] != n_seq + 1 or (slots is not None and slots.shape[0] != n_seq) or (slots is None and page_table.shape[0] < n_seq):
+        raise KernelError("attention_q8: row offsets, start positions and slots do not fit each other")
+    if max_q_len < 0 or max_kv_len < 0 or window < 0:
+        raise KernelError("attention_q8: bounds and window must not be negative")
+    _same_device("attention_q8", q, out, cu_q, start_pos, slots, page_table, cache)
+
+
+@functools.lru_cache(maxsize=4096)
+def _attention_q8_scratch(head_dim, rows, n_seq, n_heads, n_kv, max_q_len, max_kv_len, window) -> int:
+    """Floats of scratch that a launch of these sizes needs."""
+    lib = _lib("attention_q8", (("HEAD_DIM", head_dim),))
+    lib.dlgo_attention_q8_scratch.restype = ctypes.c_longlong
+    return lib.dlgo_attention_q8_scratch(rows, n_seq, n_heads, n_kv, max_q_len, max_kv_len, window)
 
 
 def attention_q8(q: torch.Tensor, out: torch.Tensor, n_heads: int, n_kv: int, head_dim: int, cu_q: torch.Tensor,
@@ -802,39 +873,39 @@ def attention_q8(q: torch.Tensor, out: torch.Tensor, n_heads: int, n_kv: int, he
     rows a sequence brings and the tokens it holds afterwards: a captured step passes what it allows for; rows and
     tokens beyond the bounds are left out or slow, never out of bounds.  scratch(n) returns a float32 buffer of at least n elements for what
     several blocks find of a row (allocated here if not given).  A row that finds no page at all is zeros."""
-    _need(q, "attention_q8: query rows", torch.bfloat16, 2)
-    _need(out, "attention_q8: output", torch.bfloat16, 2)
-    for what, v, dims in (("row offsets", cu_q, 1), ("start positions", start_pos, 1), ("slots", slots, 1), ("page table", page_table, 2)):
-        if v is None and what == "slots":
-            continue
-        _need(v, f"attention_q8: {what}", torch.int32, dims)
-        if not v.is_contiguous():
-            raise KernelError(f"attention_q8: {what} must be contiguous")
+    # as in rope_kv_q8(): one look at each tensor, and the checks that can say what is wrong where that is not enough
+    try:
+        dev = q.get_device()
+        t, width = q.shape
+        n_seq = start_pos.numel()
+        n_slots, max_pages = page_table.shape
+        plain = (dev >= 0 and dev == _current_device() and n_kv > 0 and n_heads % n_kv == 0 and width == n_heads * head_dim and q.dtype is _BF16
+                 and out.dtype is _BF16 and out.shape == (t, width) and out.get_device() == dev and _is_vector(cu_q, n_seq + 1, dev)
+                 and _is_vector(start_pos, n_seq, dev) and (n_slots >= n_seq if slots is None else _is_vector(slots, n_seq, dev))
+                 and _is_vector(page_table, n_slots * max_pages, dev) and cache.get_device() == dev
+                 and max_q_len >= 0 and max_kv_len >= 0 and window >= 0)
+    except (AttributeError, TypeError, ValueError):
+        plain = False
+    if not plain:
+        _attention_q8_check(q, out, n_heads, n_kv, head_dim, cu_q, start_pos, slots, page_table, cache, page_stride, max_q_len, max_kv_len, window)
+        t, n_seq = q.shape[0], start_pos.shape[0]
+        n_slots, max_pages = page_table.shape
     n_pages = _q8_cache("attention_q8", cache, page_stride, n_kv, head_dim)
-    t, n_seq = q.shape[0], start_pos.shape[0]
-    if n_kv < 1 or n_heads % n_kv or q.shape[1] != n_heads * head_dim or out.shape != q.shape:
-        raise KernelError(f"attention_q8: query rows {tuple(q.shape)} and output {tuple(out.shape)} do not fit {n_heads} heads of {head_dim} over {n_kv} kv heads")
-    if cu_q.shape[0] != n_seq + 1 or (slots is not None and slots.shape[0] != n_seq) or (slots is None and page_table.shape[0] < n_seq):
-        raise KernelError("attention_q8: row offsets, start positions and slots do not fit each other")
-    if max_q_len < 0 or max_kv_len < 0 or window < 0:
-        raise KernelError("attention_q8: bounds and window must not be negative")
     if scale is None:
         scale = 1.0 / math.sqrt(head_dim)
-    _same_device("attention_q8", q, out, cu_q, start_pos, slots, page_table, cache)
     if t == 0 or n_seq == 0 or max_q_len == 0:
         return out
     max_q_len = min(int(max_q_len), t)
-    max_kv_len = max(1, min(int(max_kv_len), page_table.shape[1] * PAGE))
+    max_kv_len = max(1, min(int(max_kv_len), max_pages * PAGE))
+    need = _attention_q8_scratch(head_dim, t, n_seq, n_heads, n_kv, max_q_len, max_kv_len, int(window))
     lib = _lib("attention_q8", (("HEAD_DIM", head_dim),))
-    lib.dlgo_attention_q8_scratch.restype = ctypes.c_longlong
-    need = lib.dlgo_attention_q8_scratch(t, n_seq, n_heads, n_kv, max_q_len, max_kv_len, int(window))
     part = None
     if need:
         part = scratch(need) if scratch is not None else torch.empty(need, dtype=torch.float32, device=q.device)
         _need(part, "attention_q8: scratch", torch.float32, 1)
     _check(lib.dlgo_attention_q8(_ptr(q), _rows(q, "attention_q8: query rows"), _ptr(out), _rows(out, "attention_q8: output"), t, n_seq,
                                  n_heads, n_kv, head_dim, _ptr(cu_q), _ptr(start_pos), _ptr(slots), _ptr(page_table),
-                                 page_table.shape[0], page_table.shape[1], _ptr(cache), ctypes.c_longlong(page_stride), n_pages,
+                                 n_slots, max_pages, _ptr(cache), ctypes.c_longlong(page_stride), n_pages,
                                  max_q_len, max_kv_len, int(window), ctypes.c_float(scale), _ptr(part),
                                  ctypes.c_longlong(part.numel() if part is not None else 0), _stream()))
     return out
@@ -902,25 +973,10 @@ def sample(logits: torch.Tensor, work: torch.Tensor, temperature: torch.Tensor, 
     return out
 
 
-def verify_drafts(logits: torch.Tensor, draft_tokens: torch.Tensor, cu_drafts: torch.Tensor, temperature: torch.Tensor,
-                  uniform: torch.Tensor, accepted: torch.Tensor, token: torch.Tensor, max_drafts: int,
-                  draft_logits: Optional[torch.Tensor] = None, probs: Optional[torch.Tensor] = None, scratch=None) -> None:
-    """How many of each sequence's drafted tokens the target model keeps, and the token that follows them.
-
-    Sequence i drafted the tokens cu_drafts[i] to cu_drafts[i+1] of draft_tokens (int32, D in all; none is allowed, more
-    than max_drafts are not looked at) and
-    brings one row of the target's float32 logits [D + n, V] for the place of each draft and one for the place after them,
-    from row cu_drafts[i] + i on; uniform [D + n] has a number in [0, 1) for each of those rows.  temperature [n]; 0 is
-    greedy.  draft_logits [D, V]: the logits that the drafts were drawn from (at the same temperature); None: the drafts
-    are certain of their tokens (looked up, or a greedy draft model's).
-
-    With p = softmax(logits / T) and q = softmax(draft_logits / T) (or one for the drafted token), draft j is kept while
-    uniform_j * q(token_j) < p(token_j); accepted[i] (int32) counts the kept ones, token[i] (int32) is drawn from max(p - q, 0)
-    of the first refused draft's row, or from p of the last row, as the first index whose running sum exceeds the
-    sequence's last uniform number times the whole.  Greedy: a draft is kept if it is the row's maximum (lowest index), and the token is
-    the maximum.  Sums are 64-bit, in an order that only the shapes decide.  A logit of -inf or NaN has no weight.  A token
-    outside the vocabulary is refused.  probs [D] (float32, optional): p(token_j) for every draft.  scratch(n) returns a uint8 buffer of at least n
-    bytes (allocated here if not given)."""
+def _verify_drafts_check(logits, draft_tokens, cu_drafts, temperature, uniform, accepted, token, max_drafts, draft_logits, probs):
+    """What verify_drafts() needs of its arguments, one after the other."""
+    _need(temperature, "verify_drafts: temperature", torch.float32, 1)
+    _need(draft_tokens, "verify_drafts: draft tokens", torch.int32, 1)
     _need(logits, "verify_drafts: logits", torch.float32, 2)
     n, v = temperature.shape[0], logits.shape[1]
     d = draft_tokens.shape[0]
@@ -941,12 +997,55 @@ def verify_drafts(logits: torch.Tensor, draft_tokens: torch.Tensor, cu_drafts: t
     if max_drafts < 0:
         raise KernelError("verify_drafts: max_drafts must not be negative")
     _same_device("verify_drafts", logits, draft_tokens, cu_drafts, temperature, uniform, accepted, token, draft_logits, probs)
+
+
+@functools.lru_cache(maxsize=4096)
+def _verify_drafts_scratch(n, d, vocab, model_drafts) -> int:
+    """Bytes of scratch that a call of these sizes needs."""
+    lib = _lib("verify")
+    lib.dlgo_verify_drafts_scratch.restype = ctypes.c_longlong
+    return lib.dlgo_verify_drafts_scratch(n, d, vocab, int(model_drafts))
+
+
+def verify_drafts(logits: torch.Tensor, draft_tokens: torch.Tensor, cu_drafts: torch.Tensor, temperature: torch.Tensor,
+                  uniform: torch.Tensor, accepted: torch.Tensor, token: torch.Tensor, max_drafts: int,
+                  draft_logits: Optional[torch.Tensor] = None, probs: Optional[torch.Tensor] = None, scratch=None) -> None:
+    """How many of each sequence's drafted tokens the target model keeps, and the token that follows them.
+
+    Sequence i drafted the tokens cu_drafts[i] to cu_drafts[i+1] of draft_tokens (int32, D in all; none is allowed, more
+    than max_drafts are not looked at) and
+    brings one row of the target's float32 logits [D + n, V] for the place of each draft and one for the place after them,
+    from row cu_drafts[i] + i on; uniform [D + n] has a number in [0, 1) for each of those rows.  temperature [n]; 0 is
+    greedy.  draft_logits [D, V]: the logits that the drafts were drawn from (at the same temperature); None: the drafts
+    are certain of their tokens (looked up, or a greedy draft model's).
+
+    With p = softmax(logits / T) and q = softmax(draft_logits / T) (or one for the drafted token), draft j is kept while
+    uniform_j * q(token_j) < p(token_j); accepted[i] (int32) counts the kept ones, token[i] (int32) is drawn from max(p - q, 0)
+    of the first refused draft's row, or from p of the last row, as the first index whose running sum exceeds the
+    sequence's last uniform number times the whole.  Greedy: a draft is kept if it is the row's maximum (lowest index), and the token is
+    the maximum.  Sums are 64-bit, in an order that only the shapes decide.  A logit of -inf or NaN has no weight.  A token
+    outside the vocabulary is refused.  probs [D] (float32, optional): p(token_j) for every draft.  scratch(n) returns a uint8 buffer of at least n
+    bytes (allocated here if not given)."""
+    # as in rope_kv_q8(): one look at each tensor, and the checks that can say what is wrong where that is not enough
+    try:
+        dev = logits.get_device()
+        n, d = temperature.numel(), draft_tokens.numel()
+        rows, v = logits.shape
+        plain = (dev >= 0 and dev == _current_device() and logits.dtype is _F32 and rows == d + n and v > 0 and max_drafts >= 0
+                 and _is_vector(temperature, n, dev, _F32) and _is_vector(draft_tokens, d, dev) and _is_vector(cu_drafts, n + 1, dev)
+                 and _is_vector(uniform, d + n, dev, _F32) and _is_vector(accepted, n, dev) and _is_vector(token, n, dev)
+                 and (probs is None or _is_vector(probs, d, dev, _F32))
+                 and (draft_logits is None or (draft_logits.dtype is _F32 and draft_logits.shape == (d, v) and draft_logits.get_device() == dev)))
+    except (AttributeError, TypeError, ValueError):
+        plain = False
+    if not plain:
+        _verify_drafts_check(logits, draft_tokens, cu_drafts, temperature, uniform, accepted, token, max_drafts, draft_logits, probs)
+        n, d, v = temperature.shape[0], draft_tokens.shape[0], logits.shape[1]
     if n == 0:
         return
     model_drafts = draft_logits is not None and d > 0
     lib = _lib("verify")
-    lib.dlgo_verify_drafts_scratch.restype = ctypes.c_longlong
-    need = lib.dlgo_verify_drafts_scratch(n, d, v, int(model_drafts))
+    need = _verify_drafts_scratch(n, d, v, model_drafts)
     work = scratch(need) if scratch is not None else torch.empty(need, dtype=torch.uint8, device=logits.device)
     _need(work, "verify_drafts: scratch", torch.uint8, 1)
     _check(lib.dlgo_verify_drafts(_ptr(logits), ctypes.c_longlong(_rows(logits, "verify_drafts: logits")), _ptr(draft_tokens),

@@ -177,6 +177,16 @@ STORES = [   # q_lens, past, H, KV, hd, rot, interleaved
     ([129, 1, 17], [2, 700, 30], 5, 1, 256, 256, False),
     ([300], [1], 2, 1, 32, 6, True),
     ([1] * 140, [(37 * i) % 200 for i in range(140)], 4, 2, 64, 32, False),      # many rows, each of another sequence
+    # from 512 rows on another kernel, with every offset in a page and a word
+    ([600], [0], 4, 2, 64, 64, False),
+    ([130, 70, 400], [1, 62, 3], 8, 2, 128, 128, False),
+    ([64, 64, 65, 3, 500], [0, 64, 63, 6, 1], 3, 3, 16, 8, True),
+    ([513], [2], 5, 1, 256, 256, False),
+    ([300, 300], [61, 7], 2, 1, 32, 6, True),
+    ([600], [3], 9, 2, 80, 64, False),
+    ([700], [64], 6, 3, 48, 48, False),
+    ([1] * 530, [(37 * i) % 200 for i in range(530)], 4, 2, 64, 32, False),
+    ([1, 5, 2] * 70, [(41 * i) % 130 for i in range(210)], 4, 1, 32, 32, True),
 ]
 
 
@@ -217,22 +227,23 @@ def test_store(q_lens, past, H, KV, hd, rot, inter):
     assert same[~touched].all(), "bytes of other tokens were written"
 
 
-def test_store_in_place_and_queries_only():
-    s = Step([70, 90], [10, 0], 8, 2, 64, seed=3)
-    cos, sin = tables(200, 64)
+@pytest.mark.parametrize("q_lens", [[70, 90], [400, 190]])
+def test_store_in_place_and_queries_only(q_lens):
+    s = Step(q_lens, [10, 0], 8, 2, 64, seed=3)
+    cos, sin = tables(500, 64)
     q = s.store(cos=cos, sin=sin)
     pages = s.storage.clone()
     kv = s.qkv[:, 8 * 64:].clone()
     s.store(q_out=s.qkv[:, :8 * 64], cos=cos, sin=sin)       # into their own place
     assert torch.equal(s.qkv[:, :8 * 64], q) and torch.equal(s.qkv[:, 8 * 64:], kv) and torch.equal(s.storage, pages)
-    s2 = Step([70, 90], [10, 0], 8, 2, 64, seed=3)
+    s2 = Step(q_lens, [10, 0], 8, 2, 64, seed=3)
     before = s2.storage.clone()
     q2 = torch.empty_like(q)
     _ops().rope_kv_q8(s2.qkv, q2, 8, 2, 64, 64, False, cos, sin, i32(s2.pos), None, None, None, None, 0, write_kv=False)
     assert torch.equal(q2, q) and torch.equal(s2.storage, before)
 
 
-@pytest.mark.parametrize("rows", [3, 150])
+@pytest.mark.parametrize("rows", [3, 150, 520])
 def test_store_of_zeros_tiny_huge_and_what_is_not_finite(rows):
     H, KV, hd = 2, 2, 32
     s = Step([rows], [0], H, KV, hd, seed=11)
@@ -262,7 +273,7 @@ def test_store_of_zeros_tiny_huge_and_what_is_not_finite(rows):
 
 
 def test_store_writes_nothing_where_there_is_no_page():
-    for rows in (5, 140):
+    for rows in (5, 140, 600):
         s = Step([rows, 7], [0, 0], 4, 2, 64, seed=rows)
         table = s.table.copy()
         s.table[s.slots[0], 0] = -1                       # a hole
