@@ -116,8 +116,9 @@ class LLM:
 
     def model_info(self) -> str:
         """dlgo.go:170-185."""
+        kept = self.engine.cache.kv_dtype
         return " | ".join([self.config.architecture, *self.config.describe(), f"ctx {self.max_seq_len}",
-                           str(self.engine.dtype).replace('torch.', '')])
+                           str(self.engine.dtype).replace('torch.', ''), *([f"cache {kept}"] if kept else [])])
 
 
 def load_llm(model: Union[str, ModelConfig, Mapping], max_seq_len: int = 0, dtype: str = "bfloat16", device: str = "cuda:0",
@@ -129,7 +130,8 @@ def load_llm(model: Union[str, ModelConfig, Mapping], max_seq_len: int = 0, dtyp
     max_seq_len <= 0 or beyond the model's context means the model's context (models/llm/generate.go:56-58).  The
     cache is sized for `max_tokens` tokens over all live sequences; by default for max_batch sequences of max_seq_len,
     or for as many tokens as the device's free memory holds once the weights are loaded (a fifth of it stays free,
-    and room for the recordings of steps), if that is less."""
+    and room for the recordings of steps), if that is less.  cache_dtype="e4m3" keeps keys and values in 8 bits: about
+    twice the tokens in the same memory, and half the bytes a step reads of them.  Other options are Engine's."""
     if isinstance(model, ModelConfig):
         config = model
     elif isinstance(model, Mapping):
@@ -152,7 +154,8 @@ def load_llm(model: Union[str, ModelConfig, Mapping], max_seq_len: int = 0, dtyp
         del tensors
     if max_tokens is None:
         free, _ = torch.cuda.mem_get_info(torch.device(device))
-        fit = tokens_that_fit(built.unit_needs, rd, free, recordings_bytes(built.vocab, max_batch, **engine_options))
+        fit = tokens_that_fit(built.unit_needs, rd, free, recordings_bytes(built.vocab, max_batch, **engine_options),
+                              kv_dtype=engine_options.get("cache_dtype"))
         if fit < PAGE:
             raise EngineError(f"no device memory left for a cache ({free >> 20} MiB free after the weights)")
         max_tokens = fit if ctx is None else min(max_batch * ctx, fit)

@@ -15,7 +15,10 @@ that is zero-filled on reset (memory/ssmstate.go:4-69).  Here:
 * giving a slot back returns its pages at once; data is never cleared, because
   attention reads positions below the length only;
 * fixed-size state lives in [slot, ...] tensors per unit and is zeroed when a
-  slot is handed out.
+  slot is handed out;
+* with kv_dtype "e4m3" keys and values are kept in 8 bits: an e4m3 number an element
+  and a power of two for each token's key and value of a head (csrc/q8_page.h),
+  about half the bytes of a bfloat16 cache.  Everything above is the same.
 
 The bookkeeping is plain host code and runs without a GPU.
 """
@@ -75,14 +78,29 @@ class GroupSpec:
     units: List[int] = field(default_factory=list)     # cache unit ids, in storage order
 
 
+KV_DTYPES = (None, "e4m3")      # how keys and values are kept: in the run dtype, or in 8 bits
+
+
+def _check_kv_dtype(kv_dtype: Optional[str]) -> None:
+    if kv_dtype not in KV_DTYPES:
+        raise CacheError(f"cache: keys and values are kept in the run dtype (None) or in \"e4m3\", not {kv_dtype!r}")
+
+
 class KVGroup:
     def __init__(self, spec: GroupSpec, n_pages: int, max_slots: int, max_pages_per_seq: int,
-                 dtype: torch.dtype, device: torch.device):
+                 dtype: torch.dtype, device: torch.device, kv_dtype: Optional[str] = None):
         self.spec = spec
         self.pool = PagePool(n_pages)
-        self.unit_elems = 2 * spec.kv_heads * PAGE * spec.head_dim     # keys then values of one unit in a page
-        self.page_stride = self.unit_elems * len(spec.units)
+        self.q8 = kv_dtype == "e4m3"
         self.v_off = spec.kv_heads * PAGE * spec.head_dim
+        if self.q8:          # bytes: each head's keys, values and powers of two lie together
+            if spec.head_dim % 16 or spec.head_dim > 256:
+                raise CacheError(f"cache: e4m3 keys and values take head sizes in steps of 16, up to 256, not {spec.head_dim}")
+            self.unit_elems = spec.kv_heads * 2 * PAGE * (spec.head_dim + 1)
+            dtype = torch.uint8
+        else:
+            self.unit_elems = 2 * spec.kv_heads * PAGE * spec.head_dim     # keys then values of one unit in a page
+        self.page_stride = self.unit_elems * len(spec.units)
         # never cleared and never read beyond a sequence's length
         self.storage = torch.empty(n_pages * self.page_stride, dtype=dtype, device=device)
         self.table_host = np.full((max_slots, max_pages_per_seq), -1, dtype=np.int32)
@@ -109,11 +127,14 @@ class KVGroup:
 
 class Cache:
     def __init__(self, unit_needs: Sequence[Sequence[CacheNeed]], max_tokens: int, max_ctx: int, dtype: torch.dtype,
-                 device, max_slots: Optional[int] = None, max_step_tokens: Optional[int] = None):
+                 device, max_slots: Optional[int] = None, max_step_tokens: Optional[int] = None, kv_dtype: Optional[str] = None):
         """unit_needs[u]: what cache unit u asks for.  max_tokens: the most tokens live sequences hold together,
-        each sequence rounded up to whole pages.  max_ctx: the longest sequence."""
+        each sequence rounded up to whole pages.  max_ctx: the longest sequence.  kv_dtype: None keeps keys and values
+        in `dtype`, "e4m3" in 8 bits."""
+        _check_kv_dtype(kv_dtype)
         self.device = torch.device(device)
         self.dtype = dtype
+        self.kv_dtype = kv_dtype
         if max_tokens < 1 or max_ctx < 1:
             raise CacheError("cache: max_tokens and max_ctx must be positive")
         self.n_pages = (max_tokens + PAGE - 1) // PAGE
@@ -149,7 +170,7 @@ class Cache:
             if spec.window is not None:
                 per_seq = min(per_seq, (spec.window + min(self.max_step_tokens, self.max_ctx) + PAGE - 1) // PAGE + 1)
                 n_pages = min(n_pages, self.max_slots * per_seq)
-            group = KVGroup(spec, n_pages, self.max_slots, self.max_pages_per_seq, dtype, self.device)
+            group = KVGroup(spec, n_pages, self.max_slots, self.max_pages_per_seq, dtype, self.device, kv_dtype)
             group.pages_per_seq = per_seq       # the most pages one sequence holds of this group at any time
             self.groups.append(group)
 
@@ -248,6 +269,33 @@ class Cache:
             t[dst].copy_(t[src])
         return dst
 
+    def rewind(self, slot: int, length: int) -> None:
+        """The slot holds its first `length` tokens only, as if the others had never been given to it (drafted tokens that
+        were refused); the pages that held nothing else go back.  State is not a function of a length: with state units
+        a slot cannot be rewound; a windowed group must still hold every page that a token at `length` sees."""
+        self._check_live(slot)
+        have = int(self.lengths[slot])
+        if not 0 <= length <= have:
+            raise CacheError(f"rewind: slot {slot} holds {have} tokens, {length} asked")
+        if length == have:
+            return
+        if self.state:
+            raise CacheError("rewind: per-sequence state cannot be taken back to an earlier length")
+        plans = []
+        for gi, g in enumerate(self.groups):
+            held = self._held[slot][gi]
+            last = (length - 1) // PAGE if length > 0 else -1
+            missing = [i for i in range(g.first_needed_page(length), last + 1) if i not in held]
+            if missing:
+                raise CacheError(f"rewind: slot {slot} no longer holds pages {missing} that a token at {length} sees")
+            plans.append([i for i in held if i > last])
+        for gi, (g, gone) in enumerate(zip(self.groups, plans)):
+            if gone:
+                g.pool.give([self._held[slot][gi].pop(i) for i in gone])
+                g.table_host[slot, gone] = -1
+                g.touch(slot)
+        self.lengths[slot] = length
+
     def _check_live(self, slot: int) -> None:
         if not (0 <= slot < self.max_slots) or not self._live[slot]:
             raise CacheError(f"slot {slot} is not in use")
@@ -308,14 +356,25 @@ class Cache:
                     g.table_host[slot, i] = p
                 g.touch(slot)
 
-    def advance(self, slot: int, n_tokens: int) -> None:
-        """The slot now holds n_tokens more; pages no later token can see go back to their pool."""
+    def advance(self, slot: int, n_tokens: int, sure: Optional[int] = None) -> None:
+        """The slot now holds n_tokens more; pages no later token can see go back to their pool.  sure: the slot may yet
+        be rewound to a length down to this one, so what a token there sees is kept until settle()."""
         self._check_live(slot)
         self.lengths[slot] += n_tokens
+        self._give_unseen(slot, int(self.lengths[slot]) if sure is None else min(sure, int(self.lengths[slot])))
+
+    def settle(self, slots: Sequence[int]) -> None:
+        """The slots are not rewound any more: what advance() kept for that goes back."""
+        if self.has_windows:
+            for slot in slots:
+                self._check_live(slot)
+                self._give_unseen(slot, int(self.lengths[slot]))
+
+    def _give_unseen(self, slot: int, length: int) -> None:
         for gi, g in enumerate(self.groups):
             if g.spec.window is None:
                 continue
-            first = g.first_needed_page(int(self.lengths[slot]))
+            first = g.first_needed_page(length)
             held = self._held[slot][gi]
             gone = [i for i in held if i < first]
             if gone:
@@ -381,7 +440,7 @@ class Cache:
     def kv_view(self, unit: int) -> "KVView":
         gi, ui = self.unit_group[unit]
         g = self.groups[gi]
-        return KVView(g.unit_view(ui), g.page_stride, g.v_off, g.table, g.spec.kv_heads, g.spec.head_dim, g.spec.window, gi)
+        return KVView(g.unit_view(ui), g.page_stride, g.v_off, g.table, g.spec.kv_heads, g.spec.head_dim, g.spec.window, gi, g.q8)
 
     def state_of(self, unit: int) -> torch.Tensor:
         return self.state[unit]
@@ -408,18 +467,20 @@ class Cache:
             raise CacheError("slot accounting broken")
 
 
-def kv_bytes_per_token(unit_needs: Sequence[Sequence[CacheNeed]], dtype: torch.dtype) -> int:
+def kv_bytes_per_token(unit_needs: Sequence[Sequence[CacheNeed]], dtype: torch.dtype, kv_dtype: Optional[str] = None) -> int:
     """Bytes of keys and values that one token adds over all cache units (a windowed unit counts like a full one)."""
+    _check_kv_dtype(kv_dtype)
     item = torch.empty(0, dtype=dtype).element_size()
-    return sum(2 * need.kv_heads * need.head_dim * item for needs in unit_needs for need in needs if need.kind == "kv")
+    per_head = lambda hd: hd * item if kv_dtype is None else hd + 1      # a byte an element and one for the power of two
+    return sum(2 * need.kv_heads * per_head(need.head_dim) for needs in unit_needs for need in needs if need.kind == "kv")
 
 
 def tokens_that_fit(unit_needs: Sequence[Sequence[CacheNeed]], dtype: torch.dtype, free_bytes: int, recordings_bytes: int = 0,
-                    keep_free: float = 0.2, reserve_bytes: int = 2 << 30) -> int:
+                    keep_free: float = 0.2, reserve_bytes: int = 2 << 30, kv_dtype: Optional[str] = None) -> int:
     """How many tokens (a whole number of pages) a cache may be sized for when `free_bytes` of device memory are left:
     a fifth of it and 2 GiB stay free for the step's buffers, and `recordings_bytes` for what the recordings of steps
     will keep (they do not exist yet when the cache is sized)."""
-    per_token = kv_bytes_per_token(unit_needs, dtype)
+    per_token = kv_bytes_per_token(unit_needs, dtype, kv_dtype)
     budget = int(free_bytes * (1.0 - keep_free)) - reserve_bytes - int(recordings_bytes)
     if per_token == 0:
         return 1 << 20
@@ -437,3 +498,4 @@ class KVView:
     head_dim: int
     window: Optional[int]
     group: int = 0             # index of the storage group (its page table is shared by the group's units)
+    q8: bool = False           # 8-bit pages (csrc/q8_page.h): `cache` is bytes, page_stride counts them, v_off means nothing

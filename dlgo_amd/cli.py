@@ -32,6 +32,10 @@ def main(argv=None) -> int:
     ap.add_argument("--seed", type=int, default=-1, help="sampling seed (< 0: from the clock)")
     ap.add_argument("--ignore-eos", action="store_true", help="do not stop at stop tokens")
     ap.add_argument("--dtype", default="bfloat16", choices=["bfloat16", "float32"])
+    ap.add_argument("--cache-dtype", choices=["e4m3"], default=None,
+                    help="keep keys and values in 8 bits (bfloat16 runs; default: in the run's own dtype)")
+    ap.add_argument("--lookup-drafts", type=int, default=0, metavar="N",
+                    help="draft up to N tokens a step from the text itself (with --greedy, or with top-k, top-p and penalty off)")
     ap.add_argument("--prompt-ids", action="append", default=[], help="a prompt as token ids, e.g. 1,15,27 (repeatable)")
     ap.add_argument("--prompts-file", help="a file with one prompt of token ids per line")
     ap.add_argument("--random-config", metavar="CONFIG_JSON",
@@ -77,16 +81,17 @@ def main(argv=None) -> int:
     except (OSError, ValueError) as e:
         print(f"Error reading prompts (token ids separated by commas or spaces): {e}", file=sys.stderr)
         return 1
-    from . import (with_greedy, with_ignore_eos, with_max_tokens, with_min_p, with_repetition_penalty, with_seed,
-                   with_temperature, with_top_k, with_top_p)
+    from . import (with_greedy, with_ignore_eos, with_lookup_drafts, with_max_tokens, with_min_p, with_repetition_penalty,
+                   with_seed, with_temperature, with_top_k, with_top_p)
     from .api import load_llm
+    kept = {"cache_dtype": args.cache_dtype} if args.cache_dtype else {}
     try:
         batch = max(1, min(64, len(prompts) or 1))
         if args.random_config:
             llm = load_llm(args.random_config, args.ctx, args.dtype, max_batch=batch, random_seed=args.weight_seed,
-                           random_std=args.weight_std)
+                           random_std=args.weight_std, **kept)
         else:
-            llm = load_llm(args.model, args.ctx, args.dtype, max_batch=batch)
+            llm = load_llm(args.model, args.ctx, args.dtype, max_batch=batch, **kept)
     except Exception as e:
         print(f"Error loading model: {e}", file=sys.stderr)
         return 1
@@ -102,6 +107,8 @@ def main(argv=None) -> int:
         opts.append(with_greedy())
     if args.ignore_eos:
         opts.append(with_ignore_eos())
+    if args.lookup_drafts:
+        opts.append(with_lookup_drafts(args.lookup_drafts))
     try:
         results = llm.generate(prompts, *opts)
     except Exception as e:

@@ -66,10 +66,13 @@ def _require_gpu() -> None:
 @dataclass
 class Entry:
     """One sequence's part of a step: its slot, its next tokens, and the places among
-    these tokens whose logits are wanted."""
+    these tokens whose logits are wanted.  `undecided`: so many of the last tokens may be
+    taken back by rewind() before the slot's next step (drafts), so what a window needs
+    for that is kept."""
     slot: int
     tokens: Sequence[int]
     want: Sequence[int] = ()
+    undecided: int = 0
 
 
 @dataclass
@@ -91,11 +94,12 @@ class Engine:
     def __init__(self, model, dtype="bfloat16", device="cuda:0", max_tokens: int = 8192, max_ctx: Optional[int] = None,
                  max_slots: Optional[int] = None, max_step_tokens: int = 8192, logits_rows: int = 1024,
                  use_graphs: bool = True, graph_max_batch: int = 128, prompt_graph_max_tokens: int = 4096,
-                 prompt_graph_limit: int = 32, prompt_graph_bytes: int = 1 << 30):
+                 prompt_graph_limit: int = 32, prompt_graph_bytes: int = 1 << 30, cache_dtype: Optional[str] = None):
         """`model` holds its weights already (see from_folder / from_random).  use_graphs: steps of single tokens are
         recorded per batch size, and steps of fresh prompts of up to prompt_graph_max_tokens rows per shape (the
         prompt_graph_limit most recently used shapes are kept, as long as the logits they keep stay within
-        prompt_graph_bytes), the second time a size or shape is seen."""
+        prompt_graph_bytes), the second time a size or shape is seen.  cache_dtype: None keeps keys and values in the run
+        dtype, "e4m3" in 8 bits (bfloat16 runs only: half the cache's bytes, each element rounded to 4 significant bits)."""
         _require_gpu()
         self.model = model
         self.dtype = run_dtype(dtype)
@@ -111,9 +115,17 @@ class Engine:
                 part.check(self.dtype)
             except ValueError as e:
                 raise EngineError(f"{name}: {e}") from None
-        kernel_build.ensure_built(model.kernel_variants(self.dtype))
-        self.cache = Cache(model.unit_needs, max_tokens, self.max_ctx, self.dtype, self.device, max_slots,
-                           self.max_step_tokens)
+        if cache_dtype is not None and self.dtype != torch.bfloat16:
+            raise EngineError(f"a cache in {cache_dtype} goes with a bfloat16 run: the float32 path rounds nothing to fewer bits")
+        variants = list(model.kernel_variants(self.dtype))
+        for _, part in model.named_parts():
+            variants += [v for v in part.cache_kernel_variants(cache_dtype) if v not in variants]
+        try:
+            self.cache = Cache(model.unit_needs, max_tokens, self.max_ctx, self.dtype, self.device, max_slots,
+                               self.max_step_tokens, cache_dtype)
+        except CacheError as e:
+            raise EngineError(str(e)) from None
+        kernel_build.ensure_built(variants)
         self.workspace = Workspace(self.device, self.max_step_tokens)
         model.prepare(self.max_ctx, self.device)
         self.vocab = model.vocab
@@ -181,6 +193,19 @@ class Engine:
             raise EngineError(f"fork: {e}") from None
         self.cache.sync_tables()
         return new
+
+    @property
+    def can_rewind(self) -> bool:
+        """Nothing but keys and values is kept of a sequence, so it can be taken back to an earlier length."""
+        return not self.cache.state
+
+    def rewind(self, slot: int, length: int) -> None:
+        """The sequence holds its first `length` tokens only from now on: what a step gave it beyond (drafted tokens that
+        were refused) is forgotten, and the next step goes on from there."""
+        try:
+            self.cache.rewind(slot, length)
+        except CacheError as e:
+            raise EngineError(str(e)) from None
 
     def close(self, slots: Sequence[int]) -> None:
         for s in slots:
@@ -305,6 +330,8 @@ class Engine:
                 raise EngineError(f"step: slot {e.slot} brings no tokens")
             if start + n > self.max_ctx:
                 raise EngineError(f"step: slot {e.slot} would hold {start + n} tokens, the context is {self.max_ctx}")
+            if not 0 <= e.undecided <= n or e.undecided > self.max_step_tokens:
+                raise EngineError(f"step: slot {e.slot} brings {n} tokens (at most {self.max_step_tokens} a piece), {e.undecided} of them undecided")
             for w in e.want:
                 if not 0 <= w < n:
                     raise EngineError(f"step: slot {e.slot} wants logits at place {w} of {n} tokens")
@@ -314,13 +341,14 @@ class Engine:
         if tokens.min() < 0 or tokens.max() >= self.vocab:
             bad = int(tokens[(tokens < 0) | (tokens >= self.vocab)][0])
             raise EngineError(f"step: token id {bad} is outside the vocabulary of {self.vocab}")
+        self.cache.settle(seen)
         why = self.cache.can_reserve([(e.slot, s + n) for e, s, n in zip(entries, starts, q_lens)])
         if why:
             raise EngineError(f"step: {why}")
         self.steps_run += 1
 
         if (sink is None
-                and all(n == 1 for n in q_lens) and all(list(e.want) == [0] for e in entries)):
+                and all(n == 1 for n in q_lens) and all(list(e.want) == [0] and not e.undecided for e in entries)):
             self.steps_run -= 1
             # decode() hands out a view of a buffer that the next step overwrites; a step's result is the caller's to keep
             return self.decode([e.slot for e in entries], tokens, checked=True).clone()
@@ -371,8 +399,8 @@ class Engine:
             else:
                 arrays = self._upload(fields)
                 self._run_piece(StepContext(self, len(seqs), c1 - c0, arrays, host), arrays, sel, out, sink)
-            for sl, q in zip(slots, piece_q):
-                self.cache.advance(int(sl), int(q))
+            for i, sl, q in zip(seqs, slots, piece_q):
+                self.cache.advance(int(sl), int(q), starts[i] + q_lens[i] - entries[i].undecided)
         return out
 
     def _run_piece(self, ctx: StepContext, arrays: Dict[str, torch.Tensor], sel: np.ndarray, out: Optional[torch.Tensor],
@@ -487,6 +515,7 @@ class Engine:
             if (starts + 1 > self.max_ctx).any():
                 raise EngineError(f"decode: a sequence would exceed the context of {self.max_ctx}")
             if needs_pages:
+                self.cache.settle(slots)
                 why = self.cache.can_reserve([(int(s), int(st) + 1) for s, st in zip(slot_arr, starts)])
                 if why:
                     raise EngineError(f"decode: {why}")

@@ -16,8 +16,10 @@ through a handful of calls, so its decisions can be tested with stand-ins:
 
     engine:  open(n) -> slots, close(slots), step(entries) -> logits rows (the prompts),
              decode(slots, ids) -> logits rows (one token each; ids as the sampler left them on the device),
-             max_ctx, free_slots(), free_pages() and page_demand(n_tokens) (per storage group of the cache)
-    sampler: start(keys), choose_async(logits, configs, uniforms, keys=) -> (ids on the device, wait() -> ids on the host)
+             max_ctx, free_slots(), free_pages() and page_demand(n_tokens) (per storage group of the cache);
+             where drafts are wanted also rewind(slot, length) (and can_rewind)
+    sampler: start(keys), choose_async(logits, configs, uniforms, keys=) -> (ids on the device, wait() -> ids on the host);
+             where drafts are wanted also verify(logits, drafts, configs, uniforms) -> (kept counts, tokens)
 
 The loop runs one step ahead of the host: the step that feeds the tokens just
 chosen is queued before those tokens reach the host, so the GPU does not wait
@@ -56,6 +58,8 @@ class Stats:
     batches: int = 0
     steps: int = 0
     step_ms: List[float] = field(default_factory=list)
+    drafted_tokens: int = 0        # drafts that were verified, and those of them that were kept
+    kept_drafts: int = 0
 
     @property
     def tokens_per_sec(self) -> float:
@@ -159,6 +163,105 @@ def _decode_batch(engine, sampler, live, logits, prompts, results, stats, on_tok
         live = [live[r] for r in still]
 
 
+class LookupDrafts:
+    """Drafts from a request's own text: what followed the last place where its last three tokens (else two) stood."""
+
+    GRAMS = (3, 2)
+
+    def __init__(self, tokens: Sequence[int]):
+        self.tokens: List[int] = []
+        self._after = {}                     # the last tokens of some place -> the index of the token that followed them
+        self.extend(tokens)
+
+    def extend(self, tokens: Sequence[int]) -> None:
+        for t in tokens:
+            n = len(self.tokens)
+            for g in self.GRAMS:
+                if n >= g:
+                    self._after[tuple(self.tokens[n - g:])] = n
+            self.tokens.append(int(t))
+
+    def propose(self, most: int) -> List[int]:
+        if most < 1:
+            return []
+        for g in self.GRAMS:
+            if len(self.tokens) >= g:
+                at = self._after.get(tuple(self.tokens[-g:]))
+                if at is not None:
+                    return self.tokens[at:at + most]
+        return []
+
+
+#: the numbers that decide about drafts are a stream of their own beside the draws', keyed by the draft's place
+_VERIFY_STREAM = 0x5DEECE66D
+
+
+def _drafted_batch(engine, sampler, live, logits, prompts, results, stats, on_token) -> None:
+    """The decode loop of a batch in which some requests draft tokens.  `logits` has one row per entry of `live`: those
+    after the prompts.  drafts[i] are the tokens whose logits, and the place after them, the rows of entry i are."""
+    def finish(l, reason):
+        results[l.index] = Result(l.tokens, reason, len(prompts[l.index]))
+        engine.close([l.slot])
+        l.slot = -1
+
+    texts = {l.index: LookupDrafts(prompts[l.index]) for l in live}
+    drafts: List[List[int]] = [[] for _ in live]
+    last = time.perf_counter()
+    while live:
+        keep = []
+        for row, l in enumerate(live):                 # (drafts are empty where a request may not go on at all)
+            if len(l.tokens) >= l.config.max_tokens:
+                finish(l, "length")
+            elif l.pos >= engine.max_ctx - 1:
+                finish(l, "context")
+            else:
+                keep.append(row)
+        if len(keep) != len(live):
+            logits = _take(engine, logits, keep) if keep else None
+            live, drafts = [live[r] for r in keep], [drafts[r] for r in keep]
+        if not live:
+            return
+        uniforms = [[uniform(l.seed ^ _VERIFY_STREAM, l.index, len(l.tokens) + j) for j in range(len(x))]
+                    + [uniform(l.seed, l.index, len(l.tokens))] for l, x in zip(live, drafts)]
+        kept, tokens = sampler.verify(logits, drafts, [l.config.sampler for l in live], uniforms)
+        now = time.perf_counter()
+        stats.step_ms.append((now - last) * 1000.0)
+        last = now
+        still = []
+        for l, x, k, tok in zip(live, drafts, kept, tokens):
+            stats.drafted_tokens += len(x)
+            stats.kept_drafts += k
+            if k < len(x):
+                engine.rewind(l.slot, l.pos + k)       # the refused drafts were given to the sequence: not any more
+            new = list(x[:k]) + [int(tok)]
+            texts[l.index].extend(new)
+            for t in new:
+                if t in l.stop:
+                    finish(l, "stop")
+                    break
+                l.tokens.append(t)
+                l.pos += 1
+                stats.output_tokens += 1
+                if on_token is not None:
+                    on_token(l.index, t)
+                if len(l.tokens) >= l.config.max_tokens:
+                    finish(l, "length")
+                    break
+                if l.pos >= engine.max_ctx - 1:
+                    finish(l, "context")
+                    break
+            else:
+                still.append(l)
+        live = still
+        if not live:
+            return
+        # a step may emit a token more than it drafts: no more drafts than what may still be emitted allows
+        drafts = [texts[l.index].propose(min(l.config.lookup_drafts, l.config.max_tokens - len(l.tokens) - 1, engine.max_ctx - 2 - l.pos))
+                  for l in live]
+        logits = engine.step([Entry(l.slot, [l.tokens[-1]] + x, list(range(len(x) + 1)), undecided=len(x)) for l, x in zip(live, drafts)])
+        stats.steps += 1
+
+
 def generate(engine, sampler, prompts: Sequence[Sequence[int]], configs: Sequence[GenerateConfig],
              default_stop: Sequence[int] = (), on_token: Optional[Callable[[int, int], None]] = None,
              max_batch: int = 64, sync: Optional[Callable[[], None]] = None):
@@ -171,6 +274,11 @@ def generate(engine, sampler, prompts: Sequence[Sequence[int]], configs: Sequenc
             raise GenerationError(f"request {i}: empty prompt")
         if len(p) >= engine.max_ctx:
             raise GenerationError(f"request {i}: prompt too long: {len(p)} tokens (max {engine.max_ctx})")
+    for i, c in enumerate(configs):
+        if c.lookup_drafts > 0 and not c.sampler.temperature_alone:
+            raise GenerationError(f"request {i}: drafts are verified greedily or at a temperature alone (no top-k, top-p, min-p or repetition penalty)")
+        if c.lookup_drafts > 0 and not getattr(engine, "can_rewind", True):
+            raise GenerationError(f"request {i}: this model keeps state besides keys and values, so refused drafts cannot be taken back")
     results: List[Optional[Result]] = [None] * len(prompts)
     stats = Stats()
     sync = sync or (lambda: None)
@@ -200,7 +308,11 @@ def generate(engine, sampler, prompts: Sequence[Sequence[int]], configs: Sequenc
             stats.prompt_tokens += sum(len(prompts[l.index]) for l in live)
             stats.steps += 1
             sampler.start([l.slot for l in live])
-            _decode_batch(engine, sampler, live, logits, prompts, results, stats, on_token)
+            # a batch takes the drafting loop as a whole (its other requests draft nothing there), or, where one of its
+            # requests wants a distribution that cannot be verified, nobody in it drafts
+            drafting = any(l.config.lookup_drafts > 0 for l in live) and all(l.config.sampler.temperature_alone for l in live)
+            loop = _drafted_batch if drafting else _decode_batch
+            loop(engine, sampler, live, logits, prompts, results, stats, on_token)
             sync()
             stats.generate_ms += (time.perf_counter() - t1) * 1000.0
         except BaseException:

@@ -18,6 +18,10 @@ the projections (`bias`; `out_bias` for the output projection's), and an RMSNorm
 of every q and k head over the head's own elements (`qk_norm_eps`).  A layer
 without them launches nothing for them; a layer with them takes the separate
 rotation kernel, since the fused ones read the product's result as it is.
+
+Over a cache of 8-bit keys and values (KVView.q8) the rotation kernel stores them
+so, and attention reads them: one pair of kernels for every step, whatever the
+number of rows a sequence brings.
 """
 from __future__ import annotations
 
@@ -121,6 +125,10 @@ class Attention(Mixer):
         from ..kernels.build import variant
         return tuple(variant(m, dtype) for m in self.kernel_modules) + (variant("attention", dtype, (("HEAD_DIM", self.head_dim),)),)
 
+    def cache_kernel_variants(self, kv_dtype):
+        """Kernel files of their own that a cache of this kind needs (None: the run dtype)."""
+        return (("kv_q8", ()), ("attention_q8", (("HEAD_DIM", self.head_dim),))) if kv_dtype == "e4m3" else ()
+
     def cache_needs(self) -> List[CacheNeed]:
         return [CacheNeed(kind="kv", kv_heads=self.n_kv_heads, head_dim=self.head_dim, window=self.window)]
 
@@ -161,7 +169,7 @@ class Attention(Mixer):
         kv = ctx.cache.kv_view(unit)
         rot = self.position.rotation()
         # a step of single tokens: the attention kernel rotates and stores by itself; else a kernel of its own does
-        fused = not self._between and ops.attention_fuses_rotation(ctx.dtype, self.head_dim, self.n_heads // self.n_kv_heads,
+        fused = not kv.q8 and not self._between and ops.attention_fuses_rotation(ctx.dtype, self.head_dim, self.n_heads // self.n_kv_heads,
                                                                    ctx.max_q_len, rot.width if rot else 0, ctx.n_seq, self.n_kv_heads)
         unsummed = None
         if isinstance(xn, ops.UnscaledNorm):   # the norm's factor is applied to the product's sums
@@ -170,7 +178,7 @@ class Attention(Mixer):
             ops.gemm_rmsnorm(self.w_qkv[:cols], xn, norm.weight, norm.eps, qkv[:, :cols])
         else:
             # a product that shares k out over blocks leaves its runs to the rotation kernel, which adds them up as it reads
-            if not fused and not self._between and ops.rope_takes_unsummed(ctx.dtype, self.head_dim, rot.width if rot else 0):
+            if not fused and not kv.q8 and not self._between and ops.rope_takes_unsummed(ctx.dtype, self.head_dim, rot.width if rot else 0):
                 unsummed = ops.gemm_runs(self.w_qkv[:cols], xn, split)
             if unsummed is None:
                 ops.gemm(self.w_qkv[:cols], xn, qkv[:, :cols], scratch=split)
@@ -180,15 +188,22 @@ class Attention(Mixer):
             ops.head_rmsnorm(qkv, 0, self.n_heads, self.head_dim, self.q_norm, self.qk_norm_eps)
             if n_kv:
                 ops.head_rmsnorm(qkv, self.q_dim, n_kv, self.head_dim, self.k_norm, self.qk_norm_eps)
-        if not fused:
+        if kv.q8:
+            pages = self._seq_pages(ctx, kv)
+            table, slots = (kv.page_table, ctx.slots) if pages is None else (pages, ctx.tok_seq)      # row i is sequence i's
+            q = qkv[:, :self.q_dim]
+            ops.rope_kv_q8(qkv, q, self.n_heads, self.n_kv_heads, self.head_dim, rot.width if rot else 0, rot.interleaved if rot else False,
+                           rot.cos if rot else None, rot.sin if rot else None, ctx.positions, ctx.tok_seq, slots, table, kv.cache,
+                           kv.page_stride, write_kv=owns_cache)
+        elif not fused:
             ops.rope_kv(qkv, self.n_heads, n_kv, self.head_dim, rot.width if rot else 0, rot.interleaved if rot else False,
                         rot.cos if rot else None, rot.sin if rot else None, ctx.positions,
                         ctx.tok_seq, ctx.slots, kv.page_table, kv.cache, kv.page_stride, kv.v_off, write_kv=owns_cache,
                         unsummed=unsummed, single_tokens=ctx.max_q_len == 1,
                         seq_pages=getattr(ctx, "seq_pages", {}).get(kv.group) if ctx.max_q_len == 1 else None)
         out = ctx.buffer("attention.out", (t, self.q_dim), ctx.dtype)
-        self.attend(qkv, out, ctx, kv, rotation=(rot.cos, rot.sin, rot.width, rot.interleaved) if fused and rot else None,
-                    new_kv=fused and owns_cache)
+        self.attend(qkv[:, :self.q_dim] if kv.q8 else qkv, out, ctx, kv,
+                    rotation=(rot.cos, rot.sin, rot.width, rot.interleaved) if fused and rot else None, new_kv=fused and owns_cache)
         if self.out_bias:        # the bias goes into the residual after the product: no norm of it can be left on the way
             ops.gemm(self.w_o, out, residual, ops.EPI_ACCUM_F32, scratch=split)
             ops.bias_add(residual, self.b_o)
@@ -210,9 +225,22 @@ class Attention(Mixer):
         ops.gemm(self.w_o, out, residual, ops.EPI_ACCUM_F32, scratch=split)
         return False
 
+    @staticmethod
+    def _seq_pages(ctx, kv):
+        """Steps of single tokens: the sequences' page-table rows in the order of the step, if the engine keeps them."""
+        return getattr(ctx, "seq_pages", {}).get(kv.group) if ctx.max_q_len == 1 else None
+
     def attend(self, q, out, ctx, kv, rotation=None, new_kv=False) -> None:
         """Attention of the step's (rotated) query rows over the cache; the kernel is chosen by the
         step's shape and the run dtype, the arithmetic is the same."""
+        if kv.q8:
+            pages = self._seq_pages(ctx, kv)
+            table, slots = (kv.page_table, ctx.slots) if pages is None else (pages, None)
+            bound = ctx.max_kv_len if ctx.max_pages_used is None else ctx.max_pages_used * ops.PAGE
+            ops.attention_q8(q, out, self.n_heads, self.n_kv_heads, self.head_dim, ctx.cu_q, ctx.start_pos, slots, table, kv.cache,
+                             kv.page_stride, ctx.max_q_len, bound, window=self.window or 0, scale=self.scale,
+                             scratch=lambda n: ctx.scratch("attention.partials", n, torch.float32))
+            return
         ops.attention(q, out, self.n_heads, self.n_kv_heads, self.head_dim, ctx.positions, ctx.tok_seq, ctx.slots,
                       kv.page_table, kv.cache, kv.page_stride, kv.v_off, ctx.host["q_lens"], ctx.host["start_pos"],
                       window=self.window or 0, scale=self.scale, cu_q=ctx.cu_q, start_pos_dev=ctx.start_pos,

@@ -67,6 +67,11 @@ class Part:
         from ..kernels.build import variant
         return tuple(variant(m, dtype) for m in self.kernel_modules)
 
+    def cache_kernel_variants(self, kv_dtype: Optional[str]):
+        """(module, defines) pairs that this part launches only over a cache of this kind (None: keys and values in the
+        run dtype)."""
+        return ()
+
 
 def stored(t: torch.Tensor, spec: TensorSpec, device: torch.device, dtype: torch.dtype) -> torch.Tensor:
     """The storage rule: matrices in the run dtype, vectors in float32, tables in int32."""

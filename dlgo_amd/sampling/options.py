@@ -21,6 +21,11 @@ class SamplerConfig:
     def greedy(self) -> bool:
         return self.temperature <= 0
 
+    @property
+    def temperature_alone(self) -> bool:
+        """Nothing cuts or changes the distribution but the temperature (or the choice is greedy)."""
+        return self.greedy or (self.top_k <= 0 and self.top_p >= 1.0 and self.min_p <= 0.0 and self.repetition_penalty <= 1.0)
+
 
 @dataclass
 class GenerateConfig:
@@ -29,6 +34,7 @@ class GenerateConfig:
     seed: int = -1                               # < 0: seeded from the clock
     stop_tokens: Optional[Tuple[int, ...]] = None   # None: the model's own (eos ids of its configuration)
     ignore_eos: bool = False                     # benchmarks: never stop on a token
+    lookup_drafts: int = 0                       # tokens drafted a step from the request's own text (0 = none)
 
 
 Option = Callable[[GenerateConfig], None]
@@ -96,6 +102,16 @@ def with_ignore_eos(on: bool = True) -> Option:
     return opt
 
 
+def with_lookup_drafts(n: int) -> Option:
+    """Draft up to n tokens a step by looking up where the text's last tokens stood before, and have one step of the model
+    verify them all: fewer steps where the text repeats itself, the same distribution of tokens.  Takes greedy decoding
+    or a temperature alone (no top-k, top-p, min-p or repetition penalty); a batch that holds a request with one of those
+    drafts nothing."""
+    def opt(c: GenerateConfig) -> None:
+        c.lookup_drafts = int(n)
+    return opt
+
+
 def apply_options(opts: Sequence[Option], base: Optional[GenerateConfig] = None) -> GenerateConfig:
     """Options over the defaults (dlgo.go:242-248)."""
     cfg = copy.deepcopy(base) if base is not None else GenerateConfig()
@@ -105,4 +121,6 @@ def apply_options(opts: Sequence[Option], base: Optional[GenerateConfig] = None)
         raise ValueError("max_tokens must be >= 0")
     if cfg.sampler.temperature < 0:
         raise ValueError("temperature must be >= 0")
+    if cfg.lookup_drafts < 0:
+        raise ValueError("lookup_drafts must be >= 0")
     return cfg

@@ -31,6 +31,8 @@ class Sampler:
         self._staging: List[tuple] = []                 # (pinned int32 buffer, event of the copy that last read it)
         self._staging_next = 0
         self._options: Optional[torch.Tensor] = None    # the device's copy: 7 rows of int32/float32 bits
+        self._verify_dev: Optional[torch.Tensor] = None    # verify()'s arrays and scratch on the device
+        self._verify_work: Optional[torch.Tensor] = None
         self._rings: Optional[torch.Tensor] = None      # [keys, RECENT] last tokens chosen per key
         self._counts: Optional[torch.Tensor] = None     # [keys] tokens chosen so far per key
 
@@ -152,3 +154,58 @@ class Sampler:
             rec = torch.from_numpy(r).to(self.device)
         ops.sample(logits, self._work, fd[0], kd[0], fd[1], fd[2], fd[3], rec, fd[4], out, dealt_rows=dealt_rows)
         return out
+
+    def verify(self, logits: torch.Tensor, drafts: Sequence[Sequence[int]], configs: Sequence[SamplerConfig],
+               uniforms: Sequence[Sequence[float]], draft_logits: Optional[torch.Tensor] = None):
+        """Sequence i drafted the tokens drafts[i] (perhaps none) and logits holds, for sequence after sequence, the target
+        model's rows for the place of each draft and the place after them ([sum(len + 1), vocab] float32 on the device).
+        Returns (kept, tokens) as host lists: how many of each sequence's drafts are kept, and the token that follows
+        them; both are then distributed as if the target had chosen every token itself.  uniforms[i]: a number in [0, 1)
+        for each draft and one for the token after.  draft_logits [sum(len), vocab]: what a draft model drew the drafts
+        from, at the same temperature; None where they are certain (looked up).  Greedy rows keep what is the maximum."""
+        n, d = len(drafts), sum(len(x) for x in drafts)
+        if len(configs) != n or len(uniforms) != n or any(len(u) != len(x) + 1 for u, x in zip(uniforms, drafts)):
+            raise ValueError("sampler: one configuration per sequence, and a uniform number for each draft and one more")
+        if logits.shape[0] != n + d:
+            raise ValueError(f"sampler: {n} sequences with {d} drafts need {n + d} rows of logits, not {logits.shape[0]}")
+        for c in configs:
+            if not c.temperature_alone:
+                raise ValueError("sampler: drafts are verified greedily or at a temperature alone (no top-k, top-p, min-p or repetition penalty)")
+        if n == 0:
+            return [], []
+        lens = np.array([len(x) for x in drafts], dtype=np.int64)
+        # one copy up (drafts, their offsets, temperatures, uniform numbers), one down (kept counts and tokens)
+        parts = (np.fromiter((t for x in drafts for t in x), dtype=np.int32, count=d),
+                 np.concatenate([[0], np.cumsum(lens)]).astype(np.int32),
+                 np.array([max(0.0, c.temperature) for c in configs], dtype=np.float32).view(np.int32),
+                 np.fromiter((v for u in uniforms for v in u), dtype=np.float32, count=n + d).view(np.int32))
+        offs, total = [], 0
+        for a in parts:
+            offs.append(total)
+            total += (len(a) + 3) // 4 * 4
+        if self._verify_dev is None or self._verify_dev.numel() < total + 2 * n:
+            self._verify_dev = torch.empty(2 * (total + 2 * n), dtype=torch.int32, device=self.device)
+        i = self._pin_next
+        self._pin_next = (i + 1) % len(self._pinned)
+        if self._pinned[i].shape[0] < max(total, 2 * n):
+            self._pinned[i] = torch.empty(2 * max(total, 2 * n), dtype=torch.int32, pin_memory=True)
+        host = self._pinned[i]
+        for a, o in zip(parts, offs):
+            host.numpy()[o:o + len(a)] = a
+        dev = self._verify_dev
+        dev[:total].copy_(host[:total], non_blocking=True)
+        at = [dev[o:o + len(a)] for a, o in zip(parts, offs)]
+        out = dev[total:total + 2 * n]
+
+        def scratch(size):
+            if self._verify_work is None or self._verify_work.numel() < size:
+                self._verify_work = torch.empty(size, dtype=torch.uint8, device=self.device)
+            return self._verify_work
+        ops.verify_drafts(logits, at[0], at[1], at[2].view(torch.float32), at[3].view(torch.float32), out[:n], out[n:], int(lens.max()),
+                          draft_logits=draft_logits, scratch=scratch)
+        host[:2 * n].copy_(out, non_blocking=True)         # behind the copy up, in the same stream
+        event = torch.cuda.Event()
+        event.record()
+        event.synchronize()
+        got = host[:2 * n].tolist()
+        return got[:n], got[n:]

@@ -1,0 +1,241 @@
+"""The 8-bit cache and drafted tokens through the library's entry points, on the GPU.
+
+Tolerances of the 8-bit runs.  The plain implementation rounds keys and values as the cache does, so what is left is the
+run's own bfloat16 (3e-2 of the largest logit, as over a bfloat16 cache) and the elements that it puts on the other side of
+a border of the 8-bit grid.  Through a few layers of bfloat16 an element is off by about d = 1e-2 (what plain.forward gives
+when every product's result, norm and gate is rounded to bfloat16: 0.6e-2 to 1.6e-2 of the largest logit for these models).
+The grid's steps are s = 2^-3 to 2^-4 of an element; d / s of the elements move, by s each: sqrt(d / s) * s = sqrt(d s) =
+sqrt(1e-2 * 2^-3.5) = 3e-2 in the root mean square, in every layer's values, and a row that sees one token has nothing to
+average over.  So 3e-2 for each layer more.  (2^-8, the rounding of the stored element alone, in place of d gave 3e-2 for
+all layers together; the plain implementation itself, rounded to bfloat16 as above, is off by up to 7.9e-2 for model C.)"""
+import json
+import subprocess
+import sys
+
+import numpy as np
+import pytest
+import torch
+
+import plain_llama as plain
+from conftest import ROOT, TINY_A, TINY_B, TINY_C, TINY_D, make_folder
+from test_verify_gpu import plain as plain_verify
+
+pytestmark = pytest.mark.gpu
+
+CONFIGS = {"A": (TINY_A, dict(std=0.1)), "B": (TINY_B, dict(norm_jitter=0.1, std=0.08)), "C": (TINY_C, dict(norm_jitter=0.1, std=0.12)),
+           "D": (TINY_D, dict(norm_jitter=0.2, std=0.08))}
+TOL = {name: 3e-2 + 3e-2 * raw["num_hidden_layers"] for name, (raw, _) in CONFIGS.items()}
+
+
+@pytest.fixture(scope="module")
+def folders(tmp_path_factory):
+    out = {}
+    for name, (raw, kw) in CONFIGS.items():
+        for dtype in ("bfloat16", "float32"):
+            out[name, dtype] = str(tmp_path_factory.mktemp(f"drafts{name}"))
+            make_folder(raw, 31 + len(out), out[name, dtype], dtype=dtype, **kw)
+    return out
+
+
+def rounded(x, heads, hd):
+    """Rows of a cache of 8 bits: e4m3 times the least power of two that holds a head's largest element."""
+    x = torch.as_tensor(x).view(-1, heads, hd)
+    m = x.abs().amax(-1, keepdim=True)
+    e = torch.ceil(torch.log2(m.clamp(min=2.0 ** -200) / 448)).clamp(min=-126)
+    e = torch.where(m > 448 * torch.exp2(e), e + 1, e)
+    return ((x / torch.exp2(e)).float().to(torch.float8_e4m3fn).double() * torch.exp2(e)).view(len(x), heads * hd).numpy()
+
+
+@pytest.fixture
+def plain_q8(monkeypatch):
+    """plain.forward over rounded keys and values."""
+    exact = plain.attention
+
+    def attention(q, k, v, H, KV, hd, window=None):
+        return exact(q, rounded(k, KV, hd), rounded(v, KV, hd), H, KV, hd, window)
+    monkeypatch.setattr(plain, "attention", attention)
+    return plain
+
+
+def rel_err(got, want):
+    return np.abs(got.double().cpu().numpy() - want).max() / np.abs(want).max()
+
+
+def texts_of(raw, lens, seed):
+    rng = np.random.default_rng(seed)
+    return [rng.integers(0, raw["vocab_size"], size=n).tolist() for n in lens]
+
+
+@pytest.mark.parametrize("graphs", [False, True])
+@pytest.mark.parametrize("name", ["A", "B", "C", "D"])
+def test_an_8_bit_cache_under_every_kind_of_step(folders, plain_q8, name, graphs):
+    """Prompts whole and in pieces, single tokens (recorded from the second on), a few tokens at once, a copied sequence,
+    unequal batches in slots that were used before."""
+    from dlgo_amd.engine import Engine, Entry
+    raw = CONFIGS[name][0]
+    eng = Engine.from_folder(folders[name, "bfloat16"], "bfloat16", max_tokens=2048, max_step_tokens=96, use_graphs=graphs, cache_dtype="e4m3")
+    assert eng.cache.groups[0].storage.dtype == torch.uint8
+    cfg, w = plain.read_model(folders[name, "bfloat16"])
+    for turn in range(2):
+        texts = texts_of(raw, [120, 9, 70], seed=turn)
+        want = [plain_q8.forward(cfg, w, t) for t in texts]
+        slots = eng.open(3)
+        first = [len(t) - 6 for t in texts]
+        out = eng.step([Entry(s, t[:n], range(n)) for s, t, n in zip(slots, texts, first)])
+        for o, x, n in zip(torch.split(out, first), want, first):
+            assert rel_err(o, x[:n]) <= TOL[name]
+        for j in range(3):
+            out = eng.decode(slots, [t[n + j] for t, n in zip(texts, first)])
+            for i, n in enumerate(first):
+                assert rel_err(out[i], want[i][n + j]) <= TOL[name], (turn, i, j)
+        twin = eng.fork(slots[0])
+        out = eng.step([Entry(s, t[n + 3:], (0, 1, 2)) for s, t, n in zip(slots, texts, first)])
+        alone = eng.step([Entry(twin, texts[0][first[0] + 3:], (0, 1, 2))])
+        for i, n in enumerate(first):
+            assert rel_err(out[3 * i:3 * i + 3], want[i][n + 3:]) <= TOL[name]
+        assert rel_err(alone, want[0][first[0] + 3:]) <= TOL[name]
+        eng.close(slots + [twin])
+    eng.cache.check_consistent()
+
+
+@pytest.mark.parametrize("cache_dtype", [None, "e4m3"])
+@pytest.mark.parametrize("window", [None, 70])
+def test_a_rewound_sequence_goes_on_as_if_nothing_had_been_there(folders, monkeypatch, window, cache_dtype):
+    """Wrong drafts behind a sequence, taken back, then the right tokens: the same bits as without the drafts, around the
+    ends of pages and with layers that see a window only."""
+    from dlgo_amd.engine import Engine, EngineError, Entry
+    from dlgo_amd.parts.attention import Attention
+    if window:
+        init = Attention.__init__
+        monkeypatch.setattr(Attention, "__init__", lambda self, *a, **kw: init(self, *a, **{**kw, "window": window}))
+    eng = Engine.from_folder(folders["B", "bfloat16"], "bfloat16", max_tokens=1024, max_ctx=256, max_step_tokens=64, cache_dtype=cache_dtype)
+    assert eng.can_rewind and (eng.cache.has_windows == bool(window))
+    (text,) = texts_of(TINY_B, [200], seed=5)
+    a, b = eng.open(2)
+    pos = 0
+    for n in (50, 9, 3, 1, 4, 60, 5, 12, 2, 33, 8):
+        piece = text[pos:pos + n]
+        wrong = [(t + 1) % TINY_B["vocab_size"] for t in text[pos:pos + min(9, 64 - n)]]
+        if pos:
+            eng.step([Entry(a, [text[pos]] + wrong, range(len(wrong) + 1), undecided=len(wrong) + 1)])
+            eng.rewind(a, pos)
+        x = eng.step([Entry(a, piece, range(n))])
+        y = eng.step([Entry(b, piece, range(n))])
+        assert torch.equal(x, y) and torch.isfinite(x).all()
+        pos += n
+        eng.cache.check_consistent()
+    with pytest.raises(EngineError, match="rewind"):
+        eng.rewind(a, pos + 1)
+    with pytest.raises(EngineError, match="undecided"):
+        eng.step([Entry(a, [1, 2], (1,), undecided=3)])
+    eng.close([a])
+    with pytest.raises(EngineError, match="not in use"):
+        eng.rewind(a, 0)
+
+
+def repeating(raw, seed, n=30, period=7):
+    return (texts_of(raw, [period], seed)[0] * n)[:n]
+
+
+def test_greedy_with_drafts_is_greedy(folders):
+    """In float32 the tokens are the plain implementation's, drafts or none; where the text repeats, in fewer steps."""
+    import dlgo_amd
+    folder = folders["A", "float32"]
+    cfg, w = plain.read_model(folder)
+    llm = dlgo_amd.load_llm(folder, dtype="float32", max_tokens=1024, max_batch=3)
+    prompts = [repeating(TINY_A, 3), texts_of(TINY_A, [1], 4)[0], repeating(TINY_A, 5, 20, 3), repeating(TINY_A, 6, 9, 4), [7, 7, 7]]
+    want = [plain.greedy_generate(cfg, w, p, 40) for p in prompts]
+    for n in (1, 4, 15):
+        got = llm.generate(prompts, dlgo_amd.with_greedy(), dlgo_amd.with_max_tokens(40), dlgo_amd.with_ignore_eos(), dlgo_amd.with_lookup_drafts(n))
+        assert [r.tokens for r in got] == want and all(r.finish_reason == "length" for r in got)
+    # up to the context's end, and a stop token among what would be emitted
+    long = llm.generate(prompts[0], dlgo_amd.with_greedy(), dlgo_amd.with_max_tokens(500), dlgo_amd.with_ignore_eos(), dlgo_amd.with_lookup_drafts(6))
+    assert long.finish_reason == "context" and len(prompts[0]) + len(long.tokens) == TINY_A["max_position_embeddings"] - 1
+    assert long.tokens == plain.greedy_generate(cfg, w, prompts[0], len(long.tokens))
+    stop = want[0][9]
+    r = llm.generate(prompts[0], dlgo_amd.with_greedy(), dlgo_amd.with_max_tokens(40), dlgo_amd.with_stop_tokens([stop]), dlgo_amd.with_lookup_drafts(6))
+    assert r.tokens == plain.greedy_generate(cfg, w, prompts[0], 40, stop_tokens=(stop,)) and r.finish_reason == "stop"
+    llm.engine.cache.check_consistent()
+    assert llm.engine.free_slots() == llm.engine.cache.max_slots
+
+
+def test_sampling_with_drafts_is_what_the_formulas_say(folders):
+    """The whole loop again with the plain model and the plain verification, number by number; and the same twice."""
+    import dlgo_amd
+    from dlgo_amd.engine.generate import _VERIFY_STREAM, LookupDrafts
+    from dlgo_amd.sampling import uniform
+    folder = folders["B", "float32"]
+    cfg, w = plain.read_model(folder)
+    llm = dlgo_amd.load_llm(folder, dtype="float32", max_tokens=1024)
+    prompts = [repeating(TINY_B, 8, 25, 5), texts_of(TINY_B, [3], 9)[0], repeating(TINY_B, 10, 40, 4)]
+    opts = [dlgo_amd.with_temperature(0.25), dlgo_amd.with_top_k(0), dlgo_amd.with_top_p(1.0), dlgo_amd.with_repetition_penalty(1.0),
+            dlgo_amd.with_seed(77), dlgo_amd.with_max_tokens(20), dlgo_amd.with_ignore_eos(), dlgo_amd.with_lookup_drafts(3)]
+    got = llm.generate(prompts, *opts)
+    assert [r.tokens for r in llm.generate(prompts, *opts)] == [r.tokens for r in got]
+    t = float(np.float32(0.25))
+    decided = 0
+    for i, (p, r) in enumerate(zip(prompts, got)):
+        out, drafts = [], []
+        text = LookupDrafts(p)
+        while len(out) < 20:
+            u = [uniform(77 ^ _VERIFY_STREAM, i, len(out) + j) for j in range(len(drafts))] + [uniform(77, i, len(out))]
+            rows = range(len(p) + len(out) - 1, len(p) + len(out) + len(drafts))
+            logits = torch.as_tensor(plain.forward(cfg, w, p + out + drafts, rows=rows))
+            (kept,), (token,), _ = plain_verify(logits, drafts, [len(drafts)], [t], u, None)
+            decided += len(drafts)
+            new = drafts[:kept] + [token]
+            out += new
+            text.extend(new)
+            drafts = text.propose(min(3, 20 - len(out) - 1))
+        assert r.tokens == out, i
+    assert decided >= 6, "too few drafts: the check says little"
+
+
+def test_drafts_over_an_8_bit_cache_keep_to_the_margins(folders, plain_q8):
+    """The three operators together as a server runs them: prompts stored and attended in 8 bits, tokens drafted, verified and
+    taken back.  Every emitted token is the plain maximum, or within the tolerance of it."""
+    import dlgo_amd
+    folder = folders["A", "bfloat16"]
+    cfg, w = plain.read_model(folder)
+    llm = dlgo_amd.load_llm(folder, dtype="bfloat16", max_tokens=2048, cache_dtype="e4m3")
+    assert "e4m3" in llm.model_info()
+    prompts = [repeating(TINY_A, 13), texts_of(TINY_A, [2], 14)[0], repeating(TINY_A, 15, 61, 3), repeating(TINY_A, 16, 66, 5)]
+    results = llm.generate(prompts, dlgo_amd.with_greedy(), dlgo_amd.with_max_tokens(30), dlgo_amd.with_ignore_eos(), dlgo_amd.with_lookup_drafts(5))
+    for p, r in zip(prompts, results):
+        assert len(r.tokens) == 30
+        x = plain_q8.forward(cfg, w, p + r.tokens)[len(p) - 1:-1]
+        off = x.max(-1) - x[np.arange(30), r.tokens]
+        assert (off <= 2 * TOL["A"] * np.abs(x).max()).all()
+    llm.engine.cache.check_consistent()
+
+
+def test_what_does_not_go_together_is_refused(folders):
+    import dlgo_amd
+    from dlgo_amd.engine import Engine, EngineError
+    from dlgo_amd.sampling import SamplerConfig
+    from dlgo_amd.sampling.sampler import Sampler
+    with pytest.raises(EngineError, match="bfloat16 run"):
+        Engine.from_folder(folders["A", "float32"], "float32", max_tokens=128, cache_dtype="e4m3")
+    with pytest.raises(EngineError, match="e5m2"):
+        Engine.from_folder(folders["A", "bfloat16"], "bfloat16", max_tokens=128, cache_dtype="e5m2")
+    llm = dlgo_amd.load_llm(folders["A", "bfloat16"], dtype="bfloat16", max_tokens=128)
+    with pytest.raises(ValueError, match="drafts are verified"):
+        llm.generate([1, 2], dlgo_amd.with_lookup_drafts(2))               # the default options cut the distribution
+    s = Sampler(256, "cuda:0")
+    greedy, logits = SamplerConfig(temperature=0), torch.randn(3, 256, device="cuda:0")
+    assert s.verify(logits, [[logits[0].argmax().item()], []], [greedy] * 2, [[0.5, 0.5], [0.5]]) == ([1, 0], logits.argmax(-1)[1:].tolist())
+    assert s.verify(logits[:0], [], [], []) == ([], [])
+    for args in [([[1], []], [greedy], [[0.5, 0.5], [0.5]]), ([[1], []], [greedy] * 2, [[0.5], [0.5]]), ([[1]], [greedy], [[0.5, 0.5]]),
+                 ([[1], []], [greedy, SamplerConfig()], [[0.5, 0.5], [0.5]])]:
+        with pytest.raises(ValueError, match="sampler"):
+            s.verify(logits, *args)
+
+
+def test_the_command_line_takes_both(folders):
+    cmd = [sys.executable, "-m", "dlgo_amd", folders["A", "bfloat16"], "--greedy", "--max-tokens", "8", "--ignore-eos",
+           "--prompt-ids", "5,6,7,5,6,7,5,6", "--ctx", "128", "--cache-dtype", "e4m3", "--lookup-drafts", "3"]
+    p = subprocess.run(cmd, cwd=ROOT, capture_output=True, text=True, timeout=100)
+    assert p.returncode == 0, p.stderr
+    lines = p.stdout.splitlines()
+    assert "e4m3" in lines[0]
+    assert len(json.loads(next(x for x in lines if x.startswith("{")))["tokens"]) == 8
