@@ -96,7 +96,8 @@ class Engine:
                  use_graphs: bool = True, graph_max_batch: int = 128, prompt_graph_max_tokens: int = 4096,
                  prompt_graph_limit: int = 32, prompt_graph_bytes: int = 1 << 30, cache_dtype: Optional[str] = None):
         """`model` holds its weights already (see from_folder / from_random).  use_graphs: steps of single tokens are
-        recorded per batch size, and steps of fresh prompts of up to prompt_graph_max_tokens rows per shape (the
+        recorded per batch size, and per shape steps of fresh prompts of up to prompt_graph_max_tokens rows and steps of
+        drafts (as many for each sequence, every row wanted) of up to graph_max_batch rows (the
         prompt_graph_limit most recently used shapes are kept, as long as the logits they keep stay within
         prompt_graph_bytes), the second time a size or shape is seen.  cache_dtype: None keeps keys and values in the run
         dtype, "e4m3" in 8 bits (bfloat16 runs only: half the cache's bytes, each element rounded to 4 significant bits)."""
@@ -362,13 +363,16 @@ class Engine:
         seq_of = np.repeat(np.arange(len(entries)), q_lens)
         pos_all = np.concatenate([np.arange(s, s + n) for s, n in zip(starts, q_lens)])
 
-        # Fresh prompts of a shape seen before: the launches depend on the rows per sequence and the wanted places only,
-        # so the step is recorded the second time the shape comes and replayed from then on.
+        # Fresh prompts of a shape seen before, and as many drafts behind each sequence (a step that wants every row):
+        # the launches depend on the rows per sequence and the wanted places only (and on a bound of the lengths: the
+        # context's, for drafts), so the step is recorded the second time the shape comes and replayed from then on.
         shape = None
+        fresh = not any(starts)
         # (a recording keeps its logits: not where those would be more than 64 MB)
         if (self.use_graphs and sink is None and n_out and total <= min(self.max_step_tokens, self.prompt_graph_max_tokens)
-                and n_out * self.vocab * 4 <= min(64 << 20, self.prompt_graph_bytes) and not any(starts)):
-            shape = (tuple(q_lens), tuple(wanted))
+                and n_out * self.vocab * 4 <= min(64 << 20, self.prompt_graph_bytes)
+                and (fresh or (n_out == total <= self.graph_max_batch and len(set(q_lens)) == 1))):
+            shape = (tuple(q_lens), tuple(wanted), fresh)
         out = None
         if sink is None and (shape is None or shape not in self._prompt_graphs):
             out = torch.empty((n_out, self.vocab), dtype=torch.float32, device=self.device)
@@ -426,7 +430,7 @@ class Engine:
 
     def _prompt_step(self, shape, fields: Dict[str, np.ndarray], host: Dict[str, np.ndarray], n_seq: int, n_rows: int,
                      sel: np.ndarray, out: Optional[torch.Tensor]) -> torch.Tensor:
-        """A whole step of fresh prompts whose shape may be recorded: replayed if it is, recorded the second time it is
+        """A whole step of fresh prompts or of drafts whose shape may be recorded: replayed if it is, recorded the second time it is
         seen, run as it is the first time.  Returns the logits (the caller's own tensor)."""
         g = self._prompt_graphs.get(shape)
         if g is not None:
@@ -447,6 +451,8 @@ class Engine:
         logits = torch.empty((len(sel), self.vocab), dtype=torch.float32, device=self.device)
         arrays = self._upload(fields, dest=meta)
         ctx = StepContext(self, n_seq, n_rows, arrays, host)
+        if not shape[2]:
+            ctx.max_pages_used = self.cache.max_pages_per_seq         # the recorded launches must cover any later length
         graph = torch.cuda.CUDAGraph()
         torch.cuda.synchronize()
         gc.collect()

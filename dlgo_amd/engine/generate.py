@@ -196,6 +196,19 @@ class LookupDrafts:
 _VERIFY_STREAM = 0x5DEECE66D
 
 
+#: rows that a step may be filled up to.  Llama 3.2 1B, eight sequences with seven drafts each: 1.50 ms a recorded step of 64
+#: rows, 1.79 ms launch by launch with the rows that were drafted only; at twice the rows the products cost what that saves.
+FILL_ROWS = 64
+
+
+def fill_drafts(drafts: List[List[int]], room: Sequence[int], last: Sequence[int]) -> List[List[int]]:
+    """Where some sequence has drafts and the step stays small, every sequence that may draft brings as many as it has
+    room for, so that steps keep one shape, which the engine records: the last token again, refused unless it is right."""
+    if not any(drafts) or sum(room) + len(room) > FILL_ROWS:
+        return drafts
+    return [x + [t] * (r - len(x)) for x, r, t in zip(drafts, room, last)]
+
+
 def _drafted_batch(engine, sampler, live, logits, prompts, results, stats, on_token) -> None:
     """The decode loop of a batch in which some requests draft tokens.  `logits` has one row per entry of `live`: those
     after the prompts.  drafts[i] are the tokens whose logits, and the place after them, the rows of entry i are."""
@@ -256,8 +269,8 @@ def _drafted_batch(engine, sampler, live, logits, prompts, results, stats, on_to
         if not live:
             return
         # a step may emit a token more than it drafts: no more drafts than what may still be emitted allows
-        drafts = [texts[l.index].propose(min(l.config.lookup_drafts, l.config.max_tokens - len(l.tokens) - 1, engine.max_ctx - 2 - l.pos))
-                  for l in live]
+        room = [min(l.config.lookup_drafts, l.config.max_tokens - len(l.tokens) - 1, engine.max_ctx - 2 - l.pos) for l in live]
+        drafts = fill_drafts([texts[l.index].propose(r) for l, r in zip(live, room)], room, [l.tokens[-1] for l in live])
         logits = engine.step([Entry(l.slot, [l.tokens[-1]] + x, list(range(len(x) + 1)), undecided=len(x)) for l, x in zip(live, drafts)])
         stats.steps += 1
 

@@ -8,7 +8,7 @@ import torch
 
 from dlgo_amd.cache import PAGE, Cache, CacheError
 from dlgo_amd.cache.cache import kv_bytes_per_token
-from dlgo_amd.engine.generate import GenerationError, LookupDrafts, generate
+from dlgo_amd.engine.generate import FILL_ROWS, GenerationError, LookupDrafts, fill_drafts, generate
 from dlgo_amd.parts import CacheNeed
 from dlgo_amd.sampling import GenerateConfig, SamplerConfig, apply_options, with_lookup_drafts, with_temperature
 from test_cache_and_loop import FakeEngine, ScriptSampler
@@ -24,6 +24,15 @@ def test_lookup_of_the_last_three_then_two_tokens():
     assert t.propose(1) == [9]                       # three (9, 2, 3) nowhere; two: the latest (2, 3) was followed by 9
     assert LookupDrafts([]).propose(3) == [] and LookupDrafts([7]).propose(3) == [] and LookupDrafts([7, 7]).propose(3) == []
     assert LookupDrafts([7, 7, 7]).propose(3) == [7]           # (7, 7) was followed by 7; there is no more text
+
+
+def test_small_steps_are_filled_to_one_shape():
+    assert fill_drafts([[], []], [3, 3], [8, 9]) == [[], []]                                     # nobody drafts: single tokens
+    assert fill_drafts([[1], [], [4, 5, 6]], [3, 2, 3], [7, 8, 9]) == [[1, 7, 7], [8, 8], [4, 5, 6]]
+    assert fill_drafts([[1], []], [3, 0], [7, 8]) == [[1, 7, 7], []]                             # no room, or does not draft
+    n = FILL_ROWS // 8
+    assert all(len(x) == 7 for x in fill_drafts([[1]] + [[]] * (n - 1), [7] * n, [0] * n))
+    assert fill_drafts([[1]] + [[]] * n, [7] * (n + 1), [0] * (n + 1)) == [[1]] + [[]] * n       # too many rows
 
 
 # -- the loop ------------------------------------------------------------------------

@@ -133,6 +133,37 @@ def test_a_rewound_sequence_goes_on_as_if_nothing_had_been_there(folders, monkey
         eng.rewind(a, 0)
 
 
+@pytest.mark.parametrize("dtype,cache_dtype", [("bfloat16", "e4m3"), ("bfloat16", None), ("float32", None)])
+def test_steps_of_drafts_are_recorded(folders, dtype, cache_dtype):
+    """A shape's third step and those after it are replayed, at lengths that had not been reached when it was recorded, with
+    other sequences in other slots, and give the bits that the launches one by one give."""
+    from dlgo_amd.engine import Engine, Entry
+    folder = folders["B", dtype]
+    made = [Engine.from_folder(folder, dtype, max_tokens=1024, max_ctx=512, use_graphs=g, cache_dtype=cache_dtype) for g in (True, False)]
+    texts = texts_of(TINY_B, [400, 390], seed=8)
+    pos = [12, 3]
+    slots = [eng.open(3) for eng in made]
+    for eng, s in zip(made, slots):
+        eng.step([Entry(s[i], texts[i][:pos[i]], (pos[i] - 1,)) for i in (0, 1)])
+        eng.step([Entry(s[2], texts[1][:70], (69,))])
+    for turn in range(16):
+        take = (0, 1) if turn % 4 < 3 else (1, 0)
+        outs = [eng.step([Entry(s[i], texts[i][pos[i]:pos[i] + 5], range(5), undecided=4) for i in take]) for eng, s in zip(made, slots)]
+        assert torch.equal(*outs), turn
+        for eng, s in zip(made, slots):
+            for i in take:
+                eng.rewind(s[i], pos[i] + 2 + 3 * i)
+        pos = [pos[0] + 2, pos[1] + 5]
+        if turn == 9:                                        # far ahead: pages and lengths the recording never saw
+            for eng, s in zip(made, slots):
+                eng.step([Entry(s[i], texts[i][pos[i]:pos[i] + 250], (0,)) for i in (0, 1)])
+            pos = [p + 250 for p in pos]
+        torch.cuda.synchronize()
+    assert [len(eng._prompt_graphs) for eng in made] == [1, 0]
+    for eng in made:
+        eng.cache.check_consistent()
+
+
 def repeating(raw, seed, n=30, period=7):
     return (texts_of(raw, [period], seed)[0] * n)[:n]
 
@@ -162,7 +193,7 @@ def test_greedy_with_drafts_is_greedy(folders):
 def test_sampling_with_drafts_is_what_the_formulas_say(folders):
     """The whole loop again with the plain model and the plain verification, number by number; and the same twice."""
     import dlgo_amd
-    from dlgo_amd.engine.generate import _VERIFY_STREAM, LookupDrafts
+    from dlgo_amd.engine.generate import _VERIFY_STREAM, LookupDrafts, fill_drafts
     from dlgo_amd.sampling import uniform
     folder = folders["B", "float32"]
     cfg, w = plain.read_model(folder)
@@ -174,20 +205,23 @@ def test_sampling_with_drafts_is_what_the_formulas_say(folders):
     assert [r.tokens for r in llm.generate(prompts, *opts)] == [r.tokens for r in got]
     t = float(np.float32(0.25))
     decided = 0
-    for i, (p, r) in enumerate(zip(prompts, got)):
-        out, drafts = [], []
-        text = LookupDrafts(p)
-        while len(out) < 20:
-            u = [uniform(77 ^ _VERIFY_STREAM, i, len(out) + j) for j in range(len(drafts))] + [uniform(77, i, len(out))]
-            rows = range(len(p) + len(out) - 1, len(p) + len(out) + len(drafts))
-            logits = torch.as_tensor(plain.forward(cfg, w, p + out + drafts, rows=rows))
-            (kept,), (token,), _ = plain_verify(logits, drafts, [len(drafts)], [t], u, None)
-            decided += len(drafts)
-            new = drafts[:kept] + [token]
-            out += new
-            text.extend(new)
-            drafts = text.propose(min(3, 20 - len(out) - 1))
-        assert r.tokens == out, i
+    out, drafts, texts = [[] for _ in prompts], [[] for _ in prompts], [LookupDrafts(p) for p in prompts]
+    while any(len(o) < 20 for o in out):
+        live = [i for i, o in enumerate(out) if len(o) < 20]
+        for i in live:
+            u = [uniform(77 ^ _VERIFY_STREAM, i, len(out[i]) + j) for j in range(len(drafts[i]))] + [uniform(77, i, len(out[i]))]
+            at = len(prompts[i]) + len(out[i]) - 1
+            logits = torch.as_tensor(plain.forward(cfg, w, prompts[i] + out[i] + drafts[i], rows=range(at, at + len(drafts[i]) + 1)))
+            (kept,), (token,), _ = plain_verify(logits, drafts[i], [len(drafts[i])], [t], u, None)
+            decided += len(drafts[i])
+            new = drafts[i][:kept] + [token]
+            out[i] += new
+            texts[i].extend(new)
+        live = [i for i in live if len(out[i]) < 20]
+        room = [min(3, 20 - len(out[i]) - 1) for i in live]
+        for i, x in zip(live, fill_drafts([texts[i].propose(r) for i, r in zip(live, room)], room, [out[i][-1] for i in live])):
+            drafts[i] = x
+    assert [r.tokens for r in got] == out
     assert decided >= 6, "too few drafts: the check says little"
 
 
