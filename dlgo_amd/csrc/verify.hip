@@ -241,135 +241,17 @@ struct Whole {        // a row from its parts: 1 / sum, maximum, its index
   int arg;
 };
 
-// grid (ceil(parts / judge_run), sequences).  Every block of a sequence judges its drafts (from a few hundred numbers that
-// the first kernel left, eight lanes a row) and sums the weights of its parts of the row that the next token comes from.
-__global__ __launch_bounds__(THREADS) void verify_judge_kernel(Verify a) {
-  extern __shared__ __attribute__((aligned(16))) char lds[];
-  Whole* rows = (Whole*)lds;               // [most + 1] of the target, [most] of the drafts
-  __shared__ double ss[THREADS / WAVE];
-  const int part0 = blockIdx.x * a.judge_run, seq = blockIdx.y, wave = threadIdx.x / WAVE, lane = threadIdx.x & 63;
-  const int part1 = part0 + a.judge_run < a.parts ? part0 + a.judge_run : a.parts;
-  int c0, c1;
-  drafts_of(a, seq, c0, c1);
-  const int d = c1 - c0;
-  const float t = a.temperature[seq];
-  const bool greedy = !(t > 0.f);
-  const double c = greedy ? 1.0 : LOG2E / (double)t;
-  // a lane for each draft (every wave judges all of them): its token and the two logits
-  auto logits_of = [&](int j, bool& in, float& x, float& y) {
-    const int tok = a.tokens[c0 + j];
-    in = tok >= 0 && tok < a.vocab;
-    x = a.logits[(c0 + seq + j) * a.ldl + (in ? tok : 0)];
-    y = a.drafts ? a.drafts[(c0 + j) * a.ldd + (in ? tok : 0)] : 0.f;
-  };
-  bool in0 = false;
-  float x0 = 0.f, y0 = 0.f;
-  if (lane < d) logits_of(lane, in0, x0, y0);
-  const int n_rows = d + 1 + (a.drafts && !greedy ? d : 0), sub = threadIdx.x & 7;
-  for (int q0 = 0; q0 < n_rows; q0 += THREADS / 8) {
-    const int q = q0 + (int)threadIdx.x / 8, qc = q < n_rows ? q : n_rows - 1;
-    const Piece16* p = a.pieces + (size_t)(qc <= d ? c0 + seq + qc : a.d + a.n + c0 + qc - d - 1) * a.parts;
-    Whole w;
-    w.max = -INFINITY;
-    w.arg = -1;
-    for (int i = sub; i < a.parts; i += 8) take_max(w.max, w.arg, p[i].max, p[i].arg);
-#pragma unroll
-    for (int o = 4; o > 0; o >>= 1) {
-      const float m2 = __shfl_xor(w.max, o, WAVE);
-      const int at2 = __shfl_xor(w.arg, o, WAVE);
-      take_max(w.max, w.arg, m2, at2);
-    }
-    double sum = 0.0;
-    for (int i = sub; i < a.parts; i += 8) sum += p[i].sum * weight(p[i].max, w.max, c);
-#pragma unroll
-    for (int o = 4; o > 0; o >>= 1) sum += __shfl_xor(sum, o, WAVE);
-    w.inv = 1.0 / sum;
-    if (sub == 0 && q < n_rows) rows[q] = w;
-  }
-  __syncthreads();
-  int kept = d;
-  for (int j0 = 0; j0 < d && kept == d; j0 += WAVE) {
-    const int j = j0 + lane;
-    if (j0 > 0 && j < d) logits_of(j, in0, x0, y0);
-    bool keep = true;
-    if (j < d) {
-      double p, q = 1.0;
-      if (greedy) {
-        p = in0 && a.tokens[c0 + j] == rows[j].arg ? 1.0 : 0.0;
-        keep = p > 0.0;
-      } else {
-        p = in0 ? weight(x0, rows[j].max, c) * rows[j].inv : 0.0;
-        if (a.drafts) q = in0 ? weight(y0, rows[d + 1 + j].max, c) * rows[d + 1 + j].inv : 0.0;
-        keep = (double)a.uniform[c0 + seq + j] * q < p;
-      }
-      if (part0 == 0 && wave == 0 && a.probs) a.probs[c0 + j] = (float)p;
-    }
-    const unsigned long long refused = __ballot(!keep);
-    if (refused) kept = j0 + __builtin_ctzll(refused);
-  }
-  if (part0 == 0 && wave == 0 && a.probs)             // the drafts behind the first 64 and a refused one have a probability too
-    for (int j = (kept / WAVE + 1) * WAVE + lane; kept < d && j < d; j += WAVE) {
-      logits_of(j, in0, x0, y0);
-      a.probs[c0 + j] = !in0 ? 0.f : greedy ? (a.tokens[c0 + j] == rows[j].arg ? 1.f : 0.f) : (float)(weight(x0, rows[j].max, c) * rows[j].inv);
-    }
-  const bool refused = kept < d;
-  const Whole r = rows[kept], less = rows[refused && a.drafts && !greedy ? d + 1 + kept : kept];
-  const int row = c0 + seq + kept;
-  Choice ch;
-  ch.accepted = kept;
-  ch.row = row;
-  ch.draft_row = refused && !greedy && a.drafts ? c0 + kept : -1;
-  ch.without = refused && !greedy && !a.drafts ? a.tokens[c0 + kept] : -1;
-  ch.drawn = greedy ? (r.arg < 0 ? 0 : r.arg) : -1;
-  ch.tmax = r.max;
-  ch.dmax = less.max;
-  ch.tinv = r.inv;
-  ch.dinv = less.inv;
-  if (part0 == 0 && threadIdx.x == 0) a.choice[seq] = ch;
-  if (greedy) return;
-  if (!refused) {                          // the whole row: its parts' sums are known
-    const int part = part0 + (int)threadIdx.x;
-    if (part < part1) {
-      const Piece16 p = a.pieces[(size_t)row * a.parts + part];
-      a.mass[(size_t)seq * a.parts + part] = p.sum * weight(p.max, r.max, c) * r.inv;
-    }
-    return;
-  }
-  const float* src = a.logits + row * a.ldl;
-  const float* src2 = a.drafts ? a.drafts + (long long)ch.draft_row * a.ldd : src;
-  for (int part = part0; part < part1; ++part) {
-    float x[PER], y[PER];
-    load16(src, part * CHUNK, a.vocab, x);
-    load16(src2, part * CHUNK, a.vocab, y);
-    double s = 0.0;
-#pragma unroll
-    for (int k = 0; k < PER; ++k) {
-      double w = weight(x[k], r.max, c) * r.inv;
-      if (a.drafts) w -= weight(y[k], less.max, c) * less.inv;
-      else if (part * CHUNK + in_runs(k) == ch.without) w = 0.0;
-      s += fmax(w, 0.0);
-    }
-    s = wave_sum64(s);
-    if (part > part0) __syncthreads();     // the part before has been read
-    if (lane == 0) ss[wave] = s;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-      s = ss[0];
-#pragma unroll
-      for (int w = 1; w < THREADS / WAVE; ++w) s += ss[w];
-      a.mass[(size_t)seq * a.parts + part] = s;
-    }
-  }
-}
+// what a part adds to its row's probability
+__device__ __forceinline__ double share(const Piece16& p, float max, double inv, double c) { return p.sum * weight(p.max, max, c) * inv; }
 
-// grid (sequences).  The part whose running sum passes the target, then the element in it.
-__global__ __launch_bounds__(THREADS) void verify_draw_kernel(Verify a) {
+// Writes what was found of a sequence.  Where a token is still to be drawn: the part whose running sum passes the target,
+// then the element in it; mass(i) is what part i (the lane's number modulo 64) weighs.
+template <typename Mass>
+__device__ __forceinline__ void draw(const Verify& a, int seq, const Choice& ch, Mass mass) {
   __shared__ double wave_run[THREADS / WAVE];
   __shared__ int found;
-  const int seq = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x / WAVE;
-  const Choice ch = a.choice[seq];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x / WAVE;
   const float t = a.temperature[seq];
-  const double own = a.mass[(size_t)seq * a.parts + (lane < a.parts ? lane : 0)];      // of the first 64 parts
   int c0, c1;
   drafts_of(a, seq, c0, c1);
   const double u = (double)a.uniform[c1 + seq];
@@ -385,14 +267,17 @@ __global__ __launch_bounds__(THREADS) void verify_draw_kernel(Verify a) {
   // every wave by itself: the parts' masses one a lane, their running sums
   const Piece16* p = a.pieces + (size_t)ch.row * a.parts;
   bool plain = false;
+  double run64 = 0.0, v64 = 0.0;           // of the first 64 parts
   auto mass_of = [&](int i) {              // of part i, whose number is the lane's modulo 64
-    if (plain) return i < a.parts ? p[i].sum * weight(p[i].max, ch.tmax, c) * ch.tinv : 0.0;
-    return i < a.parts ? (i < WAVE ? own : a.mass[(size_t)seq * a.parts + i]) : 0.0;
+    if (plain) return i < a.parts ? share(p[i], ch.tmax, ch.tinv, c) : 0.0;
+    return i < a.parts ? mass(i) : 0.0;
   };
   auto total_of = [&]() {
-    double v = 0.0;
-    for (int i = lane; i < a.parts; i += WAVE) v += mass_of(i);
-    return wave_sum64(v);
+    v64 = mass_of(lane);
+    run64 = wave_running64(v64);
+    double sum = __shfl(run64, WAVE - 1, WAVE);
+    for (int i0 = WAVE; i0 < a.parts; i0 += WAVE) sum = __shfl(wave_running64(mass_of(i0 + lane)) + sum, WAVE - 1, WAVE);
+    return sum;
   };
   double total = total_of();
   if (!(total > 0.0)) {                    // nothing is left beside the draft's distribution: the target's own
@@ -403,8 +288,8 @@ __global__ __launch_bounds__(THREADS) void verify_draw_kernel(Verify a) {
   int part = -1, last_part = 0;
   double before = 0.0, last_before = 0.0, sum_so_far = 0.0;
   for (int i0 = 0; i0 < a.parts && part < 0; i0 += WAVE) {
-    const double v = mass_of(i0 + lane);
-    const double incl = wave_running64(v) + sum_so_far, excl = incl - v;
+    const double v = i0 == 0 ? v64 : mass_of(i0 + lane);
+    const double incl = i0 == 0 ? run64 : wave_running64(v) + sum_so_far, excl = incl - v;
     const unsigned long long over = __ballot(v > 0.0 && incl > target), some = __ballot(v > 0.0);
     if (some) {
       const int at = 63 - __builtin_clzll(some);
@@ -468,6 +353,172 @@ __global__ __launch_bounds__(THREADS) void verify_draw_kernel(Verify a) {
   if (threadIdx.x == 0) a.token[seq] = found < 0 ? 0 : found;
 }
 
+// grid (ceil(parts / judge_run), sequences).  Every block of a sequence judges its drafts (from a few hundred numbers that
+// the first kernel left, eight lanes a row) and sums the weights of its parts of the row that the next token comes from.
+// CERTAIN, where the drafts are: a refused one's row is the target's without one token, so all parts but that token's
+// weigh what the first kernel found, and one block a sequence does the rest, the draw included.
+template <bool CERTAIN>
+__global__ __launch_bounds__(THREADS) void verify_judge_kernel(Verify a) {
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  Whole* rows = (Whole*)lds;               // [most + 1] of the target, [most] of the drafts
+  __shared__ double ss[THREADS / WAVE];
+  const int part0 = blockIdx.x * a.judge_run, seq = blockIdx.y, wave = threadIdx.x / WAVE, lane = threadIdx.x & 63;
+  const int part1 = part0 + a.judge_run < a.parts ? part0 + a.judge_run : a.parts;
+  int c0, c1;
+  drafts_of(a, seq, c0, c1);
+  const int d = c1 - c0;
+  const float t = a.temperature[seq];
+  const bool greedy = !(t > 0.f);
+  const double c = greedy ? 1.0 : LOG2E / (double)t;
+  // a lane for each draft (every wave judges all of them): its token and the two logits
+  auto logits_of = [&](int j, bool& in, float& x, float& y) {
+    const int tok = a.tokens[c0 + j];
+    in = tok >= 0 && tok < a.vocab;
+    x = a.logits[(c0 + seq + j) * a.ldl + (in ? tok : 0)];
+    y = a.drafts ? a.drafts[(c0 + j) * a.ldd + (in ? tok : 0)] : 0.f;
+  };
+  bool in0 = false;
+  float x0 = 0.f, y0 = 0.f, u0 = 0.f;
+  if (lane < d) {
+    u0 = a.uniform[c0 + seq + lane];
+    logits_of(lane, in0, x0, y0);
+  }
+  const int n_rows = d + 1 + (a.drafts && !greedy ? d : 0), sub = threadIdx.x & 7;
+  for (int q0 = 0; q0 < n_rows; q0 += THREADS / 8) {
+    const int q = q0 + (int)threadIdx.x / 8, qc = q < n_rows ? q : n_rows - 1;
+    const Piece16* p = a.pieces + (size_t)(qc <= d ? c0 + seq + qc : a.d + a.n + c0 + qc - d - 1) * a.parts;
+    Whole w;
+    w.max = -INFINITY;
+    w.arg = -1;
+    double sum = 0.0;
+    // eight pieces a lane are asked for at once; a piece past the last is the last again and counts nothing
+    for (int i0 = 0; i0 < a.parts; i0 += 64) {
+      Piece16 v[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const int i = i0 + 8 * k + sub;
+        v[k] = p[i < a.parts ? i : a.parts - 1];
+      }
+      const float before = w.max;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) take_max(w.max, w.arg, v[k].max, v[k].arg);
+#pragma unroll
+      for (int o = 4; o > 0; o >>= 1) {
+        const float m2 = __shfl_xor(w.max, o, WAVE);
+        const int at2 = __shfl_xor(w.arg, o, WAVE);
+        take_max(w.max, w.arg, m2, at2);
+      }
+      if (i0 > 0) sum *= weight(before, w.max, c);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) sum += i0 + 8 * k + sub < a.parts ? v[k].sum * weight(v[k].max, w.max, c) : 0.0;
+    }
+#pragma unroll
+    for (int o = 4; o > 0; o >>= 1) sum += __shfl_xor(sum, o, WAVE);
+    w.inv = 1.0 / sum;
+    if (sub == 0 && q < n_rows) rows[q] = w;
+  }
+  __syncthreads();
+  int kept = d;
+  for (int j0 = 0; j0 < d && kept == d; j0 += WAVE) {
+    const int j = j0 + lane;
+    if (j0 > 0 && j < d) {
+      u0 = a.uniform[c0 + seq + j];
+      logits_of(j, in0, x0, y0);
+    }
+    bool keep = true;
+    if (j < d) {
+      double p, q = 1.0;
+      if (greedy) {
+        p = in0 && a.tokens[c0 + j] == rows[j].arg ? 1.0 : 0.0;
+        keep = p > 0.0;
+      } else {
+        p = in0 ? weight(x0, rows[j].max, c) * rows[j].inv : 0.0;
+        if (a.drafts) q = in0 ? weight(y0, rows[d + 1 + j].max, c) * rows[d + 1 + j].inv : 0.0;
+        keep = (double)u0 * q < p;
+      }
+      if (part0 == 0 && wave == 0 && a.probs) a.probs[c0 + j] = (float)p;
+    }
+    const unsigned long long refused = __ballot(!keep);
+    if (refused) kept = j0 + __builtin_ctzll(refused);
+  }
+  if (part0 == 0 && wave == 0 && a.probs)             // the drafts behind the first 64 and a refused one have a probability too
+    for (int j = (kept / WAVE + 1) * WAVE + lane; kept < d && j < d; j += WAVE) {
+      logits_of(j, in0, x0, y0);
+      a.probs[c0 + j] = !in0 ? 0.f : greedy ? (a.tokens[c0 + j] == rows[j].arg ? 1.f : 0.f) : (float)(weight(x0, rows[j].max, c) * rows[j].inv);
+    }
+  const bool refused = kept < d;
+  const Whole r = rows[kept], less = rows[refused && a.drafts && !greedy ? d + 1 + kept : kept];
+  const int row = c0 + seq + kept;
+  Choice ch;
+  ch.accepted = kept;
+  ch.row = row;
+  ch.draft_row = refused && !greedy && a.drafts ? c0 + kept : -1;
+  ch.without = refused && !greedy && !a.drafts ? a.tokens[c0 + kept] : -1;
+  ch.drawn = greedy ? (r.arg < 0 ? 0 : r.arg) : -1;
+  ch.tmax = r.max;
+  ch.dmax = less.max;
+  ch.tinv = r.inv;
+  ch.dinv = less.inv;
+  const Piece16* own = a.pieces + (size_t)row * a.parts;
+  const float* src = a.logits + row * a.ldl;
+  if constexpr (CERTAIN) {
+    const int special = ch.without >= 0 && ch.without < a.vocab ? ch.without / CHUNK : -1;
+    double s = 0.0;
+    if (special >= 0) {                    // the same in the whole block
+      float x[PER];
+      load16(src, special * CHUNK, a.vocab, x);
+#pragma unroll
+      for (int k = 0; k < PER; ++k) s += special * CHUNK + in_runs(k) == ch.without ? 0.0 : weight(x[k], r.max, c) * r.inv;
+      s = wave_sum64(s);
+      if (lane == 0) ss[wave] = s;
+      __syncthreads();
+      s = ss[0];
+#pragma unroll
+      for (int w = 1; w < THREADS / WAVE; ++w) s += ss[w];
+    }
+    draw(a, seq, ch, [&](int i) { return i == special ? s : share(own[i], r.max, r.inv, c); });
+    return;
+  }
+  if (part0 == 0 && threadIdx.x == 0) a.choice[seq] = ch;
+  if (greedy) return;
+  if (!refused) {                          // the whole row: its parts' sums are known
+    const int part = part0 + (int)threadIdx.x;
+    if (part < part1) a.mass[(size_t)seq * a.parts + part] = share(own[part], r.max, r.inv, c);
+    return;
+  }
+  const float* src2 = a.drafts + (long long)ch.draft_row * a.ldd;
+  for (int part = part0; part < part1; ++part) {
+    float x[PER], y[PER];
+    load16(src, part * CHUNK, a.vocab, x);
+    load16(src2, part * CHUNK, a.vocab, y);
+    double s = 0.0;
+#pragma unroll
+    for (int k = 0; k < PER; ++k) {
+      const double w = weight(x[k], r.max, c) * r.inv - weight(y[k], less.max, c) * less.inv;
+      s += fmax(w, 0.0);
+    }
+    s = wave_sum64(s);
+    if (part > part0) __syncthreads();     // the part before has been read
+    if (lane == 0) ss[wave] = s;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      s = ss[0];
+#pragma unroll
+      for (int w = 1; w < THREADS / WAVE; ++w) s += ss[w];
+      a.mass[(size_t)seq * a.parts + part] = s;
+    }
+  }
+}
+
+// grid (sequences).  Draws from what the second kernel left.
+__global__ __launch_bounds__(THREADS) void verify_draw_kernel(Verify a) {
+  const int seq = blockIdx.x, lane = threadIdx.x & 63;
+  const Choice ch = a.choice[seq];
+  const double* mass = a.mass + (size_t)seq * a.parts;
+  const double own = mass[lane < a.parts ? lane : 0];      // of the first 64 parts: asked for beside the choice
+  draw(a, seq, ch, [&](int i) { return i < WAVE ? own : mass[i]; });
+}
+
 static long long round16(long long n) { return (n + 15) / 16 * 16; }
 
 // bytes of scratch for n sequences with d drafts in all, over a vocabulary
@@ -499,8 +550,13 @@ extern "C" const char* dlgo_verify_drafts(const float* logits, long long ldl, co
   a.run = rows * parts >= 8192 ? 4 : 1;
   hipLaunchKernelGGL(verify_rows_kernel, dim3((unsigned)(rows * ((parts + a.run - 1) / a.run))), dim3(THREADS), 0, stream, a);
   DLGO_LAUNCH_CHECK("verify_drafts");
+  if (!drafts) {
+    hipLaunchKernelGGL(verify_judge_kernel<true>, dim3(1, (unsigned)n), dim3(THREADS), (most + 1) * (int)sizeof(Whole), stream, a);
+    DLGO_LAUNCH_CHECK("verify_drafts");
+    return nullptr;
+  }
   a.judge_run = n * parts >= 1024 ? 2 : 1;
-  hipLaunchKernelGGL(verify_judge_kernel, dim3((unsigned)((parts + a.judge_run - 1) / a.judge_run), (unsigned)n), dim3(THREADS), (2 * most + 1) * (int)sizeof(Whole), stream, a);
+  hipLaunchKernelGGL(verify_judge_kernel<false>, dim3((unsigned)((parts + a.judge_run - 1) / a.judge_run), (unsigned)n), dim3(THREADS), (2 * most + 1) * (int)sizeof(Whole), stream, a);
   DLGO_LAUNCH_CHECK("verify_drafts");
   hipLaunchKernelGGL(verify_draw_kernel, dim3((unsigned)n), dim3(THREADS), 0, stream, a);
   DLGO_LAUNCH_CHECK("verify_drafts");
