@@ -40,21 +40,14 @@ struct AttnQ8 {
   int ldq, ldo, n_rows, n_seq, n_heads, n_kv, group, n_slots, max_pages, n_pages, window;
   float scale_log2e;             // not negative; `flip` is its sign
   uint32_t flip;
-  int splits, fill;              // blocks that a sequence's pages may be dealt to: see splits_of
+  int max_q, shared;             // rows of a sequence that are looked at; blocks that take one share of its pages (kv heads * chunks)
+  int dealt, least, fill, most;  // how a sequence's pages are dealt to blocks: see Plan
 };
+enum { WHOLE, EVENLY, BY_LENGTH };
 
 // Waves of a block: four.  Eight leave room for one block a compute unit (a block's own start, its first trips to memory,
 // is then nobody's time to use): 64 sequences of 2,300 tokens 31.1 against 29.3 us, 16 sequences with drafts 21.6 against 18.7.
 #define WAVES 4
-
-// How many of the launch's blocks a sequence with n pages uses: enough to fill the chip (`fill`, known at the launch),
-// but not more than leave each wave a page, and so many that a wave has at most 16 pages.
-__device__ __forceinline__ int splits_of(const AttnQ8& a, int n) {
-  const int by_wave = (n + WAVES - 1) / WAVES, by_16 = (n + 16 * WAVES - 1) / (16 * WAVES);
-  int s = a.fill < by_wave ? a.fill : by_wave;
-  if (s < by_16) s = by_16;
-  return s < 1 ? 1 : (s > a.splits ? a.splits : s);
-}
 
 // The rows and pages of a sequence, from numbers that live on the device; nothing outside the buffers whatever they are.
 struct Span {
@@ -77,6 +70,47 @@ __device__ __forceinline__ Span span_of(const AttnQ8& a, int seq) {
   int last = (s.len - 1) / Q8_PAGE;
   if (last >= a.max_pages) last = a.max_pages - 1;
   s.n_pages = s.rows > 0 && last >= s.first_page ? last - s.first_page + 1 : 0;
+  return s;
+}
+
+// EVENLY: shares of a sequence with n pages: enough to fill the chip, but not more than leave each wave a page, and so many
+// that a wave has at most 16 pages.
+__device__ __forceinline__ int even_shares(const AttnQ8& a, int n) {
+  const int by_wave = (n + WAVES - 1) / WAVES, by_16 = (n + 16 * WAVES - 1) / (16 * WAVES);
+  int s = a.fill < by_wave ? a.fill : by_wave;
+  if (s < by_16) s = by_16;
+  return s < 1 ? 1 : (s > a.most ? a.most : s);
+}
+// BY_LENGTH: sequences are dealt out in shares of about the same number of pages, about BLOCKS blocks in all: one of n pages
+// has round(n / quota) shares, at least one, so that none is longer than one and a half quotas.  The lengths are on the
+// device, so every wave works the shares out from them (a lane a sequence), which costs it 0.7 us.
+#define BLOCKS 768
+struct Shares {
+  int quota;
+  __device__ __forceinline__ int of(int pages) const {
+    const int n = (pages + (quota >> 1)) / quota;
+    return n < 1 ? 1 : n;
+  }
+};
+__device__ __forceinline__ int wave_running(int v) {
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int o = 1; o < WAVE; o <<= 1) {
+    const int u = __shfl_up(v, o, WAVE);
+    if (lane >= o) v += u;
+  }
+  return v;
+}
+// `first`: what the lane's sequence (its number modulo 64) is among the first 64
+__device__ __forceinline__ Shares shares_of(const AttnQ8& a, const Span& first) {
+  const int lane = threadIdx.x & 63;
+  unsigned long long sum = lane < a.n_seq ? first.n_pages : 0;
+  for (int i = WAVE + lane; i < a.n_seq; i += WAVE) sum += span_of(a, i).n_pages;
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, WAVE);
+  const unsigned long long quota = (sum * a.shared + BLOCKS - 1) / BLOCKS;
+  Shares s;
+  s.quota = quota < (unsigned)a.least ? a.least : (quota > (1u << 30) ? 1 << 30 : (int)quota);
   return s;
 }
 
@@ -112,7 +146,7 @@ __device__ __forceinline__ bf16x8_t eight(uint32_t w0, uint32_t w1, float scale)
 __device__ __forceinline__ uint32_t first_bytes(uint32_t w, int n) { return n >= 4 ? w : (n <= 0 ? 0u : w & ((1u << (8 * n)) - 1u)); }
 
 // ---------------------------------------------------------------------------------------------------------------------
-// Few rows a sequence.  grid (kv heads * chunks of columns, sequences, splits), WAVES waves.  A wave holds a whole page of
+// Few rows a sequence.  grid: shares * chunks of columns * kv heads, WAVES waves.  A wave holds a whole page of
 // its head in registers: the keys of 16 tokens are KLOADS loads of 16 bytes a lane, the values of 16 elements one, all
 // of them consecutive in memory, and each is an operand of the matrix instructions as it lies once its bytes are
 // converted.  The next page's loads are on their way while this one is multiplied.  The scores come out with a lane
@@ -160,12 +194,47 @@ __global__ __launch_bounds__(WAVES* WAVE) __attribute__((amdgpu_waves_per_eu(EU(
   extern __shared__ __attribute__((aligned(16))) float merge[];    // [WAVES][COLS][HD], then [WAVES][COLS] maxima and sums
   const int lane = threadIdx.x & 63, g = lane >> 4, n = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);        // known to be the same in all lanes, as all that follows from it
-  const int kvh = blockIdx.x % a.n_kv, chunk = blockIdx.x / a.n_kv, seq = blockIdx.y, split = blockIdx.z;
-  const Span s = span_of(a, seq);
-  const int cols = s.rows * a.group, col0 = chunk * COLS(NC);
+  const int in_share = blockIdx.x % a.shared, kvh = in_share % a.n_kv, chunk = in_share / a.n_kv, item = blockIdx.x / a.shared;
+  Span s;
+  int split = 0, used = 1, place = item;               // the share's place among the partial results
+  if (a.dealt != BY_LENGTH) {
+    const int seq = item % a.n_seq;                     // WHOLE: item is below n_seq
+    s = span_of(a, seq);
+    if (a.dealt == EVENLY) {
+      used = even_shares(a, s.n_pages);
+      split = item / a.n_seq;
+      if (split >= used) return;
+      place = seq * a.most + split;
+    }
+  } else {
+    Span mine = span_of(a, lane < a.n_seq ? lane : a.n_seq - 1);
+    const Shares sh = shares_of(a, mine);
+    int before = 0, seq = -1;
+    for (int i0 = 0; i0 < a.n_seq; i0 += WAVE) {
+      const int i = i0 + lane;
+      if (i0 > 0) mine = span_of(a, i < a.n_seq ? i : a.n_seq - 1);
+      const int n = i < a.n_seq ? sh.of(mine.n_pages) : 0, upto = before + wave_running(n);
+      const unsigned long long past = __ballot(upto > item);
+      if (past) {
+        const int at = __builtin_ctzll(past);
+        seq = i0 + at;
+        used = __builtin_amdgcn_readlane(n, at);
+        split = item - (__builtin_amdgcn_readlane(upto, at) - used);
+        s.row0 = __builtin_amdgcn_readlane(mine.row0, at);
+        s.rows = __builtin_amdgcn_readlane(mine.rows, at);
+        s.start = __builtin_amdgcn_readlane(mine.start, at);
+        s.len = __builtin_amdgcn_readlane(mine.len, at);
+        s.slot = __builtin_amdgcn_readlane(mine.slot, at);
+        s.first_page = __builtin_amdgcn_readlane(mine.first_page, at);
+        s.n_pages = __builtin_amdgcn_readlane(mine.n_pages, at);
+        break;
+      }
+      before = __builtin_amdgcn_readlane(upto, WAVE - 1);
+    }
+    if (seq < 0) return;                   // fewer shares than there might have been
+  }
+  const int cols = (s.rows < a.max_q ? s.rows : a.max_q) * a.group, col0 = chunk * COLS(NC);
   if (col0 >= cols) return;
-  const int used = splits_of(a, s.n_pages);
-  if (split >= used) return;
   const int per = (s.n_pages + used - 1) / used;
   const int pg0 = s.first_page + split * per;
   const int pg1 = pg0 + per < s.first_page + s.n_pages ? pg0 + per : s.first_page + s.n_pages;      // pages [pg0, pg1)
@@ -174,7 +243,7 @@ __global__ __launch_bounds__(WAVES* WAVE) __attribute__((amdgpu_waves_per_eu(EU(
   // first + k * WAVES.
   const int32_t* table = a.page_table + (size_t)s.slot * a.max_pages;
   const int turns = pg1 - pg0 > wave ? (pg1 - pg0 - wave + WAVES - 1) / WAVES : 0;
-  const int first = turns > 0 ? pg0 + wave : s.first_page;
+  const int first = turns > 0 ? pg0 + wave : 0;
   int ids = table[first + (lane < turns ? lane : 0) * WAVES];
 
   // this lane's column of each of the NC blocks of 16: a row of the step and a head (a column past the last reads the last)
@@ -374,7 +443,7 @@ __global__ __launch_bounds__(WAVES* WAVE) __attribute__((amdgpu_waves_per_eu(EU(
       const float inv = L == 0.f ? 0.f : 1.0f / L;       // a row that sees no token at all (its pages are missing): zeros
       Elem<bf16_t>::store4(a.out + (size_t)row * a.ldo + (size_t)h * HD + e4 * 4, acc[0] * inv, acc[1] * inv, acc[2] * inv, acc[3] * inv);
     } else {
-      float* dst = a.part + ((size_t)((size_t)row * a.n_heads + h) * a.splits + split) * PART_ROW;
+      float* dst = a.part + ((size_t)((size_t)place * a.max_q + row - s.row0) * a.n_heads + h) * PART_ROW;
       *(f32x4_t*)(dst + e4 * 4) = acc;
       if (e4 == 0) {
         dst[HD] = M;
@@ -387,17 +456,31 @@ __global__ __launch_bounds__(WAVES* WAVE) __attribute__((amdgpu_waves_per_eu(EU(
 // One wave for each row and head that several blocks left results of.  grid (most rows a sequence * heads, sequences).
 #include "exact_begin.h"
 __global__ __launch_bounds__(WAVE) void attn_combine_kernel(AttnQ8 a) {
-  const int lane = threadIdx.x, h = blockIdx.x % a.n_heads, r = blockIdx.x / a.n_heads;
-  const Span s = span_of(a, blockIdx.y);
+  const int lane = threadIdx.x, h = blockIdx.x % a.n_heads, r = blockIdx.x / a.n_heads, seq = blockIdx.y;
+  const Span s = span_of(a, seq);
   if (r >= s.rows) return;
-  const int used = splits_of(a, s.n_pages);
-  if (used == 1) return;                               // written by its block
+  int used, place;                                     // the sequence's shares, and the first one's place
+  if (a.dealt == EVENLY) {
+    used = even_shares(a, s.n_pages);
+    place = seq * a.most;
+    if (used == 1) return;                             // written by its block
+  } else {
+    const Span mine = span_of(a, lane < a.n_seq ? lane : a.n_seq - 1);
+    const Shares sh = shares_of(a, mine);
+    used = sh.of(s.n_pages);
+    if (used == 1) return;
+    place = 0;
+    for (int i = lane; i < seq; i += WAVE) place += sh.of(i < WAVE ? mine.n_pages : span_of(a, i).n_pages);
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) place += __shfl_xor(place, o, WAVE);
+  }
   const int row = s.row0 + r;
-  const float* base = a.part + (size_t)((size_t)row * a.n_heads + h) * a.splits * PART_ROW;
+  const size_t step = (size_t)a.max_q * a.n_heads * PART_ROW;
+  const float* base = a.part + ((size_t)((size_t)place * a.max_q + r) * a.n_heads + h) * PART_ROW;
   const int per = (s.n_pages + used - 1) / used;
-  const int filled = (s.n_pages + per - 1) / per;      // blocks that were given pages
+  const int filled = (s.n_pages + per - 1) / per;      // shares that were given pages
   float M = -INFINITY;
-  for (int i = lane; i < filled; i += WAVE) M = fmaxf(M, base[(size_t)i * PART_ROW + HD]);
+  for (int i = lane; i < filled; i += WAVE) M = fmaxf(M, base[i * step + HD]);
   M = wave_max(M);
   constexpr int NE = (HD + WAVE - 1) / WAVE;
   float L = 0.f, acc[NE];
@@ -408,7 +491,7 @@ __global__ __launch_bounds__(WAVE) void attn_combine_kernel(AttnQ8 a) {
     float mm[8], ll[8], v[8][NE];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const float* p = base + (size_t)(i0 + i < filled ? i0 + i : filled - 1) * PART_ROW;
+      const float* p = base + (i0 + i < filled ? i0 + i : filled - 1) * step;
       mm[i] = p[HD];
       ll[i] = p[HD + 1];
 #pragma unroll
@@ -662,7 +745,8 @@ __global__ __launch_bounds__(PF_WAVES* WAVE) __attribute__((amdgpu_waves_per_eu(
 // What a launch looks like, from sizes that the host knows.  max_q_len and max_kv_len bound the sequences' rows and
 // lengths (a recorded launch passes the context's).
 struct Plan {
-  int tiled, nc, chunks, splits, fill;
+  int tiled, nc, chunks, dealt, least, fill, most;
+  long long items;                           // shares of sequences that there may be
 };
 static Plan plan_of(int n_seq, int n_heads, int n_kv, int max_q_len, int max_kv_len, int window) {
   Plan p = {};
@@ -678,13 +762,26 @@ static Plan plan_of(int n_seq, int n_heads, int n_kv, int max_q_len, int max_kv_
     const int seen = (window + max_q_len + Q8_PAGE - 2) / Q8_PAGE + 1;
     if (seen < pages) pages = seen;
   }
-  const long long pairs = (long long)n_seq * n_kv * p.chunks;
-  const int target = 512;
-  p.fill = pairs >= target ? 1 : (int)((target + pairs - 1) / pairs);
-  const int by_wave = (pages + WAVES - 1) / WAVES, by_16 = (pages + 16 * WAVES - 1) / (16 * WAVES);
-  p.splits = p.fill < by_wave ? p.fill : by_wave;
-  if (p.splits < by_16) p.splits = by_16;
-  if (p.splits < 1) p.splits = 1;
+  // How the pages are dealt (head size 64 and 128, us): with up to a quarter of the chip's blocks evenly, each sequence
+  // to as many blocks as any (one sequence of 2,300 tokens 8.4 against 9.9 by length, 16 with drafts 18.1 against 21.3);
+  // with more of them by length, where an even deal leaves the longest to too few (32 sequences of 64 to 8,192 tokens 56.9
+  // against 63.6); and where the sequences fill the chip each to one block, unless some may be longer than 96 pages.
+  const long long blocks = (long long)n_seq * n_kv * p.chunks;
+  const int chip = 512;
+  p.items = n_seq;
+  if (blocks <= chip / 4) {
+    const int by_wave = (pages + WAVES - 1) / WAVES, by_16 = (pages + 16 * WAVES - 1) / (16 * WAVES);
+    p.fill = (int)((chip + blocks - 1) / blocks);
+    p.most = p.fill < by_wave ? p.fill : by_wave;
+    if (p.most < by_16) p.most = by_16;
+    if (p.most < 1) p.most = 1;
+    p.dealt = p.most > 1 ? EVENLY : WHOLE;
+    p.items *= p.most;
+  } else {
+    p.least = blocks >= chip ? 16 * WAVES : WAVES;
+    p.dealt = pages + p.least / 2 >= 2 * p.least ? BY_LENGTH : WHOLE;        // the least length with two shares
+    if (p.dealt) p.items += BLOCKS / (n_kv * p.chunks);
+  }
   return p;
 }
 
@@ -694,7 +791,7 @@ extern "C" int dlgo_attention_q8_head_dim() { return HD; }
 extern "C" long long dlgo_attention_q8_scratch(int n_rows, int n_seq, int n_heads, int n_kv, int max_q_len, int max_kv_len, int window) {
   if (n_rows <= 0 || n_seq <= 0 || n_kv <= 0 || n_heads < n_kv || max_q_len <= 0 || max_kv_len <= 0) return 0;
   const Plan p = plan_of(n_seq, n_heads, n_kv, max_q_len, max_kv_len, window);
-  return p.tiled || p.splits <= 1 ? 0 : (long long)n_rows * n_heads * p.splits * PART_ROW;
+  return p.tiled || !p.dealt ? 0 : p.items * max_q_len * n_heads * PART_ROW;
 }
 
 template <int NC>
@@ -725,7 +822,7 @@ extern "C" const char* dlgo_attention_q8(const void* q, int ldq, void* out, int 
   const Plan p = plan_of(n_seq, n_heads, n_kv, max_q_len, max_kv_len, window);
   AttnQ8 a = {(const bf16_t*)q, (bf16_t*)out, part, cu_q, start_pos, slots, page_table, (const uint8_t*)cache, page_stride, ldq, ldo, n_rows, n_seq,
               n_heads, n_kv, n_heads / n_kv, n_slots, max_pages, n_pages, window > 0 ? window : 0,
-              (scale < 0 ? -scale : scale) * 1.44269504088896341f, scale < 0 ? 0x80008000u : 0u, p.splits, p.fill};
+              (scale < 0 ? -scale : scale) * 1.44269504088896341f, scale < 0 ? 0x80008000u : 0u, max_q_len, n_kv * p.chunks, p.dealt, p.least, p.fill, p.most};
   hipError_t e = hipSuccess;
   if (p.tiled) {
     const int tokens = PF_WAVES * 32 / a.group, n_tiles = (max_q_len + tokens - 1) / tokens;
@@ -735,15 +832,15 @@ extern "C" const char* dlgo_attention_q8(const void* q, int ldq, void* out, int 
     if (lds > 64 * 1024) e = hipFuncSetAttribute((const void*)attn_prefill_kernel, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
     if (e == hipSuccess) hipLaunchKernelGGL(attn_prefill_kernel, dim3((unsigned)blocks), dim3(PF_WAVES * WAVE), lds, stream, a, tokens);
   } else {
-    DLGO_REQUIRE(p.splits <= 65535, "attention_q8: sequences of %d tokens are too long", max_kv_len);
-    const long long need = p.splits > 1 ? (long long)n_rows * n_heads * p.splits * PART_ROW : 0;
+    const long long need = p.dealt ? p.items * max_q_len * n_heads * PART_ROW : 0, blocks = p.items * a.shared;
     DLGO_REQUIRE(need == 0 || (part && part_elems >= need && ((uintptr_t)part & 15) == 0), "attention_q8: scratch of %lld floats is needed, %lld given", need, part ? part_elems : 0ll);
-    const dim3 grid((unsigned)(n_kv * p.chunks), (unsigned)n_seq, (unsigned)p.splits);
+    DLGO_REQUIRE(blocks < (1ll << 31), "attention_q8: too many rows at once");
+    const dim3 grid((unsigned)blocks);
     e = hipErrorInvalidValue;
     if (p.nc == 1) e = launch_decode<1>(a, grid, stream);
     if constexpr (NC_MOST >= 2) if (p.nc == 2) e = launch_decode<2>(a, grid, stream);
     if constexpr (NC_MOST >= 4) if (p.nc == 4) e = launch_decode<4>(a, grid, stream);
-    if (e == hipSuccess && p.splits > 1) {
+    if (e == hipSuccess && p.dealt) {
       DLGO_LAUNCH_CHECK("attention_q8");
       hipLaunchKernelGGL(attn_combine_kernel, dim3((unsigned)(max_q_len * n_heads), (unsigned)n_seq), dim3(WAVE), 0, stream, a);
     }

@@ -349,6 +349,51 @@ def test_attention_with_a_table_for_far_longer_sequences():
             s.check(s.attend(q, bound_len=bound), q)
 
 
+UNEQUAL = [   # sequences, rows each, the longest pasts, H, KV, hd, window: pages dealt by length, in groups of 64 sequences
+    (150, (1,), [1300, 40], 3, 1, 16, 0),
+    (130, (0, 1, 2), [700, 650, 5], 6, 1, 32, 90),
+    (20, (1,), [9000, 300], 32, 8, 64, 0),
+    (40, (2, 1), [2100, 100], 8, 4, 48, 0),
+    (17, (1,), [1500, 900], 160, 4, 64, 0),               # two blocks for a group's heads
+    (70, (1,), [7000, 130], 8, 8, 16, 0),                 # the sequences alone fill the chip, one is far longer
+    (33, (3, 1), [500, 2500], 8, 4, 256, 0),
+]
+
+
+@pytest.mark.parametrize("n,rows,longest,H,KV,hd,window", UNEQUAL)
+def test_attention_over_many_unequal_sequences(n, rows, longest, H, KV, hd, window):
+    rng = np.random.default_rng(n + hd)
+    past = rng.integers(0, 130, size=n).tolist()
+    for i, p in zip(rng.permutation(n), longest):
+        past[i] = p
+    s = Step([rows[i % len(rows)] for i in range(n)], past, H, KV, hd, seed=n)
+    s.fill()
+    q = torch.randn(s.rows, H * hd, generator=s.gen).bfloat16().to(DEV)
+    s.check(s.attend(q, window), q, window)
+    # bounds for longer sequences and more rows
+    s.check(s.attend(q, window, bound_len=s.table.shape[1] * PAGE, bound_q=max(rows) + 1), q, window)
+
+
+@pytest.mark.parametrize("rows,n,window", [(1, 3, 10), (1, 3, 0), (1, 40, 10), (40, 2, 10)])
+def test_positions_behind_the_table(rows, n, window):
+    """Nothing is read past the table's end: with a window such a row sees nothing and gets zeros.  (Without one it sees what
+    the table holds, places that nothing was stored in among it, so its numbers are anybody's.)"""
+    s = Step([rows] * n, [70] * n, 8, 4, 64, seed=rows)
+    s.fill()
+    q = torch.randn(s.rows, 8 * 64, generator=s.gen).bfloat16().to(DEV)
+    past = list(s.past)
+    s.past = [p if i % 2 else 64 * s.table.shape[1] + 500 for i, p in enumerate(past)]
+    out = s.attend(q, window, bound_len=20000)
+    s.past = past
+    out = out.view(n, rows, -1)
+    for i in range(0, n, 2):
+        assert not window or (out[i] == 0).all()
+    want, mag = s.wanted(q, window)
+    for i in range(1, n, 2):
+        off = (out[i].double().cpu() - want.view(n, rows, -1)[i]).abs()
+        assert (off <= 2.0 ** -8 * want.view(n, rows, -1)[i].abs() + (2.0 ** -8 + 2.0 ** -10) * mag.view(n, rows, -1)[i] + 1e-30).all()
+
+
 def test_attention_scales_of_either_sign_and_peaked_scores():
     for q_lens, hd in (([1, 2], 64), ([80], 64), ([3], 128)):
         s = Step(q_lens, [300] * len(q_lens), 8, 2, hd, seed=5)
