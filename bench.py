@@ -2,6 +2,7 @@
 """Decode and prefill throughput of the Llama 3.2 1B shape on one MI355X.
 
     python bench.py [--gpus 1] [--steps K] [--warmup W] [--batch 8] [--layers L] [--dtype bf16|fp32]
+                    [--cache-dtype e4m3]
 
 A step is one decode step of the whole batch as the library's own generation loop
 runs it (dlgo_amd.engine.generate): greedy choice of the next tokens on the device,
@@ -57,7 +58,9 @@ def weight_bytes(cfg, elem):
     return (cfg.num_hidden_layers * per_layer + head) * elem + norms
 
 
-def kv_bytes_per_token(cfg, elem):
+def kv_bytes_per_token(cfg, elem, cache_dtype=None):
+    if cache_dtype == "e4m3":       # a byte an element, and one for each head's power of two
+        return cfg.num_hidden_layers * 2 * (cfg.kv_dim + cfg.num_key_value_heads)
     return cfg.num_hidden_layers * 2 * cfg.kv_dim * elem
 
 
@@ -84,7 +87,8 @@ def ragged(args, cfg, full_layers, elem) -> int:
     lens = rng.integers(lo, hi + 1, size=n)
     prompts = [rng.integers(0, cfg.vocab_size, size=int(k)).tolist() for k in lens]
     held = sum((int(k) + new + 63) // 64 * 64 for k in lens)
-    eng = Engine.from_random(cfg, seed=0, dtype=args.dtype, max_tokens=held, max_ctx=ctx, max_slots=n, graph_max_batch=n)
+    eng = Engine.from_random(cfg, seed=0, dtype=args.dtype, max_tokens=held, max_ctx=ctx, max_slots=n, graph_max_batch=n,
+                             cache_dtype=args.cache_dtype)
     sampler = Sampler(eng.vocab, eng.device, max_rows=n)
     conf = GenerateConfig(max_tokens=new, sampler=SamplerConfig(temperature=0.0), seed=1, ignore_eos=True)
     runs = []
@@ -94,7 +98,7 @@ def ragged(args, cfg, full_layers, elem) -> int:
     st = sorted(runs, key=lambda r: r.generate_ms)[2]
     steps = st.steps
     mean_ctx = float(lens.mean()) + (new + 1) / 2.0
-    step_bytes = weight_bytes(cfg, elem) + n * mean_ctx * kv_bytes_per_token(cfg, elem)
+    step_bytes = weight_bytes(cfg, elem) + n * mean_ctx * kv_bytes_per_token(cfg, elem, args.cache_dtype)
     achieved = step_bytes / (st.generate_ms / 1e3 / steps)
     flops = sum(prefill_flops(cfg, int(k)) for k in lens)
     line = {
@@ -107,7 +111,7 @@ def ragged(args, cfg, full_layers, elem) -> int:
                    "head_dim": cfg.head_dim, "intermediate": cfg.intermediate_size, "vocab": cfg.vocab_size,
                    "tied_embeddings": cfg.tie_word_embeddings, "global_batch": n, "seq_len": ctx,
                    "prompt_tokens": int(lens.sum()), "new_tokens": new, "parallelism": "single-gpu",
-                   "kv_cache_dtype": args.dtype, "sampling": "greedy, through the generation loop"},
+                   "kv_cache_dtype": args.cache_dtype or args.dtype, "sampling": "greedy, through the generation loop"},
         "prefill": {"value": round(st.prompt_tokens / st.prefill_ms * 1e3, 1), "tokens": int(st.prompt_tokens),
                     "ms": round(st.prefill_ms, 3), "frac": round(flops / (st.prefill_ms / 1e3) / FLOP_PEAK[args.dtype], 4)},
         "roofline": {"bound": "hbm", "achieved": round(achieved / 1e9, 1), "peak": HBM_PEAK / 1e9, "unit": "GB/s",
@@ -200,6 +204,7 @@ def main() -> int:
     ap.add_argument("--batch", type=int, default=8)
     ap.add_argument("--layers", type=int, default=0, help="fewer layers than the model has (0 = all)")
     ap.add_argument("--dtype", default="bf16", choices=["bf16", "fp32"])
+    ap.add_argument("--cache-dtype", default=None, choices=["e4m3"], help="keys and values in 8 bits (default: as --dtype; bf16 only)")
     ap.add_argument("--points", default="1,64", help="other batch sizes to report, comma separated ('' = none)")
     ap.add_argument("--point-steps", type=int, default=64)
     ap.add_argument("--no-prefill", action="store_true")
@@ -243,7 +248,7 @@ def main() -> int:
         print(f"bench.py: {PROMPT} prompt tokens, warmup and timed steps need {per_seq} tokens, the context is {CONTEXT}")
         return 2
     eng = Engine.from_random(cfg, seed=0, dtype=args.dtype, max_tokens=most * ((per_seq + 63) // 64 * 64), max_ctx=CONTEXT,
-                             max_step_tokens=8192, graph_max_batch=max(most, 8))
+                             max_step_tokens=8192, graph_max_batch=max(most, 8), cache_dtype=args.cache_dtype)
     sampler = Sampler(eng.vocab, eng.device, max_rows=most)
     rng = np.random.default_rng(0)
 
@@ -278,7 +283,7 @@ def main() -> int:
     step_s, mean_ctx, regions = decode(args.batch, args.steps, args.warmup)
     ms_step = step_s * 1000.0
     value = args.batch / step_s
-    step_bytes = weight_bytes(cfg, elem) + args.batch * mean_ctx * kv_bytes_per_token(cfg, elem)
+    step_bytes = weight_bytes(cfg, elem) + args.batch * mean_ctx * kv_bytes_per_token(cfg, elem, args.cache_dtype)
     achieved = step_bytes / step_s
 
     prefill = None
@@ -310,7 +315,7 @@ def main() -> int:
                    "hidden": cfg.hidden_size, "heads": cfg.num_attention_heads, "kv_heads": cfg.num_key_value_heads,
                    "head_dim": cfg.head_dim, "intermediate": cfg.intermediate_size, "vocab": cfg.vocab_size,
                    "tied_embeddings": cfg.tie_word_embeddings, "global_batch": args.batch, "seq_len": CONTEXT,
-                   "prompt_len": PROMPT, "parallelism": "single-gpu", "kv_cache_dtype": args.dtype,
+                   "prompt_len": PROMPT, "parallelism": "single-gpu", "kv_cache_dtype": args.cache_dtype or args.dtype,
                    "sampling": "greedy, through the generation loop"},
         "roofline": {"bound": "hbm", "achieved": round(achieved / 1e9, 1), "peak": HBM_PEAK / 1e9, "unit": "GB/s",
                      "frac": round(achieved / HBM_PEAK, 4)},

@@ -11,8 +11,8 @@
 //                        (sequence, kv head) are dealt to the waves of a block, and to several blocks where there are
 //                        too few; the columns of the matrix products are the group's heads of the sequence's rows.
 //   attn_combine_kernel  joins what several blocks left for a row.
-//   attn_prefill_kernel  prompts and pieces of prompts: 128 or 256 columns a block, pages turned to bfloat16 on their
-//                        way into LDS.
+//   attn_prefill_kernel  prompts and pieces of prompts (more than 64 rows * heads of a group): 128 columns a block, pages
+//                        turned to bfloat16 on their way into LDS.
 //
 // computerex/dlgo attends over float32 rows of the cache, one query at a time (models/llm/forward.go:258-278).
 #include "q8_page.h"
@@ -152,7 +152,14 @@ __device__ __forceinline__ uint32_t first_bytes(uint32_t w, int n) { return n >=
 // converted.  The next page's loads are on their way while this one is multiplied.  The scores come out with a lane
 // holding four neighbouring tokens of a column, which is the order of the values' bytes: no lane hands anything to
 // another but the two exchanges of the maximum.
-// Bound by memory: see the notes at the launcher.
+//
+// Bound by memory where there is much of it: 64 sequences of 2,048 to 2,303 tokens, 32 heads of 64 over 8: 145 MB in 28.7 us,
+// 5.1 TB/s, what a large copy reaches on this chip; 32 sequences of 64 to 8,192 tokens, heads of 128: 273 MB in 53 us and 5
+// for the join, 4.7 TB/s.  By latency where there is little: a block needs three trips to memory before its first product
+// (the sequence's numbers, its page numbers, the page) and hands its result over, 5 us in all: one sequence of 2,300
+// tokens takes 5.2 us and 4 for the join; 16 with up to six drafted tokens each (35 MB) 14.7 and 4.
+// Measured and not kept: eight waves a block (see WAVES), one page's registers in place of two (the same), 128 registers
+// a lane (spills), 4 or 8 pages a wave at least (slower from 8 sequences on).
 #define COLS(NC) (16 * (NC))
 #define NC_MOST (HD <= 64 ? 4 : (HD <= 128 ? 2 : 1))       // blocks of 16 columns whose sums a wave's registers hold beside two pages
 
@@ -514,10 +521,18 @@ __global__ __launch_bounds__(WAVE) void attn_combine_kernel(AttnQ8 a) {
 #include "exact_end.h"
 
 // ---------------------------------------------------------------------------------------------------------------------
-// Prompts.  A block of four waves takes 128 * CW columns (tokens x the heads of a group) of a sequence and walks the pages.
+// Prompts.  A block of four waves takes 128 columns (tokens x the heads of a group) of a sequence and walks the pages.
 // A page's bytes are turned to bfloat16 once for all its columns on the way into LDS (keys and values with their powers
 // of two: exact), the next page's bytes are on their way meanwhile, and the two places in LDS are used in turn, so that
 // a page costs one barrier.  Scores are kept transposed (keys x columns): a lane owns a column.
+//
+// Bound by instruction issue: a page is 32 scores a lane to scale, compare, raise and round beside 16 (head size 64) or 32
+// (128) matrix instructions, and one wave a SIMD finds the two of little help to each other, two waves do (381 us, not 768,
+// for 8 prompts of 64 to 2,048 tokens behind up to 2,048, 32 heads of 128 over 8).  Operands asked for four steps ahead: 366;
+// sums rescaled only where a maximum has grown and maxima exchanged without LDS: 349; pages two ahead: 319 to 334, 660
+// TFLOP/s.  A lone prompt of 2,048 tokens (heads of 64, 38.8 us) waits for its last tiles, 32 pages of 1.1 us one after the
+// other.  Measured and not kept: 64 columns a wave (78 us), eight waves with 256 columns (50 to 59), two teams of waves on
+// alternate pages (45), the scores of the next page beside this one's softmax (-3% for heads of 64, spills for 128).
 #define PF_WAVES 4
 #define PF_EU (HD <= 128 ? 2 : 1)           // waves a SIMD that the registers are to allow
 #define DT ((HD + 31) / 32)                 // tiles of 32 elements of the result

@@ -1,7 +1,8 @@
 """The verification of drafted tokens (verify_drafts) against a plain computation in 64 bits.
 
-Kept drafts and tokens are whole numbers and have to be equal: both sides decide with 64-bit sums, and a border that a
-rounding (2^-50 of the whole) could move is met by one uniform number in 10^12.  Probabilities are 64-bit values rounded to
+Kept drafts and tokens are whole numbers and have to be equal: both sides decide with 64-bit sums.  The kernel's weights are
+off by at most 1.1 * 10^-12 of themselves, each differently, so a border between two tokens moves by at most that much of the
+whole, and a draw over a few thousand tokens meets a border that moved for one uniform number in 10^8.  Probabilities are 64-bit values rounded to
 float32 once: 2^-24 of themselves, 2^-23 allowed."""
 import math
 
