@@ -7,7 +7,8 @@
 // float32 (memory/kvcache.go:5-9); its weights' 8-bit blocks carry a scale each (quant/dequant.go), as tokens do here.
 //
 // Bound by memory: a row is read once (the second read of a partner piece hits the cache), queries are written in
-// bfloat16, keys and values in 8 bits.
+// bfloat16, keys and values in 8 bits: 17,408 rows of 24 heads of 128 over 8, 330 MB, in 65.5 us, 5.0 TB/s.  Eight single
+// tokens take 4.5 us, a launch and three trips to memory.
 #include "q8_page.h"
 // everything here is float32 arithmetic whatever the storage type: no approximation can be named (exact_begin.h)
 #include "exact_begin.h"
@@ -24,6 +25,9 @@ struct RopeQ8 {
   const int32_t* page_table;
   long long page_stride;
   int ld, ldq, n_tokens, n_heads, n_kv, hd, rot, interleaved, table_rows, n_seq, n_slots, max_pages, n_pages;
+  const float* part;             // where the product that makes the rows left the runs of its inner sum unsummed: n_parts
+  long long plane;               // planes of float32, `plane` apart, rows part_ld apart
+  int n_parts, part_ld;
 };
 
 static __device__ __forceinline__ void load8(const bf16_t* p, float* f) {
@@ -34,19 +38,50 @@ static __device__ __forceinline__ void load8(const bf16_t* p, float* f) {
   f[6] = __uint_as_float(u.w << 16); f[7] = __uint_as_float(u.w & 0xffff0000u);
 }
 
+// The sum of the runs in their order, B of them asked for at once; one past the last is the last again and is not added.
+template <int B>
+static __device__ __forceinline__ void sum8(const RopeQ8& a, const float* p, float* f) {
+  for (int s0 = 0; s0 < a.n_parts; s0 += B) {
+    float4 v[B][2];
+#pragma unroll
+    for (int i = 0; i < B; ++i) {
+      const float* q = p + (s0 + i < a.n_parts ? s0 + i : a.n_parts - 1) * a.plane;
+      v[i][0] = *(const float4*)q;
+      v[i][1] = *(const float4*)(q + 4);
+    }
+#pragma unroll
+    for (int i = 0; i < B; ++i) {
+      const float w[8] = {v[i][0].x, v[i][0].y, v[i][0].z, v[i][0].w, v[i][1].x, v[i][1].y, v[i][1].z, v[i][1].w};
+#pragma unroll
+      for (int e = 0; e < 8; ++e) f[e] = s0 + i == 0 ? w[e] : (s0 + i < a.n_parts ? f[e] + w[e] : f[e]);
+    }
+  }
+}
+// Eight elements of row t from column `col` on: from the rows themselves or, SUMS, from the runs.
+template <bool SUMS>
+static __device__ __forceinline__ void row8(const RopeQ8& a, int t, int col, float* f) {
+  if constexpr (!SUMS) {
+    load8(a.qkv + (size_t)t * a.ld + col, f);
+  } else {
+    const float* p = a.part + (size_t)t * a.part_ld + col;
+    if (a.n_parts <= 2) sum8<2>(a, p, f);
+    else sum8<4>(a, p, f);
+  }
+}
+
 static __device__ __forceinline__ void store8(bf16_t* p, const float* f) {
   *(uint4*)p = make_uint4(Elem<bf16_t>::pair(f[0], f[1]), Elem<bf16_t>::pair(f[2], f[3]), Elem<bf16_t>::pair(f[4], f[5]), Elem<bf16_t>::pair(f[6], f[7]));
 }
 
-// Eight elements of a head from element d0 on, rotated.  PIECES: pairs lie in this piece (interleaved) or are this piece
+// Eight elements of a head (from column `col` of row t on) from element d0 on, rotated.  PIECES: pairs lie in this piece (interleaved) or are this piece
 // and the one half a rotated width away, all 16-byte aligned; else element by element.
-template <bool PIECES>
-static __device__ __forceinline__ void rotated8(const RopeQ8& a, const bf16_t* head, int pos, int d0, float* y) {
+template <bool PIECES, bool SUMS>
+static __device__ __forceinline__ void rotated8(const RopeQ8& a, int t, int col, int pos, int d0, float* y) {
   const int half = a.rot / 2;
   // a position beyond the table is the caller's mistake: it must not become a read out of bounds
   const size_t at = (size_t)(pos < 0 ? 0 : (pos < a.table_rows ? pos : a.table_rows - 1)) * half;
   if constexpr (PIECES) {
-    load8(head + d0, y);
+    row8<SUMS>(a, t, col + d0, y);
     if (!a.cos_t || d0 >= a.rot) return;
     float c[8], s[8], x[8];
     if (a.interleaved) {
@@ -62,7 +97,7 @@ static __device__ __forceinline__ void rotated8(const RopeQ8& a, const bf16_t* h
     }
     const bool low = d0 < half;
     const int i0 = low ? d0 : d0 - half;
-    load8(head + (low ? d0 + half : d0 - half), x);
+    row8<SUMS>(a, t, col + (low ? d0 + half : d0 - half), x);
 #pragma unroll
     for (int e = 0; e < 8; e += 4) {
       *(float4*)(c + e) = *(const float4*)(a.cos_t + at + i0 + e);
@@ -71,6 +106,7 @@ static __device__ __forceinline__ void rotated8(const RopeQ8& a, const bf16_t* h
 #pragma unroll
     for (int e = 0; e < 8; ++e) y[e] = low ? rotated_lo(y[e], x[e], c[e], s[e]) : rotated_hi(x[e], y[e], c[e], s[e]);
   } else {
+    const bf16_t* head = a.qkv + (size_t)t * a.ld + col;
 #pragma unroll 1
     for (int e = 0; e < 8; ++e) {
       const int d = d0 + e;
@@ -87,11 +123,12 @@ static __device__ __forceinline__ void rotated8(const RopeQ8& a, const bf16_t* h
   }
 }
 
-template <bool PIECES>
-static __device__ __forceinline__ void plain8(const bf16_t* p, float* y) {
+template <bool PIECES, bool SUMS>
+static __device__ __forceinline__ void plain8(const RopeQ8& a, int t, int col, float* y) {
   if constexpr (PIECES) {
-    load8(p, y);
+    row8<SUMS>(a, t, col, y);
   } else {
+    const bf16_t* p = a.qkv + (size_t)t * a.ld + col;
 #pragma unroll 1
     for (int e = 0; e < 8; ++e) y[e] = bf16_to_f32(p[e]);
   }
@@ -135,22 +172,23 @@ static __device__ __forceinline__ long long page_of(const RopeQ8& a, int t, int 
 }
 
 // The queries.  A thread takes a piece of eight elements, or the two pieces whose elements are each other's partners, of
-// QH heads of a row: the angles are read once for all of them, and their loads are asked for together.  It writes only
+// QH (four) heads of a row: the angles are read once for all of them, and their loads are asked for together.  It writes only
 // what it has read, so q_out may be the queries' own place in qkv.
-#define QH 4
+// (One head where the rows are unsummed runs: those are the loads that count then.  64 tokens, two runs: 8.9 -> 6.3 us.)
 struct QueryUnits {
   int far, per_head, groups;      // pairs of pieces half a rotated width apart; units a head; groups of QH heads
 };
-static __host__ __device__ __forceinline__ QueryUnits query_units(int n_heads, int hd, int rot, bool pieces, bool rotates, bool interleaved) {
+static __host__ __device__ __forceinline__ QueryUnits query_units(int QH, int n_heads, int hd, int rot, bool pieces, bool rotates, bool interleaved) {
   QueryUnits u;
   u.far = rotates && !interleaved ? rot / 16 : 0;
   u.per_head = pieces ? u.far + (hd - 16 * u.far) / 8 : 1;
   u.groups = (n_heads + QH - 1) / QH;
   return u;
 }
-template <bool PIECES>
+template <bool PIECES, bool SUMS>
 static __device__ __forceinline__ void queries(const RopeQ8& a, long long idx) {
-  const QueryUnits u = query_units(a.n_heads, a.hd, a.rot, PIECES, a.cos_t != nullptr, a.interleaved != 0);
+  constexpr int QH = SUMS ? 1 : 4;
+  const QueryUnits u = query_units(QH, a.n_heads, a.hd, a.rot, PIECES, a.cos_t != nullptr, a.interleaved != 0);
   const int per_row = u.groups * u.per_head;
   if (idx >= (long long)a.n_tokens * per_row) return;
   const int t = (int)(idx / per_row), c = (int)(idx % per_row), h0 = c / u.per_head * QH, unit = c % u.per_head;
@@ -163,11 +201,13 @@ static __device__ __forceinline__ void queries(const RopeQ8& a, long long idx) {
     const bool far = unit < u.far;
     const int d0 = far ? unit * 8 : 16 * u.far + (unit - u.far) * 8, d1 = far ? d0 + half : d0;
     uint4 lo[QH], hi[QH];
+    if constexpr (!SUMS) {
 #pragma unroll
-    for (int h = 0; h < QH; ++h) {                       // a head past the last: the last again
-      const bf16_t* p = src + (size_t)(h < heads ? h : heads - 1) * a.hd;
-      lo[h] = *(const uint4*)(p + d0);
-      hi[h] = *(const uint4*)(p + d1);
+      for (int h = 0; h < QH; ++h) {                     // a head past the last: the last again
+        const bf16_t* p = src + (size_t)(h < heads ? h : heads - 1) * a.hd;
+        lo[h] = *(const uint4*)(p + d0);
+        hi[h] = *(const uint4*)(p + d1);
+      }
     }
     const bool turns = a.cos_t && d0 < a.rot;
     float cs[8], sn[8];
@@ -183,8 +223,13 @@ static __device__ __forceinline__ void queries(const RopeQ8& a, long long idx) {
     for (int h = 0; h < QH; ++h) {
       if (h >= heads) break;
       float x[8], y[8];
-      load8((const bf16_t*)&lo[h], x);
-      load8((const bf16_t*)&hi[h], y);
+      if constexpr (SUMS) {
+        row8<true>(a, t, (h0 + h) * a.hd + d0, x);
+        row8<true>(a, t, (h0 + h) * a.hd + d1, y);
+      } else {
+        load8((const bf16_t*)&lo[h], x);
+        load8((const bf16_t*)&hi[h], y);
+      }
       if (turns && far) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
@@ -230,21 +275,19 @@ static __device__ __forceinline__ void queries(const RopeQ8& a, long long idx) {
 // `lanes` (a power of two, at least hd / (8 N)) neighbouring threads share a token's key and value of one head, N pieces of
 // eight elements each: with N = 2 piece p and piece p + hd / 16, which are each other's partners where the whole head is
 // rotated in halves (half the loads); with N = 1 piece p (a shorter way for a launch of few rows: 8 tokens 5.6 -> 4.5 us).
-template <bool PIECES, int N>
+template <bool PIECES, bool SUMS, int N>
 static __device__ __forceinline__ void key_and_value(const RopeQ8& a, int t, int kvh, int piece, int lanes, int pos, uint2* kb, uint2* vb,
                                                      int* ks, int* vs) {
   float k[N][8], v[N][8];
   uint32_t kt = 0, vt = 0;
   const int d0 = piece * 8, d1 = d0 + a.hd / 2;
   if (d0 < a.hd / N) {
-    const bf16_t* row = a.qkv + (size_t)t * a.ld;
-    const bf16_t* key = row + (size_t)(a.n_heads + kvh) * a.hd;
-    const bf16_t* val = row + (size_t)(a.n_heads + a.n_kv + kvh) * a.hd;
+    const int key = (a.n_heads + kvh) * a.hd, val = (a.n_heads + a.n_kv + kvh) * a.hd;
     if (N == 2 && PIECES && a.cos_t && !a.interleaved && a.rot == a.hd) {
-      load8(key + d0, k[0]);
-      load8(key + d1, k[N - 1]);
-      plain8<PIECES>(val + d0, v[0]);
-      plain8<PIECES>(val + d1, v[N - 1]);
+      row8<SUMS>(a, t, key + d0, k[0]);
+      row8<SUMS>(a, t, key + d1, k[N - 1]);
+      row8<SUMS>(a, t, val + d0, v[0]);
+      row8<SUMS>(a, t, val + d1, v[N - 1]);
       const size_t at = (size_t)(pos < 0 ? 0 : (pos < a.table_rows ? pos : a.table_rows - 1)) * (a.hd / 2) + d0;
       float c[8], s[8];
 #pragma unroll
@@ -261,8 +304,8 @@ static __device__ __forceinline__ void key_and_value(const RopeQ8& a, int t, int
     } else {
 #pragma unroll
       for (int i = 0; i < N; ++i) {
-        rotated8<PIECES>(a, key, pos, i ? d1 : d0, k[i]);
-        plain8<PIECES>(val + (i ? d1 : d0), v[i]);
+        rotated8<PIECES, SUMS>(a, t, key, pos, i ? d1 : d0, k[i]);
+        plain8<PIECES, SUMS>(a, t, val + (i ? d1 : d0), v[i]);
       }
     }
 #pragma unroll
@@ -294,10 +337,10 @@ static __device__ __forceinline__ void key_and_value(const RopeQ8& a, int t, int
 }
 
 // Few rows: no two of them need lie in one page, so a thread stores what it has where it goes (values byte by byte).
-template <bool PIECES>
+template <bool PIECES, bool SUMS>
 __global__ __launch_bounds__(256) void rope_kv_q8_rows_kernel(RopeQ8 a, int kv_blocks, int lanes) {
   if ((int)blockIdx.x >= kv_blocks) {
-    queries<PIECES>(a, (long long)((int)blockIdx.x - kv_blocks) * 256 + threadIdx.x);
+    queries<PIECES, SUMS>(a, (long long)((int)blockIdx.x - kv_blocks) * 256 + threadIdx.x);
     return;
   }
   const long long unit = ((long long)blockIdx.x * 256 + threadIdx.x) / lanes;
@@ -309,7 +352,7 @@ __global__ __launch_bounds__(256) void rope_kv_q8_rows_kernel(RopeQ8 a, int kv_b
   uint2 kb[1], vb[1];
   int ks, vs;
   const long long off = page_of(a, t, pos);
-  key_and_value<PIECES, 1>(a, t, kvh, piece, lanes, pos, kb, vb, &ks, &vs);
+  key_and_value<PIECES, SUMS, 1>(a, t, kvh, piece, lanes, pos, kb, vb, &ks, &vs);
   if (!real || off < 0 || piece * 8 >= a.hd) return;
   uint8_t* head = a.cache + off + (size_t)kvh * q8_head_bytes(a.hd);
   const int in = pos % Q8_PAGE, t16 = in >> 4, i = in & 15, g = i >> 2, r = i & 3;
@@ -327,11 +370,11 @@ __global__ __launch_bounds__(256) void rope_kv_q8_rows_kernel(RopeQ8 a, int kv_b
 // Many rows: a block takes 64 consecutive rows of the step and one kv head, brings keys and values together in LDS, and
 // stores with its lanes in the order of the page: 16 tokens of a keys' piece are 256 bytes in a row, and four tokens of a
 // value's element one word, where four neighbouring rows are neighbouring tokens of a page (elsewhere byte by byte).
-template <bool PIECES>
+template <bool PIECES, bool SUMS>
 __global__ __launch_bounds__(256) void rope_kv_q8_tiles_kernel(RopeQ8 a, int kv_blocks, int lanes) {
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
   if ((int)blockIdx.x >= kv_blocks) {
-    queries<PIECES>(a, (long long)((int)blockIdx.x - kv_blocks) * 256 + threadIdx.x);
+    queries<PIECES, SUMS>(a, (long long)((int)blockIdx.x - kv_blocks) * 256 + threadIdx.x);
     return;
   }
   __shared__ long long at[64];        // each row's page in the cache, -1 where there is none
@@ -364,7 +407,7 @@ __global__ __launch_bounds__(256) void rope_kv_q8_tiles_kernel(RopeQ8 a, int kv_
     const int t = t0 + (j < n ? j : n - 1);
     uint2 kb[2], vb[2];
     int ks, vs;
-    key_and_value<PIECES, 2>(a, t, kvh, piece, lanes, a.positions[t], kb, vb, &ks, &vs);
+    key_and_value<PIECES, SUMS, 2>(a, t, kvh, piece, lanes, a.positions[t], kb, vb, &ks, &vs);
     if (j >= 64 || piece * 16 >= a.hd) continue;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -414,7 +457,8 @@ extern "C" const char* dlgo_rope_kv_q8(const void* qkv, int ld, void* q_out, int
                                        int rot, int interleaved, const float* cos_t, const float* sin_t, int table_rows,
                                        const int32_t* positions, const int32_t* tok_seq, const int32_t* slots, int n_seq,
                                        const int32_t* page_table, int n_slots, int max_pages, void* cache, long long page_stride,
-                                       int n_pages, int write_kv, hipStream_t stream) {
+                                       int n_pages, int write_kv, const float* part, int n_parts, long long plane, int part_ld,
+                                       hipStream_t stream) {
   DLGO_REQUIRE(n_tokens >= 0 && n_heads > 0 && n_kv >= 0 && hd >= 16 && hd % 16 == 0 && hd <= 256,
                "rope_kv_q8: %d rows, %d query and %d kv heads of size %d (head sizes come in steps of 16, up to 256)", n_tokens, n_heads, n_kv, hd);
   DLGO_REQUIRE(rot >= 0 && rot <= hd && rot % 2 == 0, "rope_kv_q8: rotated width %d must be even and at most the head size %d", rot, hd);
@@ -427,9 +471,12 @@ extern "C" const char* dlgo_rope_kv_q8(const void* qkv, int ld, void* q_out, int
                "rope_kv_q8: pages %lld bytes apart (16-byte aligned pages of at least %lld bytes are needed)", page_stride, n_kv * q8_head_bytes(hd));
   if (n_tokens == 0) return nullptr;
   RopeQ8 a = {(const bf16_t*)qkv, (bf16_t*)q_out, (uint8_t*)cache, cos_t, sin_t, positions, tok_seq, slots, page_table,
-              page_stride, ld, ldq, n_tokens, n_heads, n_kv, hd, rot, interleaved, table_rows, n_seq, n_slots, max_pages, n_pages};
-  const bool pieces = rot % (interleaved ? 8 : 16) == 0 && ld % 8 == 0 && ldq % 8 == 0 && ((uintptr_t)qkv & 15) == 0 && ((uintptr_t)q_out & 15) == 0 &&
+              page_stride, ld, ldq, n_tokens, n_heads, n_kv, hd, rot, interleaved, table_rows, n_seq, n_slots, max_pages, n_pages,
+              part, plane, n_parts, part_ld};
+  const bool pieces = rot % (interleaved ? 8 : 16) == 0 && (part || (ld % 8 == 0 && ((uintptr_t)qkv & 15) == 0)) && ldq % 8 == 0 && ((uintptr_t)q_out & 15) == 0 &&
                       (!cos_t || (((uintptr_t)cos_t & 15) == 0 && ((uintptr_t)sin_t & 15) == 0));
+  DLGO_REQUIRE(!part || (pieces && n_parts > 0 && part_ld >= (n_heads + (write_kv ? 2 * n_kv : 0)) * hd && plane >= (long long)n_tokens * part_ld && part_ld % 4 == 0 && plane % 4 == 0 && ((uintptr_t)part & 15) == 0),
+               "rope_kv_q8: unsummed rows need whole 16-byte pieces (rotated width %d, %d runs of rows %d apart)", rot, n_parts, part_ld);
   // The many-rows kernel stores whole lines where the other stores single bytes, but its blocks are long: it is faster from
   // 512 rows of a prompt on (32 heads of 64 over 8: 128 rows 4.9 against 4.8 us, 512 rows 5.1 against 5.6, 1,024 6.0
   // against 7.2, 17,408 rows of 24 heads of 128: 69 us).
@@ -437,17 +484,19 @@ extern "C" const char* dlgo_rope_kv_q8(const void* qkv, int ld, void* q_out, int
   int lanes = 1;
   while (lanes * (tiles ? 16 : 8) < hd) lanes *= 2;
   const long long kv_blocks = !write_kv ? 0 : tiles ? (long long)((n_tokens + 63) / 64) * n_kv : ((long long)n_tokens * n_kv * lanes + 255) / 256;
-  const QueryUnits u = query_units(n_heads, hd, rot, pieces, cos_t != nullptr, interleaved != 0);
+  const QueryUnits u = query_units(part ? 1 : 4, n_heads, hd, rot, pieces, cos_t != nullptr, interleaved != 0);
   const long long q_blocks = ((long long)n_tokens * u.groups * u.per_head + 255) / 256;
   DLGO_REQUIRE(kv_blocks + q_blocks < (1ll << 31), "rope_kv_q8: too many rows at once");
   const dim3 grid((unsigned)(kv_blocks + q_blocks));
   const int lds = 2 * 64 * (hd + 16);
   if (tiles) {
-    if (pieces) hipLaunchKernelGGL(rope_kv_q8_tiles_kernel<true>, grid, dim3(256), lds, stream, a, (int)kv_blocks, lanes);
-    else hipLaunchKernelGGL(rope_kv_q8_tiles_kernel<false>, grid, dim3(256), lds, stream, a, (int)kv_blocks, lanes);
+    if (part) hipLaunchKernelGGL((rope_kv_q8_tiles_kernel<true, true>), grid, dim3(256), lds, stream, a, (int)kv_blocks, lanes);
+    else if (pieces) hipLaunchKernelGGL((rope_kv_q8_tiles_kernel<true, false>), grid, dim3(256), lds, stream, a, (int)kv_blocks, lanes);
+    else hipLaunchKernelGGL((rope_kv_q8_tiles_kernel<false, false>), grid, dim3(256), lds, stream, a, (int)kv_blocks, lanes);
   } else {
-    if (pieces) hipLaunchKernelGGL(rope_kv_q8_rows_kernel<true>, grid, dim3(256), 0, stream, a, (int)kv_blocks, lanes);
-    else hipLaunchKernelGGL(rope_kv_q8_rows_kernel<false>, grid, dim3(256), 0, stream, a, (int)kv_blocks, lanes);
+    if (part) hipLaunchKernelGGL((rope_kv_q8_rows_kernel<true, true>), grid, dim3(256), 0, stream, a, (int)kv_blocks, lanes);
+    else if (pieces) hipLaunchKernelGGL((rope_kv_q8_rows_kernel<true, false>), grid, dim3(256), 0, stream, a, (int)kv_blocks, lanes);
+    else hipLaunchKernelGGL((rope_kv_q8_rows_kernel<false, false>), grid, dim3(256), 0, stream, a, (int)kv_blocks, lanes);
   }
   DLGO_LAUNCH_CHECK("rope_kv_q8");
   return nullptr;

@@ -790,7 +790,8 @@ def _rope_kv_q8_check(qkv, q_out, n_heads, n_kv, head_dim, rot, cos, sin, positi
 def rope_kv_q8(qkv: torch.Tensor, q_out: torch.Tensor, n_heads: int, n_kv: int, head_dim: int, rot: int, interleaved: bool,
                cos: Optional[torch.Tensor], sin: Optional[torch.Tensor], positions: torch.Tensor,
                tok_seq: Optional[torch.Tensor], slots: Optional[torch.Tensor], page_table: Optional[torch.Tensor],
-               cache: Optional[torch.Tensor], page_stride: int, write_kv: bool = True) -> None:
+               cache: Optional[torch.Tensor], page_stride: int, write_kv: bool = True,
+               unsummed: Optional[UnsummedRows] = None) -> None:
     """rope_kv() for the 8-bit cache: the query heads of qkv [T, (H+2KV)*hd] (bfloat16) rotated into q_out [T, H*hd], which
     may be their own place in qkv; the key heads rotated and, with the values, stored in 8 bits in the page of each token
     (cache: uint8, from the first byte of this layer's part of page 0 on; page_stride in bytes).  positions [T], tok_seq
@@ -798,7 +799,8 @@ def rope_kv_q8(qkv: torch.Tensor, q_out: torch.Tensor, n_heads: int, n_kv: int, 
     two (from 2^-126 on) that brings its largest magnitude within 448; each element is rounded once, from float32.  A token whose key
     or value is not finite is marked as a whole, and every row that sees it becomes NaN in that kv head's queries' results.
     Rows whose position has no page (a hole in the table, a page the cache does not hold) store nothing.  Positions must
-    lie inside the rotation tables.  write_kv=False: queries only."""
+    lie inside the rotation tables, and no two rows may be the same token.  write_kv=False: queries only.  unsummed: as in
+    rope_kv() (the sums are not rounded before they are rotated and stored)."""
     # the usual call is told by one look at each tensor; any other goes through the checks that can say what is wrong
     n_pages = max_pages = n_slots = n_seq = 0
     try:
@@ -824,10 +826,15 @@ def rope_kv_q8(qkv: torch.Tensor, q_out: torch.Tensor, n_heads: int, n_kv: int, 
         n_pages = _q8_cache("rope_kv_q8", cache, page_stride, n_kv, head_dim)
     if t == 0:
         return
+    part = (_ptr(None), 0, ctypes.c_longlong(0), 0)
+    if unsummed is not None:
+        if unsummed.rows != t or unsummed.cols < (n_heads + (2 * n_kv if write_kv else 0)) * head_dim or unsummed.scratch.get_device() != qkv.get_device():
+            raise KernelError(f"rope_kv_q8: unsummed rows [{unsummed.rows}, {unsummed.cols}] do not fit {t} rows of qkv")
+        part = (_ptr(unsummed.scratch), unsummed.runs, ctypes.c_longlong(unsummed.rows * unsummed.cols), unsummed.cols)
     _check(_lib("kv_q8").dlgo_rope_kv_q8(_ptr(qkv), _rows(qkv, "rope_kv_q8: qkv rows"), _ptr(q_out), _rows(q_out, "rope_kv_q8: query rows"),
                                          t, n_heads, n_kv, head_dim, rot, int(interleaved), _ptr(cos), _ptr(sin), table_rows,
                                          _ptr(positions), _ptr(tok_seq), _ptr(slots), n_seq, _ptr(page_table), n_slots, max_pages,
-                                         _ptr(cache), ctypes.c_longlong(page_stride), n_pages, int(write_kv), _stream()))
+                                         _ptr(cache), ctypes.c_longlong(page_stride), n_pages, int(write_kv), *part, _stream()))
 
 
 def _attention_q8_check(q, out, n_heads, n_kv, head_dim, cu_q, start_pos, slots, page_table, cache, page_stride, max_q_len, max_kv_len, window):

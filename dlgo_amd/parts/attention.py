@@ -178,7 +178,7 @@ class Attention(Mixer):
             ops.gemm_rmsnorm(self.w_qkv[:cols], xn, norm.weight, norm.eps, qkv[:, :cols])
         else:
             # a product that shares k out over blocks leaves its runs to the rotation kernel, which adds them up as it reads
-            if not fused and not kv.q8 and not self._between and ops.rope_takes_unsummed(ctx.dtype, self.head_dim, rot.width if rot else 0):
+            if not fused and not self._between and ops.rope_takes_unsummed(ctx.dtype, self.head_dim, rot.width if rot else 0):
                 unsummed = ops.gemm_runs(self.w_qkv[:cols], xn, split)
             if unsummed is None:
                 ops.gemm(self.w_qkv[:cols], xn, qkv[:, :cols], scratch=split)
@@ -194,7 +194,7 @@ class Attention(Mixer):
             q = qkv[:, :self.q_dim]
             ops.rope_kv_q8(qkv, q, self.n_heads, self.n_kv_heads, self.head_dim, rot.width if rot else 0, rot.interleaved if rot else False,
                            rot.cos if rot else None, rot.sin if rot else None, ctx.positions, ctx.tok_seq, slots, table, kv.cache,
-                           kv.page_stride, write_kv=owns_cache)
+                           kv.page_stride, write_kv=owns_cache, unsummed=unsummed)
         elif not fused:
             ops.rope_kv(qkv, self.n_heads, n_kv, self.head_dim, rot.width if rot else 0, rot.interleaved if rot else False,
                         rot.cos if rot else None, rot.sin if rot else None, ctx.positions,

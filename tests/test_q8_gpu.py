@@ -243,6 +243,37 @@ def test_store_in_place_and_queries_only(q_lens):
     assert torch.equal(q2, q) and torch.equal(s2.storage, before)
 
 
+@pytest.mark.parametrize("runs", [1, 2, 4, 5, 9])
+@pytest.mark.parametrize("q_lens,hd,rot,inter,write", [([1, 3, 1], 64, 64, False, True), ([90], 48, 32, True, True), ([40, 2], 80, 64, False, True),
+                                                       ([300, 250], 128, 128, False, True), ([7], 256, 256, False, False), ([5], 32, 0, False, True)])
+def test_store_of_rows_that_a_product_left_unsummed(runs, q_lens, hd, rot, inter, write):
+    """Planes whose sum in their order is exactly the row (in any other order it is not): the same bits as from the row."""
+    H, KV = 6, 2
+    s = Step(q_lens, [60] * len(q_lens), H, KV, hd, units=2, unit=1, seed=runs)
+    cos, sin = tables(700, rot) if rot else (None, None)
+    kw = dict(rot=rot, inter=inter, cos=cos, sin=sin, write_kv=write)
+    before = s.storage.clone()
+    q = s.store(**kw)
+    kept = s.storage.clone()
+    s.storage.copy_(before)
+    rows = s.qkv.float()
+    width = rows.shape[1] + 8                                   # columns that are nobody's
+    planes = torch.full((runs, s.rows, width), math.nan, device=DEV)
+    planes[:, :, :rows.shape[1]] = 0.0
+    if runs == 1:
+        planes[0, :, :rows.shape[1]] = rows
+    else:                                                       # 2^30 swallows what is added before it goes again
+        planes[0, :, :rows.shape[1]], planes[runs - 1, :, :rows.shape[1]] = rows / 2, rows / 2
+        if runs >= 4:
+            planes[0, :, :rows.shape[1]], planes[1, :, :rows.shape[1]], planes[2, :, :rows.shape[1]] = 2.0 ** 30, -2.0 ** 30, rows / 2
+    from dlgo_amd.kernels.ops import UnsummedRows
+    s.qkv.fill_(math.nan)
+    assert torch.equal(s.store(unsummed=UnsummedRows(planes.view(-1), runs, s.rows, width), **kw), q)
+    assert torch.equal(s.storage, kept)
+    with pytest.raises(_ops().KernelError, match="unsummed"):
+        s.store(unsummed=UnsummedRows(planes.view(-1), runs, s.rows + 1, width), **kw)
+
+
 @pytest.mark.parametrize("rows", [3, 150, 520])
 def test_store_of_zeros_tiny_huge_and_what_is_not_finite(rows):
     H, KV, hd = 2, 2, 32
