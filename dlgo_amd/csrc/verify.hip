@@ -202,10 +202,10 @@ __global__ __launch_bounds__(THREADS) void verify_rows_kernel(Verify a) {
 #pragma unroll
       for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, WAVE));
       if (m < INFINITY) {
-        // what is -inf or NaN counts 2^-1000 here: nothing beside the maximum's 1
-        const double mc = -(double)m * c;
+        // The difference first: v c - m c in one operation would lose it where T is near zero.  What is -inf or NaN counts
+        // 2^-1000 here: nothing beside the maximum's 1, and more than nothing where a row holds no number.
 #pragma unroll
-        for (int k = 0; k < PER; ++k) s += exp2_neg(fma((double)v[k], c, mc));
+        for (int k = 0; k < PER; ++k) s += exp2_neg(((double)v[k] - (double)m) * c);
       } else {
 #pragma unroll
         for (int k = 0; k < PER; ++k) s += v[k] == m ? 1.0 : 0.0;

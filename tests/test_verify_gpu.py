@@ -109,6 +109,22 @@ def test_verify(k, vocab, model_drafts):
         assert ((probs.double().cpu() - w).abs() <= 2.0 ** -23 * w + 1e-44).all()
 
 
+@pytest.mark.parametrize("model_drafts", [True, False])
+@pytest.mark.parametrize("t", [1e-2, 1e-4, 1e-7, 1e-20, 1e-38, 1e6])
+def test_temperatures_near_zero_and_far_above(t, model_drafts):
+    """Near zero the maximum has all the weight, and equal maxima share it; far above every token has as much."""
+    logits, drafts, k, _, u, ld = case([3, 0, 2], 5000, 11, model_drafts, spread=8.0)
+    t = f32([t] * 3)
+    logits += 25.0                                        # far from zero, where a difference of products would lose it
+    if model_drafts:
+        ld += 25.0
+    logits[:, 17] = logits[:, 4321] = logits.amax(-1) + 0.25
+    got = call(logits.to(DEV), drafts, k, t, u, ld.to(DEV) if model_drafts else None)
+    want = plain(logits.double(), drafts, k, t, u, ld.double() if model_drafts else None)
+    assert got[0] == want[0] and got[1] == want[1]
+    assert torch.allclose(got[2].double().cpu(), torch.tensor(want[2], dtype=torch.float64), rtol=2.0 ** -23, atol=1e-37)
+
+
 def test_rows_further_apart_than_they_are_long_and_not_aligned():
     logits, drafts, k, t, u, ld = case([3, 2, 6], 1003, 5, True)
     want = call(logits.to(DEV), drafts, k, t, u, ld.to(DEV))
