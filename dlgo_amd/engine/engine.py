@@ -119,8 +119,11 @@ class Engine:
         if cache_dtype is not None and self.dtype != torch.bfloat16:
             raise EngineError(f"a cache in {cache_dtype} goes with a bfloat16 run: the float32 path rounds nothing to fewer bits")
         variants = list(model.kernel_variants(self.dtype))
-        for _, part in model.named_parts():
-            variants += [v for v in part.cache_kernel_variants(cache_dtype) if v not in variants]
+        for name, part in model.named_parts():
+            own = part.cache_kernel_variants(cache_dtype)
+            if cache_dtype is not None and not own and any(n.kind == "kv" for n in getattr(part, "cache_needs", list)()):
+                raise EngineError(f"{name}: keys and values in {cache_dtype} are not something this part reads")
+            variants += [v for v in own if v not in variants]
         try:
             self.cache = Cache(model.unit_needs, max_tokens, self.max_ctx, self.dtype, self.device, max_slots,
                                self.max_step_tokens, cache_dtype)
@@ -442,17 +445,20 @@ class Engine:
         self._prompt_seen[shape] = seen
         if len(self._prompt_seen) > 4096:
             self._prompt_seen.clear()
+        # drafts: the recorded launches must cover any later length (and the step before them make their scratch)
+        bound = None if shape[2] else self.cache.max_pages_per_seq
         if seen < 2:
             arrays = self._upload(fields)
-            self._run_piece(StepContext(self, n_seq, n_rows, arrays, host), arrays, sel, out, None)
+            ctx = StepContext(self, n_seq, n_rows, arrays, host)
+            ctx.max_pages_used = bound
+            self._run_piece(ctx, arrays, sel, out, None)
             return out
         total = sum((len(v) + 3) // 4 * 4 for v in fields.values())
         meta = torch.zeros(total, dtype=torch.int32, device=self.device)
         logits = torch.empty((len(sel), self.vocab), dtype=torch.float32, device=self.device)
         arrays = self._upload(fields, dest=meta)
         ctx = StepContext(self, n_seq, n_rows, arrays, host)
-        if not shape[2]:
-            ctx.max_pages_used = self.cache.max_pages_per_seq         # the recorded launches must cover any later length
+        ctx.max_pages_used = bound
         graph = torch.cuda.CUDAGraph()
         torch.cuda.synchronize()
         gc.collect()

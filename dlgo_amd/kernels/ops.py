@@ -871,7 +871,7 @@ def attention_q8(q: torch.Tensor, out: torch.Tensor, n_heads: int, n_kv: int, he
                  page_stride: int, max_q_len: int, max_kv_len: int, window: int = 0, scale: Optional[float] = None,
                  scratch=None) -> torch.Tensor:
     """Attention of a step's (rotated) query rows q [T, H*hd] over the 8-bit cache that rope_kv_q8() writes, which holds
-    the step's own tokens already; out [T, H*hd], both bfloat16.
+    the step's own tokens already; out [T, H*hd], both bfloat16 and apart in memory.
 
     cu_q [n_seq + 1], start_pos [n_seq], slots [n_seq]: int32 on the device.  Sequence i brings rows cu_q[i] to cu_q[i+1]
     (none, one, a few drafted tokens, a prompt), at positions from start_pos[i] on, and its pages are row slots[i] of

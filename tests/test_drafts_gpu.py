@@ -9,6 +9,7 @@ sqrt(1e-2 * 2^-3.5) = 3e-2 in the root mean square, in every layer's values, and
 average over.  So 3e-2 for each layer more.  (2^-8, the rounding of the stored element alone, in place of d gave 3e-2 for
 all layers together; the plain implementation itself, rounded to bfloat16 as above, is off by up to 7.9e-2 for model C.)"""
 import json
+import os
 import subprocess
 import sys
 
@@ -243,7 +244,7 @@ def test_drafts_over_an_8_bit_cache_keep_to_the_margins(folders, plain_q8):
     llm.engine.cache.check_consistent()
 
 
-def test_what_does_not_go_together_is_refused(folders):
+def test_what_does_not_go_together_is_refused(folders, monkeypatch):
     import dlgo_amd
     from dlgo_amd.engine import Engine, EngineError
     from dlgo_amd.sampling import SamplerConfig
@@ -252,6 +253,10 @@ def test_what_does_not_go_together_is_refused(folders):
         Engine.from_folder(folders["A", "float32"], "float32", max_tokens=128, cache_dtype="e4m3")
     with pytest.raises(EngineError, match="e5m2"):
         Engine.from_folder(folders["A", "bfloat16"], "bfloat16", max_tokens=128, cache_dtype="e5m2")
+    from dlgo_amd.parts.attention import Attention
+    with monkeypatch.context() as m, pytest.raises(EngineError, match="self_attn.*not something this part reads"):
+        m.setattr(Attention, "cache_kernel_variants", lambda self, kv_dtype: ())
+        Engine.from_folder(folders["A", "bfloat16"], "bfloat16", max_tokens=128, cache_dtype="e4m3")
     llm = dlgo_amd.load_llm(folders["A", "bfloat16"], dtype="bfloat16", max_tokens=128)
     with pytest.raises(ValueError, match="drafts are verified"):
         llm.generate([1, 2], dlgo_amd.with_lookup_drafts(2))               # the default options cut the distribution
@@ -263,6 +268,19 @@ def test_what_does_not_go_together_is_refused(folders):
                  ([[1], []], [greedy, SamplerConfig()], [[0.5, 0.5], [0.5]])]:
         with pytest.raises(ValueError, match="sampler"):
             s.verify(logits, *args)
+
+
+def test_the_replay_program_takes_an_8_bit_cache(folders, plain_q8, tmp_path):
+    cfg, w = plain.read_model(folders["A", "bfloat16"])
+    (text,) = texts_of(TINY_A, [75], seed=20)
+    steps = [{"step": 0, "entries": [{"id": "x", "tokens": text[:60], "want": [59]}], "end": []},
+             {"step": 1, "entries": [{"id": "x", "tokens": text[60:], "want": list(range(15))}], "end": ["x"]}]
+    p = subprocess.run([os.path.join(ROOT, "bin", "trace_run"), "--model", folders["A", "bfloat16"], "--dtype", "bfloat16", "--cache-dtype", "e4m3",
+                        "--out", str(tmp_path), "--max-tokens", "128"], input="".join(json.dumps(s) + "\n" for s in steps),
+                       capture_output=True, text=True, timeout=100)
+    assert p.returncode == 0, p.stderr
+    got = np.fromfile(tmp_path / "1.f32", dtype="<f4").reshape(15, -1)
+    assert rel_err(torch.from_numpy(got), plain_q8.forward(cfg, w, text)[60:]) <= TOL["A"]
 
 
 def test_the_command_line_takes_both(folders):
