@@ -42,8 +42,9 @@ struct AttnQ8 {
   uint32_t flip;
   int max_q, shared;             // rows of a sequence that are looked at; blocks that take one share of its pages (kv heads * chunks)
   int dealt, least, fill, most;  // how a sequence's pages are dealt to blocks: see Plan
+  int tokens;                    // prompts: tokens of a tile
 };
-enum { WHOLE, EVENLY, BY_LENGTH };
+enum { WHOLE, EVENLY, BY_LENGTH, BY_TILE };
 
 // Waves of a block: four.  Eight leave room for one block a compute unit (a block's own start, its first trips to memory,
 // is then nobody's time to use): 64 sequences of 2,300 tokens 31.1 against 29.3 us, 16 sequences with drafts 21.6 against 18.7.
@@ -62,6 +63,7 @@ __device__ __forceinline__ Span span_of(const AttnQ8& a, int seq) {
   if (s.row0 < 0) s.row0 = 0;
   if (row1 > a.n_rows) row1 = a.n_rows;
   s.rows = row1 - s.row0;
+  if (s.rows > a.max_q) s.rows = a.max_q;
   if (s.start < 0 || s.slot < 0 || s.slot >= a.n_slots) s.rows = 0;
   if (s.rows < 0) s.rows = 0;
   s.len = s.start + s.rows;
@@ -85,6 +87,7 @@ __device__ __forceinline__ int even_shares(const AttnQ8& a, int n) {
 // has round(n / quota) shares, at least one, so that none is longer than one and a half quotas.  The lengths are on the
 // device, so every wave works the shares out from them (a lane a sequence), which costs it 0.7 us.
 #define BLOCKS 768
+#define TILE_PAGES 12            // a tile that sees fewer pages is one block's
 struct Shares {
   int quota;
   __device__ __forceinline__ int of(int pages) const {
@@ -112,6 +115,18 @@ __device__ __forceinline__ Shares shares_of(const AttnQ8& a, const Span& first) 
   Shares s;
   s.quota = quota < (unsigned)a.least ? a.least : (quota > (1u << 30) ? 1 << 30 : (int)quota);
   return s;
+}
+
+// BY_TILE: the pages that a tile of a prompt sees ([lo, hi], nothing if hi < lo), and how many blocks share them.
+__device__ __forceinline__ void tile_pages(const AttnQ8& a, const Span& s, int t0, int t1, int& lo, int& hi) {
+  const int first = a.window > 0 && s.start + t0 - a.window + 1 > 0 ? s.start + t0 - a.window + 1 : 0;
+  lo = first / Q8_PAGE;
+  hi = (s.start + t1 - 1) / Q8_PAGE;
+  if (hi >= a.max_pages) hi = a.max_pages - 1;
+}
+__device__ __forceinline__ int tile_shares(const AttnQ8& a, int pages) {
+  const int n = pages / 4;
+  return pages < TILE_PAGES ? 1 : (n < a.most ? n : a.most);
 }
 
 __device__ __forceinline__ float fast_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
@@ -240,7 +255,7 @@ __global__ __launch_bounds__(WAVES* WAVE) __attribute__((amdgpu_waves_per_eu(EU(
     }
     if (seq < 0) return;                   // fewer shares than there might have been
   }
-  const int cols = (s.rows < a.max_q ? s.rows : a.max_q) * a.group, col0 = chunk * COLS(NC);
+  const int cols = s.rows * a.group, col0 = chunk * COLS(NC);
   if (col0 >= cols) return;
   const int per = (s.n_pages + used - 1) / used;
   const int pg0 = s.first_page + split * per;
@@ -466,8 +481,15 @@ __global__ __launch_bounds__(WAVE) void attn_combine_kernel(AttnQ8 a) {
   const int lane = threadIdx.x, h = blockIdx.x % a.n_heads, r = blockIdx.x / a.n_heads, seq = blockIdx.y;
   const Span s = span_of(a, seq);
   if (r >= s.rows) return;
-  int used, place;                                     // the sequence's shares, and the first one's place
-  if (a.dealt == EVENLY) {
+  int used, place = 0, pages = s.n_pages;              // the sequence's shares, the first one's place, the pages they share
+  if (a.dealt == BY_TILE) {
+    const int t0 = r / a.tokens * a.tokens, t1 = t0 + a.tokens < s.rows ? t0 + a.tokens : s.rows;
+    int lo, hi;
+    tile_pages(a, s, t0, t1, lo, hi);
+    pages = hi - lo + 1;
+    used = tile_shares(a, pages);
+    if (used == 1) return;
+  } else if (a.dealt == EVENLY) {
     used = even_shares(a, s.n_pages);
     place = seq * a.most;
     if (used == 1) return;                             // written by its block
@@ -476,16 +498,15 @@ __global__ __launch_bounds__(WAVE) void attn_combine_kernel(AttnQ8 a) {
     const Shares sh = shares_of(a, mine);
     used = sh.of(s.n_pages);
     if (used == 1) return;
-    place = 0;
     for (int i = lane; i < seq; i += WAVE) place += sh.of(i < WAVE ? mine.n_pages : span_of(a, i).n_pages);
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) place += __shfl_xor(place, o, WAVE);
   }
   const int row = s.row0 + r;
-  const size_t step = (size_t)a.max_q * a.n_heads * PART_ROW;
-  const float* base = a.part + ((size_t)((size_t)place * a.max_q + r) * a.n_heads + h) * PART_ROW;
-  const int per = (s.n_pages + used - 1) / used;
-  const int filled = (s.n_pages + per - 1) / per;      // shares that were given pages
+  const size_t step = a.dealt == BY_TILE ? (size_t)PART_ROW : (size_t)a.max_q * a.n_heads * PART_ROW;
+  const float* base = a.part + (a.dealt == BY_TILE ? ((size_t)row * a.n_heads + h) * a.most : ((size_t)place * a.max_q + r) * a.n_heads + h) * PART_ROW;
+  const int per = (pages + used - 1) / used;
+  const int filled = (pages + per - 1) / per;          // shares that were given pages
   float M = -INFINITY;
   for (int i = lane; i < filled; i += WAVE) M = fmaxf(M, base[i * step + HD]);
   M = wave_max(M);
@@ -540,25 +561,30 @@ __global__ __launch_bounds__(WAVE) void attn_combine_kernel(AttnQ8 a) {
 #define LDS_K (Q8_PAGE * HD * 2)            // [element / 8][token][8 elements]
 #define LDS_V (4 * 2 * DT * 32 * 16)        // [t][h][element][8 tokens: 16 t + 8 a + 4 h + r]
 
-__global__ __launch_bounds__(PF_WAVES* WAVE) __attribute__((amdgpu_waves_per_eu(PF_EU))) void attn_prefill_kernel(AttnQ8 a, int tokens) {
+__global__ __launch_bounds__(PF_WAVES* WAVE) __attribute__((amdgpu_waves_per_eu(PF_EU))) void attn_prefill_kernel(AttnQ8 a) {
   extern __shared__ __attribute__((aligned(16))) char pf_lds[];
   const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   // Late tiles see more keys than early ones: every sequence's tiles are dealt from its last one on, 256 blocks (one a
   // compute unit) at a time, every other time in reverse, so that the blocks that share a unit add up to about the same
   // number of pages and the launch ends with short ones.
-  const int total = gridDim.x, width = a.n_seq * a.n_kv;
-  const int turn = blockIdx.x >> 8, in_turn = total - (turn << 8) < 256 ? total - (turn << 8) : 256;
-  const int place = turn & 1 ? (turn << 8) + in_turn - 1 - (blockIdx.x & 255) : blockIdx.x;
+  const int tokens = a.tokens, total = gridDim.x / a.most, width = a.n_seq * a.n_kv, split = blockIdx.x / total, block = blockIdx.x % total;
+  const int turn = block >> 8, in_turn = total - (turn << 8) < 256 ? total - (turn << 8) : 256;
+  const int place = turn & 1 ? (turn << 8) + in_turn - 1 - (block & 255) : block;
   const int kvh = place % a.n_kv, seq = place % width / a.n_kv;
   const Span s = span_of(a, seq);
   const int tile = (s.rows + tokens - 1) / tokens - 1 - place / width, t0 = tile * tokens;
   if (tile < 0) return;
   const int t1 = t0 + tokens < s.rows ? t0 + tokens : s.rows;        // the block's rows of the sequence
-  const int lo_b = a.window > 0 && s.start + t0 - a.window + 1 > 0 ? s.start + t0 - a.window + 1 : 0;
-  const int pg_lo = lo_b / Q8_PAGE;
-  int pg_hi = (s.start + t1 - 1) / Q8_PAGE;
-  if (pg_hi >= a.max_pages) pg_hi = a.max_pages - 1;
+  int pg_lo, pg_hi;
+  tile_pages(a, s, t0, t1, pg_lo, pg_hi);
+  const int used = tile_shares(a, pg_hi - pg_lo + 1);
+  if (split >= used) return;
+  if (used > 1) {
+    const int per = (pg_hi - pg_lo + used) / used;
+    pg_lo += split * per;
+    if (pg_lo + per - 1 < pg_hi) pg_hi = pg_lo + per - 1;
+  }
 
   // this lane's column: a row of the sequence and a head (one past the last reads the block's first row and counts nothing)
   const int col = wave * 32 + (lane & 31), trow = t0 + col / a.group, hig = col % a.group;
@@ -745,6 +771,21 @@ __global__ __launch_bounds__(PF_WAVES* WAVE) __attribute__((amdgpu_waves_per_eu(
   }
   l += __shfl_xor(l, 32, WAVE);
   if (!mine) return;
+  if (used > 1) {
+    float* to = a.part + (((size_t)(s.row0 + trow) * a.n_heads + kvh * a.group + hig) * a.most + split) * PART_ROW;
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+      for (int qd = 0; qd < 4; ++qd) {
+        const int e = d * 32 + 8 * qd + 4 * half;
+        if (e < HD) *(f32x4_t*)(to + e) = (f32x4_t){o[d][4 * qd], o[d][4 * qd + 1], o[d][4 * qd + 2], o[d][4 * qd + 3]};
+      }
+    if (half == 0) {
+      to[HD] = m;
+      to[HD + 1] = l;
+    }
+    return;
+  }
   const float inv = l == 0.f ? 0.f : 1.0f / l;
   bf16_t* dst = a.out + (size_t)(s.row0 + trow) * a.ldo + (size_t)(kvh * a.group + hig) * HD;
 #pragma unroll
@@ -760,29 +801,44 @@ __global__ __launch_bounds__(PF_WAVES* WAVE) __attribute__((amdgpu_waves_per_eu(
 // What a launch looks like, from sizes that the host knows.  max_q_len and max_kv_len bound the sequences' rows and
 // lengths (a recorded launch passes the context's).
 struct Plan {
-  int tiled, nc, chunks, dealt, least, fill, most;
+  int tiled, nc, chunks, dealt, least, fill, most, tokens;
   long long items;                           // shares of sequences that there may be
 };
 static Plan plan_of(int n_seq, int n_heads, int n_kv, int max_q_len, int max_kv_len, int window) {
   Plan p = {};
   const int group = n_heads / n_kv;
   const long long cols = (long long)max_q_len * group;
-  p.tiled = cols > 64;
-  if (p.tiled) return p;
-  p.nc = cols <= 16 ? 1 : (cols <= 32 ? 2 : 4);
-  if (p.nc > NC_MOST) p.nc = NC_MOST;
-  p.chunks = (int)((cols + 16 * p.nc - 1) / (16 * p.nc));
   int pages = (max_kv_len + Q8_PAGE - 1) / Q8_PAGE;
   if (window > 0) {
     const int seen = (window + max_q_len + Q8_PAGE - 2) / Q8_PAGE + 1;
     if (seen < pages) pages = seen;
   }
+  const int chip = 512;
+  p.tiled = cols > 64;
+  if (p.tiled) {
+    // Few tiles behind a long past (the next turn of a conversation, a piece of a prompt) would each walk all of it alone, a
+    // page in 1.0 us (head size 64) to 1.4 (128): their pages are dealt to as many blocks as fill the chip.  Joining them costs
+    // 5 us and, in full, 36 to 69 MB of partial results, some 8 pages and 16 more, which the dealing has to save.  17 rows
+    // behind 16,384 tokens, 32 heads over 8: 260 -> 27 us and (128) 351 -> 33; 512 rows 266 -> 120, 362 -> 173; four
+    // sequences of 17 rows 266 -> 40, 355 -> 54; 1,024 rows behind 2,048, where it does not: 54 against 65, 74 against 83.
+    p.tokens = PF_WAVES * 32 / group;
+    p.items = (long long)((max_q_len + p.tokens - 1) / p.tokens) * n_seq;
+    const long long blocks = p.items * n_kv;
+    p.most = (int)(chip / blocks < pages / 4 ? chip / blocks : pages / 4);
+    if (p.most < 1) p.most = 1;
+    const int halves = blocks * p.most > chip / 2 ? 3 : 2;       // two blocks a unit take 1.5 times as long a page
+    p.dealt = pages - pages * halves / (2 * p.most) >= 8 + 16 * blocks * p.most / chip ? BY_TILE : WHOLE;
+    if (p.dealt == WHOLE) p.most = 1;
+    return p;
+  }
+  p.nc = cols <= 16 ? 1 : (cols <= 32 ? 2 : 4);
+  if (p.nc > NC_MOST) p.nc = NC_MOST;
+  p.chunks = (int)((cols + 16 * p.nc - 1) / (16 * p.nc));
   // How the pages are dealt (head size 64 and 128, us): with up to a quarter of the chip's blocks evenly, each sequence
   // to as many blocks as any (one sequence of 2,300 tokens 8.4 against 9.9 by length, 16 with drafts 18.1 against 21.3);
   // with more of them by length, where an even deal leaves the longest to too few (32 sequences of 64 to 8,192 tokens 56.9
   // against 63.6); and where the sequences fill the chip each to one block, unless some may be longer than 96 pages.
   const long long blocks = (long long)n_seq * n_kv * p.chunks;
-  const int chip = 512;
   p.items = n_seq;
   if (blocks <= chip / 4) {
     const int by_wave = (pages + WAVES - 1) / WAVES, by_16 = (pages + 16 * WAVES - 1) / (16 * WAVES);
@@ -800,13 +856,17 @@ static Plan plan_of(int n_seq, int n_heads, int n_kv, int max_q_len, int max_kv_
   return p;
 }
 
+static long long scratch_of(const Plan& p, int n_rows, int n_heads, int max_q_len) {
+  return p.dealt == WHOLE ? 0 : (p.tiled ? (long long)n_rows * p.most : p.items * max_q_len) * n_heads * PART_ROW;
+}
+
 extern "C" int dlgo_attention_q8_head_dim() { return HD; }
 
 // floats of scratch that a launch needs (0: none)
 extern "C" long long dlgo_attention_q8_scratch(int n_rows, int n_seq, int n_heads, int n_kv, int max_q_len, int max_kv_len, int window) {
   if (n_rows <= 0 || n_seq <= 0 || n_kv <= 0 || n_heads < n_kv || max_q_len <= 0 || max_kv_len <= 0) return 0;
   const Plan p = plan_of(n_seq, n_heads, n_kv, max_q_len, max_kv_len, window);
-  return p.tiled || !p.dealt ? 0 : p.items * max_q_len * n_heads * PART_ROW;
+  return scratch_of(p, n_rows, n_heads, max_q_len);
 }
 
 template <int NC>
@@ -837,28 +897,25 @@ extern "C" const char* dlgo_attention_q8(const void* q, int ldq, void* out, int 
   const Plan p = plan_of(n_seq, n_heads, n_kv, max_q_len, max_kv_len, window);
   AttnQ8 a = {(const bf16_t*)q, (bf16_t*)out, part, cu_q, start_pos, slots, page_table, (const uint8_t*)cache, page_stride, ldq, ldo, n_rows, n_seq,
               n_heads, n_kv, n_heads / n_kv, n_slots, max_pages, n_pages, window > 0 ? window : 0,
-              (scale < 0 ? -scale : scale) * 1.44269504088896341f, scale < 0 ? 0x80008000u : 0u, max_q_len, n_kv * p.chunks, p.dealt, p.least, p.fill, p.most};
+              (scale < 0 ? -scale : scale) * 1.44269504088896341f, scale < 0 ? 0x80008000u : 0u, max_q_len, n_kv * p.chunks, p.dealt, p.least, p.fill, p.most, p.tokens};
   hipError_t e = hipSuccess;
+  const long long need = scratch_of(p, n_rows, n_heads, max_q_len), blocks = p.items * (p.tiled ? (long long)n_kv * p.most : a.shared);
+  DLGO_REQUIRE(need == 0 || (part && part_elems >= need && ((uintptr_t)part & 15) == 0), "attention_q8: scratch of %lld floats is needed, %lld given", need, part ? part_elems : 0ll);
+  DLGO_REQUIRE(blocks < (1ll << 31), "attention_q8: too many rows at once");
   if (p.tiled) {
-    const int tokens = PF_WAVES * 32 / a.group, n_tiles = (max_q_len + tokens - 1) / tokens;
-    const long long blocks = (long long)n_tiles * n_seq * n_kv;
-    DLGO_REQUIRE(blocks < (1ll << 31), "attention_q8: too many rows at once");
     const int lds = 2 * (LDS_K + LDS_V);
     if (lds > 64 * 1024) e = hipFuncSetAttribute((const void*)attn_prefill_kernel, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
-    if (e == hipSuccess) hipLaunchKernelGGL(attn_prefill_kernel, dim3((unsigned)blocks), dim3(PF_WAVES * WAVE), lds, stream, a, tokens);
+    if (e == hipSuccess) hipLaunchKernelGGL(attn_prefill_kernel, dim3((unsigned)blocks), dim3(PF_WAVES * WAVE), lds, stream, a);
   } else {
-    const long long need = p.dealt ? p.items * max_q_len * n_heads * PART_ROW : 0, blocks = p.items * a.shared;
-    DLGO_REQUIRE(need == 0 || (part && part_elems >= need && ((uintptr_t)part & 15) == 0), "attention_q8: scratch of %lld floats is needed, %lld given", need, part ? part_elems : 0ll);
-    DLGO_REQUIRE(blocks < (1ll << 31), "attention_q8: too many rows at once");
     const dim3 grid((unsigned)blocks);
     e = hipErrorInvalidValue;
     if (p.nc == 1) e = launch_decode<1>(a, grid, stream);
     if constexpr (NC_MOST >= 2) if (p.nc == 2) e = launch_decode<2>(a, grid, stream);
     if constexpr (NC_MOST >= 4) if (p.nc == 4) e = launch_decode<4>(a, grid, stream);
-    if (e == hipSuccess && p.dealt) {
-      DLGO_LAUNCH_CHECK("attention_q8");
-      hipLaunchKernelGGL(attn_combine_kernel, dim3((unsigned)(max_q_len * n_heads), (unsigned)n_seq), dim3(WAVE), 0, stream, a);
-    }
+  }
+  if (e == hipSuccess && p.dealt) {
+    DLGO_LAUNCH_CHECK("attention_q8");
+    hipLaunchKernelGGL(attn_combine_kernel, dim3((unsigned)(max_q_len * n_heads), (unsigned)n_seq), dim3(WAVE), 0, stream, a);
   }
   DLGO_REQUIRE(e == hipSuccess, "attention_q8: %s", hipGetErrorString(e));
   DLGO_LAUNCH_CHECK("attention_q8");

@@ -370,6 +370,22 @@ def test_attention(q_lens, past, H, KV, hd, window):
     assert torch.equal(by_seq[:s.rows], out_wide[:s.rows, :H * hd])
 
 
+@pytest.mark.parametrize("q_lens,past,H,KV,hd,window", [
+    ([17], [3000], 32, 8, 64, 0), ([40, 70], [2000, 5], 8, 2, 128, 0), ([130], [1500], 8, 4, 48, 0), ([90, 1, 0, 20], [900, 1800, 40, 700], 10, 2, 80, 0),
+    ([70], [4000], 6, 3, 32, 1200), ([66], [1100], 2, 2, 256, 0), ([35], [2500], 24, 3, 16, 0), ([33, 33], [1000, 3300], 100, 1, 64, 0)])
+def test_a_few_tiles_behind_a_long_past(q_lens, past, H, KV, hd, window):
+    """A tile's pages dealt to several blocks, evenly and with less for the last; tiles and sequences that are not dealt beside
+    them; launches sized for more rows and for longer sequences."""
+    s = Step(q_lens, past, H, KV, hd, units=2, unit=1, seed=hd)
+    s.fill()
+    q = torch.randn(s.rows, H * hd, generator=s.gen).bfloat16().to(DEV)
+    for kw in (dict(), dict(bound_len=64 * s.table.shape[1] + 900), dict(bound_len=64 * s.table.shape[1], bound_q=min(s.rows, max(q_lens) + 30))):
+        out = s.attend(q, window, **kw)
+        s.check(out, q, window)
+    big = s.attend(q, window, scratch=lambda n: torch.full((n + 8,), math.nan, device=DEV))      # what is in the scratch before
+    assert torch.equal(big, s.attend(q, window))
+
+
 def test_attention_with_a_table_for_far_longer_sequences():
     """Pages of each sequence dealt to many blocks or to one, whatever the launch was sized for."""
     for width, H, KV, hd in ((600, 8, 2, 64), (1500, 4, 1, 128)):
