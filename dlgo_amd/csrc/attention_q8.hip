@@ -11,7 +11,7 @@
 //                        (sequence, kv head) are dealt to the waves of a block, and to several blocks where there are
 //                        too few; the columns of the matrix products are the group's heads of the sequence's rows.
 //   attn_combine_kernel  joins what several blocks left for a row.
-//   attn_prefill_kernel  prompts and pieces of prompts (more than 64 rows * heads of a group): 128 columns a block, pages
+//   attn_prefill_kernel  prompts and pieces of prompts (more than 32 rows * heads of a group): 128 columns a block, pages
 //                        turned to bfloat16 on their way into LDS.
 //
 // computerex/dlgo attends over float32 rows of the cache, one query at a time (models/llm/forward.go:258-278).
@@ -176,7 +176,7 @@ __device__ __forceinline__ uint32_t first_bytes(uint32_t w, int n) { return n >=
 // Measured and not kept: eight waves a block (see WAVES), one page's registers in place of two (the same), 128 registers
 // a lane (spills), 4 or 8 pages a wave at least (slower from 8 sequences on).
 #define COLS(NC) (16 * (NC))
-#define NC_MOST (HD <= 64 ? 4 : (HD <= 128 ? 2 : 1))       // blocks of 16 columns whose sums a wave's registers hold beside two pages
+#define NC_MOST (HD <= 128 ? 2 : 1)                        // blocks of 16 columns whose sums a wave's registers hold beside two pages
 
 struct PageRegs {
   uint4 k[4][KLOADS];
@@ -814,7 +814,11 @@ static Plan plan_of(int n_seq, int n_heads, int n_kv, int max_q_len, int max_kv_
     if (seen < pages) pages = seen;
   }
   const int chip = 512;
-  p.tiled = cols > 64;
+  // Up to 32 columns: with 20 and 32 of them the tiles are slower for heads of 64 (16 sequences with up to 24 columns behind
+  // 128 to 4,089 tokens 28 against 18.5 us) and as fast for 128; with 36 to 64 they are faster from no past to 16,384 tokens
+  // (16 sequences behind 1,024: 22 against 26 to 29, and 29 against 40 to 43), but for 48 and more behind 4,096 (96 against
+  // 86 to 96, 133 against 115).
+  p.tiled = cols > 32;
   if (p.tiled) {
     // Few tiles behind a long past (the next turn of a conversation, a piece of a prompt) would each walk all of it alone, a
     // page in 1.0 us (head size 64) to 1.4 (128): their pages are dealt to as many blocks as fill the chip.  Joining them costs
@@ -831,7 +835,7 @@ static Plan plan_of(int n_seq, int n_heads, int n_kv, int max_q_len, int max_kv_
     if (p.dealt == WHOLE) p.most = 1;
     return p;
   }
-  p.nc = cols <= 16 ? 1 : (cols <= 32 ? 2 : 4);
+  p.nc = cols <= 16 ? 1 : 2;
   if (p.nc > NC_MOST) p.nc = NC_MOST;
   p.chunks = (int)((cols + 16 * p.nc - 1) / (16 * p.nc));
   // How the pages are dealt (head size 64 and 128, us): with up to a quarter of the chip's blocks evenly, each sequence
@@ -911,7 +915,6 @@ extern "C" const char* dlgo_attention_q8(const void* q, int ldq, void* out, int 
     e = hipErrorInvalidValue;
     if (p.nc == 1) e = launch_decode<1>(a, grid, stream);
     if constexpr (NC_MOST >= 2) if (p.nc == 2) e = launch_decode<2>(a, grid, stream);
-    if constexpr (NC_MOST >= 4) if (p.nc == 4) e = launch_decode<4>(a, grid, stream);
   }
   if (e == hipSuccess && p.dealt) {
     DLGO_LAUNCH_CHECK("attention_q8");
