@@ -43,6 +43,9 @@ struct AttnQ8 {
   int max_q, shared;             // rows of a sequence that are looked at; blocks that take one share of its pages (kv heads * chunks)
   int dealt, least, fill, most;  // how a sequence's pages are dealt to blocks: see Plan
   int tokens;                    // prompts: tokens of a tile
+  const float* cos_t;            // FUSED: the rotation's tables
+  const float* sin_t;
+  int table_rows;
 };
 enum { WHOLE, EVENLY, BY_LENGTH, BY_TILE };
 
@@ -210,8 +213,20 @@ static __device__ __forceinline__ void fetch_page(PageRegs& p, const uint8_t* he
 // Waves a SIMD that the registers are to allow: two places for a page, the sums and the queries.
 #define EU(NC) ((NC) == 1 ? (HD <= 64 ? 3 : (HD <= 128 ? 2 : 1)) : ((NC) == 2 && HD <= 64 ? 2 : 1))
 
-template <int NC>
-__global__ __launch_bounds__(WAVES* WAVE) __attribute__((amdgpu_waves_per_eu(EU(NC)))) void attn_decode_kernel(AttnQ8 a) {
+// The key and value of a step's own token, in the lanes in which a page has its places.
+struct NewToken {
+  uint4 k[KLOADS];               // piece 4 j + lane / 16 of the key (the lanes of a piece have the same)
+  uint32_t v[PIECES];            // the byte of element 16 c + lane % 16 of the value
+  uint32_t ks, vs;
+};
+// FUSED: rows of single tokens come unrotated, with their key and value behind the queries.  A wave rotates its own columns'
+// queries, and the one that has the token's page rotates, rounds and stores the key and the value (as kv_q8.hip does, bit
+// for bit) and puts them in their places in its registers; split halves over the whole head.
+#define FUSES (HD % 32 == 0 && HD <= 128)       // (larger ones do not fit the registers)
+#define EU_OF(NC, FUSED) ((FUSED) ? (HD <= 64 ? 2 : 1) : EU(NC))
+
+template <int NC, bool FUSED>
+__global__ __launch_bounds__(WAVES* WAVE) __attribute__((amdgpu_waves_per_eu(EU_OF(NC, FUSED)))) void attn_decode_kernel(AttnQ8 a) {
   constexpr int QK = 2 * KLOADS;                         // matrix instructions for the scores of 16 tokens
   extern __shared__ __attribute__((aligned(16))) float merge[];    // [WAVES][COLS][HD], then [WAVES][COLS] maxima and sums
   const int lane = threadIdx.x & 63, g = lane >> 4, n = lane & 15;
@@ -270,6 +285,8 @@ __global__ __launch_bounds__(WAVES* WAVE) __attribute__((amdgpu_waves_per_eu(EU(
 
   // this lane's column of each of the NC blocks of 16: a row of the step and a head (a column past the last reads the last)
   uint4 qraw[NC][QK];
+  [[maybe_unused]] uint4 partner[FUSED ? QK : 1];
+  [[maybe_unused]] float4 cs[FUSED ? 2 * QK : 1], sn[FUSED ? 2 * QK : 1];
   int pos[NC], lo[NC];
 #pragma unroll
   for (int b = 0; b < NC; ++b) {
@@ -284,9 +301,35 @@ __global__ __launch_bounds__(WAVES* WAVE) __attribute__((amdgpu_waves_per_eu(EU(
 #pragma unroll
       for (int m = 0; m < 2; ++m) {
         const int piece = 4 * j + g;
-        qraw[b][2 * j + m] = *(const uint4*)(src + (piece < PIECES ? piece * 16 + m * 8 : 0));
+        const int d = piece < PIECES ? piece * 16 + m * 8 : 0;
+        qraw[b][2 * j + m] = *(const uint4*)(src + d);
+        if constexpr (FUSED) partner[2 * j + m] = *(const uint4*)(src + (d < HD / 2 ? d + HD / 2 : d - HD / 2));
       }
   }
+  if constexpr (FUSED) {
+    const size_t at = (size_t)(s.start < a.table_rows ? s.start : a.table_rows - 1) * (HD / 2);
+#pragma unroll
+    for (int j = 0; j < QK; ++j) {
+      const int piece = 4 * (j / 2) + g, d = (piece < PIECES ? piece * 16 + (j & 1) * 8 : 0) % (HD / 2);
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        cs[2 * j + e] = *(const float4*)(a.cos_t + at + d + 4 * e);
+        sn[2 * j + e] = *(const float4*)(a.sin_t + at + d + 4 * e);
+      }
+    }
+  }
+  // eight elements of a head's piece (of this lane's j-th eight), rotated
+  auto rotated = [&](int j, const uint4& own, const uint4& other, float* y) {
+    const bool low = (4 * (j / 2) + g) * 16 < HD / 2;
+    const uint32_t w[4] = {own.x, own.y, own.z, own.w}, o[4] = {other.x, other.y, other.z, other.w};
+    const float c[8] = {cs[2 * j].x, cs[2 * j].y, cs[2 * j].z, cs[2 * j].w, cs[2 * j + 1].x, cs[2 * j + 1].y, cs[2 * j + 1].z, cs[2 * j + 1].w};
+    const float sn8[8] = {sn[2 * j].x, sn[2 * j].y, sn[2 * j].z, sn[2 * j].w, sn[2 * j + 1].x, sn[2 * j + 1].y, sn[2 * j + 1].z, sn[2 * j + 1].w};
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float x = __uint_as_float(e & 1 ? w[e / 2] & 0xffff0000u : w[e / 2] << 16), z = __uint_as_float(e & 1 ? o[e / 2] & 0xffff0000u : o[e / 2] << 16);
+      y[e] = low ? rotated_lo(x, z, c[e], sn8[e]) : rotated_hi(z, x, c[e], sn8[e]);
+    }
+  };
   f32x4_t o[NC][PIECES];
   float m[NC], l[NC];
 #pragma unroll
@@ -304,12 +347,105 @@ __global__ __launch_bounds__(WAVES* WAVE) __attribute__((amdgpu_waves_per_eu(EU(
       for (int j = 0; j < QK; ++j) {
         // pieces beyond the head count as zero (the keys' lanes then hold bytes of the next piece, never NaN)
         const bool ok = PIECES % 4 == 0 || 4 * (j / 2) + g < PIECES;
-        const uint4 u = qraw[b][j];
+        uint4 u = qraw[b][j];
+        if constexpr (FUSED) {
+          float y[8];
+          rotated(j, u, partner[j], y);
+          u = make_uint4(Elem<bf16_t>::pair(y[0], y[1]), Elem<bf16_t>::pair(y[2], y[3]), Elem<bf16_t>::pair(y[4], y[5]), Elem<bf16_t>::pair(y[6], y[7]));
+        }
         qf[b][j] = __builtin_bit_cast(bf16x8_t, ok ? make_uint4(u.x ^ a.flip, u.y ^ a.flip, u.z ^ a.flip, u.w ^ a.flip) : make_uint4(0, 0, 0, 0));
       }
   };
 
   const uint8_t* head = a.cache + (size_t)kvh * q8_head_bytes(HD);
+
+  // the token's own page is this wave's last, or another wave's or nobody's
+  [[maybe_unused]] const int own_page = s.start / Q8_PAGE, in = s.start & (Q8_PAGE - 1);
+  [[maybe_unused]] const bool owner = FUSED && turns > 0 && first + (turns - 1) * WAVES == own_page;
+  [[maybe_unused]] NewToken fresh;
+  auto new_token = [&]() {
+    if constexpr (FUSED) {
+      const bf16_t* key = a.q + (size_t)s.row0 * a.ldq + (size_t)(a.n_heads + kvh) * HD;
+      const bf16_t* val = key + (size_t)a.n_kv * HD;
+      uint4 own[QK], other[QK];
+      float v[PIECES];
+#pragma unroll
+      for (int j = 0; j < QK; ++j) {
+        const int piece = 4 * (j / 2) + g, d = piece < PIECES ? piece * 16 + (j & 1) * 8 : 0;
+        own[j] = *(const uint4*)(key + d);
+        other[j] = *(const uint4*)(key + (d < HD / 2 ? d + HD / 2 : d - HD / 2));
+      }
+#pragma unroll
+      for (int c = 0; c < PIECES; ++c) v[c] = bf16_to_f32(val[16 * c + n]);
+      float y[QK][8];
+      uint32_t kt = 0, vt = 0;
+#pragma unroll
+      for (int j = 0; j < QK; ++j) {
+        rotated(j, own[j], other[j], y[j]);
+        const uint32_t top = PIECES % 4 == 0 || 4 * (j / 2) + g < PIECES ? q8_top_bits(y[j]) : 0u;
+        kt = top > kt ? top : kt;
+      }
+#pragma unroll
+      for (int c = 0; c < PIECES; ++c) {
+        const uint32_t top = __float_as_uint(v[c]) & 0x7fffffffu;
+        vt = top > vt ? top : vt;
+      }
+#pragma unroll
+      for (int o = 1; o < WAVE; o <<= 1) {
+        uint32_t& m = o < 16 ? vt : kt;
+        const uint32_t other_m = (uint32_t)__shfl_xor((int)m, o, WAVE);
+        m = other_m > m ? other_m : m;
+      }
+      const bool finite = kt < 0x7f800000u && vt < 0x7f800000u;
+      const int ke = q8_power_for(kt), ve = q8_power_for(vt);
+      const float vf = __uint_as_float((uint32_t)(127 - ve) << 23);
+#pragma unroll
+      for (int j = 0; j < KLOADS; ++j) {
+        const uint2 lo8 = q8_to_e4m3(y[2 * j], ke), hi8 = q8_to_e4m3(y[2 * j + 1], ke);
+        fresh.k[j] = finite ? make_uint4(lo8.x, lo8.y, hi8.x, hi8.y) : make_uint4(0, 0, 0, 0);
+      }
+#pragma unroll
+      for (int c = 0; c < PIECES; ++c) fresh.v[c] = finite ? (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(v[c] * vf, v[c] * vf, 0, false) & 255u : 0u;
+      fresh.ks = finite ? ke + 127 : Q8_NAN;
+      fresh.vs = finite ? ve + 127 : 127;
+    }
+  };
+  // into the page's bytes and into what this wave has of them
+  auto take_in = [&](PageRegs& cur, int id) {
+    if constexpr (FUSED) {
+      const int t16 = in >> 4, i = in & 15, g0 = i >> 2, r8 = 8 * (i & 3);
+      uint8_t* to = (uint8_t*)head + (size_t)id * a.page_stride;
+      auto with = [&](uint32_t w, uint32_t byte, int at) { return (w & ~(255u << at)) | (byte << at); };
+      if (n == i) {
+#pragma unroll
+        for (int j = 0; j < KLOADS; ++j)
+          if (PIECES % 4 == 0 || 4 * j + g < PIECES) *(uint4*)(to + (t16 * PIECES + 4 * j + g) * 256 + 16 * i) = fresh.k[j];
+        if (g == 0) to[2 * Q8_PAGE * HD + 4 * i + t16] = (uint8_t)fresh.ks;
+      }
+      if (g == g0) {
+#pragma unroll
+        for (int c = 0; c < PIECES; ++c) to[Q8_PAGE * HD + ((c * 4 + g0) * 16 + n) * 16 + 4 * t16 + (i & 3)] = (uint8_t)fresh.v[c];
+        if (n == 0) to[2 * Q8_PAGE * HD + 64 + 16 * g0 + 4 * t16 + (i & 3)] = (uint8_t)fresh.vs;
+      }
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int j = 0; j < KLOADS; ++j) {
+          const bool here = t == t16 && n == i;
+          cur.k[t][j] = make_uint4(here ? fresh.k[j].x : cur.k[t][j].x, here ? fresh.k[j].y : cur.k[t][j].y, here ? fresh.k[j].z : cur.k[t][j].z,
+                                   here ? fresh.k[j].w : cur.k[t][j].w);
+        }
+      if (n == i) cur.ks = with(cur.ks, fresh.ks, 8 * t16);
+      if (g == g0) {
+#pragma unroll
+        for (int c = 0; c < PIECES; ++c)
+          cur.v[c] = make_uint4(t16 == 0 ? with(cur.v[c].x, fresh.v[c], r8) : cur.v[c].x, t16 == 1 ? with(cur.v[c].y, fresh.v[c], r8) : cur.v[c].y,
+                                t16 == 2 ? with(cur.v[c].z, fresh.v[c], r8) : cur.v[c].z, t16 == 3 ? with(cur.v[c].w, fresh.v[c], r8) : cur.v[c].w);
+        cur.vs = make_uint4(t16 == 0 ? with(cur.vs.x, fresh.vs, r8) : cur.vs.x, t16 == 1 ? with(cur.vs.y, fresh.vs, r8) : cur.vs.y,
+                            t16 == 2 ? with(cur.vs.z, fresh.vs, r8) : cur.vs.z, t16 == 3 ? with(cur.vs.w, fresh.vs, r8) : cur.vs.w);
+      }
+    }
+  };
 
   auto page = [&](PageRegs& cur, int key0) {
       f32x4_t sc[NC][4];
@@ -415,11 +551,17 @@ __global__ __launch_bounds__(WAVES* WAVE) __attribute__((amdgpu_waves_per_eu(EU(
     if (k0 == 0) {
       __builtin_amdgcn_sched_barrier(0);               // the queries are not waited for before the first page is asked for
       queries();
+      if constexpr (FUSED)
+        if (owner) new_token();
     }
     for (int k = 0; k < here; k += 2) {
       fetch(k + 1, 1);
+      if constexpr (FUSED)
+        if (real[0] && owner && k0 + k == turns - 1) take_in(regs[0], __builtin_amdgcn_readlane(ids, k));
       if (real[0]) page(regs[0], (pg + k * WAVES) * Q8_PAGE);
       fetch(k + 2, 0);
+      if constexpr (FUSED)
+        if (real[1] && owner && k0 + k + 1 == turns - 1) take_in(regs[1], __builtin_amdgcn_readlane(ids, k + 1));
       if (real[1]) page(regs[1], (pg + (k + 1) * WAVES) * Q8_PAGE);
     }
   }
@@ -873,19 +1015,20 @@ extern "C" long long dlgo_attention_q8_scratch(int n_rows, int n_seq, int n_head
   return scratch_of(p, n_rows, n_heads, max_q_len);
 }
 
-template <int NC>
+template <int NC, bool FUSED>
 static hipError_t launch_decode(const AttnQ8& a, dim3 grid, hipStream_t stream) {
   const int lds = WAVES * COLS(NC) * (HD + 2) * 4;       // the waves' results
   hipError_t e = hipSuccess;
-  if (lds > 64 * 1024) e = hipFuncSetAttribute((const void*)attn_decode_kernel<NC>, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
-  if (e == hipSuccess) hipLaunchKernelGGL((attn_decode_kernel<NC>), grid, dim3(WAVES * WAVE), lds, stream, a);
+  if (lds > 64 * 1024) e = hipFuncSetAttribute((const void*)attn_decode_kernel<NC, FUSED>, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+  if (e == hipSuccess) hipLaunchKernelGGL((attn_decode_kernel<NC, FUSED>), grid, dim3(WAVES * WAVE), lds, stream, a);
   return e;
 }
 
 extern "C" const char* dlgo_attention_q8(const void* q, int ldq, void* out, int ldo, int n_rows, int n_seq, int n_heads, int n_kv, int head_dim,
                                          const int32_t* cu_q, const int32_t* start_pos, const int32_t* slots, const int32_t* page_table,
                                          int n_slots, int max_pages, const void* cache, long long page_stride, int n_pages, int max_q_len,
-                                         int max_kv_len, int window, float scale, float* part, long long part_elems, hipStream_t stream) {
+                                         int max_kv_len, int window, float scale, float* part, long long part_elems, const float* cos_t,
+                                         const float* sin_t, int table_rows, hipStream_t stream) {
   DLGO_REQUIRE(head_dim == HD, "attention_q8: this library is built for a head size of %d, not %d", HD, head_dim);
   DLGO_REQUIRE(n_rows >= 0 && n_seq >= 0 && n_kv > 0 && n_heads >= n_kv && n_heads % n_kv == 0, "attention_q8: %d heads over %d kv heads", n_heads, n_kv);
   DLGO_REQUIRE(n_heads / n_kv <= 128, "attention_q8: at most 128 heads share a kv head, not %d", n_heads / n_kv);
@@ -897,11 +1040,14 @@ extern "C" const char* dlgo_attention_q8(const void* q, int ldq, void* out, int 
   DLGO_REQUIRE(((uintptr_t)cache & 15) == 0 && page_stride % 16 == 0 && page_stride >= n_kv * q8_head_bytes(HD),
                "attention_q8: pages %lld bytes apart (16-byte aligned pages of at least %lld bytes are needed)", page_stride, n_kv * q8_head_bytes(HD));
   DLGO_REQUIRE(n_seq <= 65535, "attention_q8: at most 65535 sequences");
+  DLGO_REQUIRE(!cos_t || (FUSES && sin_t && table_rows > 0 && max_q_len == 1 && n_heads / n_kv <= 16 && ldq >= (n_heads + 2 * n_kv) * HD &&
+                          ((uintptr_t)cos_t & 15) == 0 && ((uintptr_t)sin_t & 15) == 0),
+               "attention_q8: rotates single tokens of up to 16 heads a kv head, of sizes in steps of 32 up to 128 (head size %d, %d heads over %d)", HD, n_heads, n_kv);
   if (max_kv_len > max_pages * (long long)Q8_PAGE) max_kv_len = max_pages * Q8_PAGE;
   const Plan p = plan_of(n_seq, n_heads, n_kv, max_q_len, max_kv_len, window);
   AttnQ8 a = {(const bf16_t*)q, (bf16_t*)out, part, cu_q, start_pos, slots, page_table, (const uint8_t*)cache, page_stride, ldq, ldo, n_rows, n_seq,
               n_heads, n_kv, n_heads / n_kv, n_slots, max_pages, n_pages, window > 0 ? window : 0,
-              (scale < 0 ? -scale : scale) * 1.44269504088896341f, scale < 0 ? 0x80008000u : 0u, max_q_len, n_kv * p.chunks, p.dealt, p.least, p.fill, p.most, p.tokens};
+              (scale < 0 ? -scale : scale) * 1.44269504088896341f, scale < 0 ? 0x80008000u : 0u, max_q_len, n_kv * p.chunks, p.dealt, p.least, p.fill, p.most, p.tokens, cos_t, sin_t, table_rows};
   hipError_t e = hipSuccess;
   const long long need = scratch_of(p, n_rows, n_heads, max_q_len), blocks = p.items * (p.tiled ? (long long)n_kv * p.most : a.shared);
   DLGO_REQUIRE(need == 0 || (part && part_elems >= need && ((uintptr_t)part & 15) == 0), "attention_q8: scratch of %lld floats is needed, %lld given", need, part ? part_elems : 0ll);
@@ -913,8 +1059,9 @@ extern "C" const char* dlgo_attention_q8(const void* q, int ldq, void* out, int 
   } else {
     const dim3 grid((unsigned)blocks);
     e = hipErrorInvalidValue;
-    if (p.nc == 1) e = launch_decode<1>(a, grid, stream);
-    if constexpr (NC_MOST >= 2) if (p.nc == 2) e = launch_decode<2>(a, grid, stream);
+    if constexpr (FUSES) if (cos_t) e = launch_decode<1, true>(a, grid, stream);
+    if (p.nc == 1 && !cos_t) e = launch_decode<1, false>(a, grid, stream);
+    if constexpr (NC_MOST >= 2) if (p.nc == 2) e = launch_decode<2, false>(a, grid, stream);
   }
   if (e == hipSuccess && p.dealt) {
     DLGO_LAUNCH_CHECK("attention_q8");

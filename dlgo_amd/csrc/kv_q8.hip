@@ -134,32 +134,6 @@ static __device__ __forceinline__ void plain8(const RopeQ8& a, int t, int col, f
   }
 }
 
-static __device__ __forceinline__ uint32_t top_bits(const float* y) {
-  uint32_t m = 0;
-#pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const uint32_t b = __float_as_uint(y[e]) & 0x7fffffffu;
-    m = b > m ? b : m;
-  }
-  return m;
-}
-
-// the least e with (the float of these bits) <= 448 * 2^e = 1.75 * 2^(8 + e), not below -126
-static __device__ __forceinline__ int power_for(uint32_t top) {
-  const int e = (int)(top >> 23) - 127 - 8 + ((top & 0x7fffffu) > 0x600000u ? 1 : 0);
-  return e < -126 ? -126 : e;
-}
-
-static __device__ __forceinline__ uint2 to_e4m3(const float* y, int power) {
-  const float f = __uint_as_float((uint32_t)(127 - power) << 23);          // 2^-power: power is -126 to 121
-  int lo = 0, hi = 0;
-  lo = __builtin_amdgcn_cvt_pk_fp8_f32(y[0] * f, y[1] * f, lo, false);
-  lo = __builtin_amdgcn_cvt_pk_fp8_f32(y[2] * f, y[3] * f, lo, true);
-  hi = __builtin_amdgcn_cvt_pk_fp8_f32(y[4] * f, y[5] * f, hi, false);
-  hi = __builtin_amdgcn_cvt_pk_fp8_f32(y[6] * f, y[7] * f, hi, true);
-  return make_uint2((uint32_t)lo, (uint32_t)hi);
-}
-
 // Where row t's token lies: its page's offset in the cache (-1 if there is no such page: nothing is written) and its
 // place in the page.
 static __device__ __forceinline__ long long page_of(const RopeQ8& a, int t, int pos) {
@@ -310,7 +284,7 @@ static __device__ __forceinline__ void key_and_value(const RopeQ8& a, int t, int
     }
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const uint32_t k1 = top_bits(k[i]), v1 = top_bits(v[i]);
+      const uint32_t k1 = q8_top_bits(k[i]), v1 = q8_top_bits(v[i]);
       kt = k1 > kt ? k1 : kt;
       vt = v1 > vt ? v1 : vt;
     }
@@ -326,11 +300,11 @@ static __device__ __forceinline__ void key_and_value(const RopeQ8& a, int t, int
     vt = v2 > vt ? v2 : vt;
   }
   const bool finite = kt < 0x7f800000u && vt < 0x7f800000u;
-  const int ke = power_for(kt), ve = power_for(vt);
+  const int ke = q8_power_for(kt), ve = q8_power_for(vt);
 #pragma unroll
   for (int i = 0; i < N; ++i) {
-    kb[i] = finite ? to_e4m3(k[i], ke) : make_uint2(0, 0);
-    vb[i] = finite ? to_e4m3(v[i], ve) : make_uint2(0, 0);
+    kb[i] = finite ? q8_to_e4m3(k[i], ke) : make_uint2(0, 0);
+    vb[i] = finite ? q8_to_e4m3(v[i], ve) : make_uint2(0, 0);
   }
   *ks = finite ? ke + 127 : Q8_NAN;
   *vs = finite ? ve + 127 : 127;

@@ -27,3 +27,30 @@ __host__ __device__ __forceinline__ constexpr long long q8_head_bytes(int hd) { 
 
 // 2^(b - 127) as a float; b = 0 (2^-127) is written by nobody and reads as 0
 __device__ __forceinline__ float q8_scale(uint32_t b) { return __uint_as_float(b << 23); }
+
+// What the writers share.  The largest magnitude of eight elements, as a float's bits.
+__device__ __forceinline__ uint32_t q8_top_bits(const float* y) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const uint32_t b = __float_as_uint(y[e]) & 0x7fffffffu;
+    m = b > m ? b : m;
+  }
+  return m;
+}
+
+// the least e with (the float of these bits) <= 448 * 2^e = 1.75 * 2^(8 + e), not below -126
+__device__ __forceinline__ int q8_power_for(uint32_t top) {
+  const int e = (int)(top >> 23) - 127 - 8 + ((top & 0x7fffffu) > 0x600000u ? 1 : 0);
+  return e < -126 ? -126 : e;
+}
+
+__device__ __forceinline__ uint2 q8_to_e4m3(const float* y, int power) {
+  const float f = __uint_as_float((uint32_t)(127 - power) << 23);          // 2^-power: power is -126 to 121
+  int lo = 0, hi = 0;
+  lo = __builtin_amdgcn_cvt_pk_fp8_f32(y[0] * f, y[1] * f, lo, false);
+  lo = __builtin_amdgcn_cvt_pk_fp8_f32(y[2] * f, y[3] * f, lo, true);
+  hi = __builtin_amdgcn_cvt_pk_fp8_f32(y[4] * f, y[5] * f, hi, false);
+  hi = __builtin_amdgcn_cvt_pk_fp8_f32(y[6] * f, y[7] * f, hi, true);
+  return make_uint2((uint32_t)lo, (uint32_t)hi);
+}

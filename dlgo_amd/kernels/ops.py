@@ -866,10 +866,20 @@ def _attention_q8_scratch(head_dim, rows, n_seq, n_heads, n_kv, max_q_len, max_k
     return lib.dlgo_attention_q8_scratch(rows, n_seq, n_heads, n_kv, max_q_len, max_kv_len, window)
 
 
+def attention_q8_fuses_rotation(head_dim: int, group: int, max_q_len: int, rot_width: int, interleaved: bool, n_seq: int, n_kv: int) -> bool:
+    """True if attention_q8() should rotate the queries and take in the new keys and values itself for such a step: one row a
+    sequence, heads rotated whole, in halves, of sizes in steps of 32 up to 128, up to 16 of them a kv head; and at most one
+    (sequence, kv head) pair for every second compute unit, so that a launch costs more than the rotation repeated in every
+    wave (8 layers of 32 heads over 8 behind 1,024 tokens, ms a step fused and not, head size 64 at 8, 16 and 24 sequences: 0.529
+    and 0.563, 0.567 and 0.601, 0.682 and 0.676; 128: 1.183 and 1.187, 1.272 and 1.278, 1.334 and 1.278)."""
+    return (max_q_len == 1 and head_dim % 32 == 0 and head_dim <= 128 and rot_width == head_dim and not interleaved and group <= 16
+            and 2 * n_seq * n_kv <= compute_units())
+
+
 def attention_q8(q: torch.Tensor, out: torch.Tensor, n_heads: int, n_kv: int, head_dim: int, cu_q: torch.Tensor,
                  start_pos: torch.Tensor, slots: Optional[torch.Tensor], page_table: torch.Tensor, cache: torch.Tensor,
                  page_stride: int, max_q_len: int, max_kv_len: int, window: int = 0, scale: Optional[float] = None,
-                 scratch=None) -> torch.Tensor:
+                 scratch=None, rotation=None) -> torch.Tensor:
     """Attention of a step's (rotated) query rows q [T, H*hd] over the 8-bit cache that rope_kv_q8() writes, which holds
     the step's own tokens already; out [T, H*hd], both bfloat16 and apart in memory.
 
@@ -879,25 +889,38 @@ def attention_q8(q: torch.Tensor, out: torch.Tensor, n_heads: int, n_kv: int, he
     of them.  Rows behind the last sequence's are left as they were.  max_q_len and max_kv_len (host) bound the
     rows a sequence brings and the tokens it holds afterwards: a captured step passes what it allows for; rows and
     tokens beyond the bounds are left out or slow, never out of bounds.  scratch(n) returns a float32 buffer of at least n elements for what
-    several blocks find of a row (allocated here if not given).  A row that finds no page at all is zeros."""
+    several blocks find of a row (allocated here if not given).  A row that finds no page at all is zeros.
+
+    rotation = (cos, sin), where attention_q8_fuses_rotation() says so (one row a sequence): q holds the step's unrotated
+    [q | k | v] rows, the kernel rotates the queries and does what rope_kv_q8() does for the keys and values, to the bit."""
     # as in rope_kv_q8(): one look at each tensor, and the checks that can say what is wrong where that is not enough
     try:
         dev = q.get_device()
         t, width = q.shape
         n_seq = start_pos.numel()
         n_slots, max_pages = page_table.shape
-        plain = (dev >= 0 and dev == _current_device() and n_kv > 0 and n_heads % n_kv == 0 and width == n_heads * head_dim and q.dtype is _BF16
-                 and out.dtype is _BF16 and out.shape == (t, width) and out.get_device() == dev and _is_vector(cu_q, n_seq + 1, dev)
+        plain = (dev >= 0 and dev == _current_device() and n_kv > 0 and n_heads % n_kv == 0 and q.dtype is _BF16
+                 and width == (n_heads if rotation is None else n_heads + 2 * n_kv) * head_dim
+                 and out.dtype is _BF16 and out.shape == (t, n_heads * head_dim) and out.get_device() == dev and _is_vector(cu_q, n_seq + 1, dev)
                  and _is_vector(start_pos, n_seq, dev) and (n_slots >= n_seq if slots is None else _is_vector(slots, n_seq, dev))
                  and _is_vector(page_table, n_slots * max_pages, dev) and cache.get_device() == dev
                  and max_q_len >= 0 and max_kv_len >= 0 and window >= 0)
     except (AttributeError, TypeError, ValueError):
         plain = False
     if not plain:
-        _attention_q8_check(q, out, n_heads, n_kv, head_dim, cu_q, start_pos, slots, page_table, cache, page_stride, max_q_len, max_kv_len, window)
+        _attention_q8_check(q if rotation is None else q[:, :n_heads * head_dim], out, n_heads, n_kv, head_dim, cu_q, start_pos, slots, page_table, cache, page_stride, max_q_len, max_kv_len, window)
         t, n_seq = q.shape[0], start_pos.shape[0]
         n_slots, max_pages = page_table.shape
     n_pages = _q8_cache("attention_q8", cache, page_stride, n_kv, head_dim)
+    cos = sin = None
+    if rotation is not None:
+        cos, sin = rotation
+        if q.shape[1] < (n_heads + 2 * n_kv) * head_dim or max_q_len != 1:
+            raise KernelError(f"attention_q8: rows {tuple(q.shape)} of up to {max_q_len} a sequence are not single tokens' [q | k | v] of {n_heads} and {n_kv} heads of {head_dim}")
+        for what, v in (("cos", cos), ("sin", sin)):
+            _need(v, f"attention_q8: {what} table", torch.float32, 2)
+            if v.shape != cos.shape or v.shape[1] != head_dim // 2 or v.shape[0] < 1 or not v.is_contiguous() or v.get_device() != q.get_device():
+                raise KernelError(f"attention_q8: {what} table {tuple(v.shape)} does not rotate heads of {head_dim}")
     if scale is None:
         scale = 1.0 / math.sqrt(head_dim)
     if t == 0 or n_seq == 0 or max_q_len == 0:
@@ -914,7 +937,8 @@ def attention_q8(q: torch.Tensor, out: torch.Tensor, n_heads: int, n_kv: int, he
                                  n_heads, n_kv, head_dim, _ptr(cu_q), _ptr(start_pos), _ptr(slots), _ptr(page_table),
                                  n_slots, max_pages, _ptr(cache), ctypes.c_longlong(page_stride), n_pages,
                                  max_q_len, max_kv_len, int(window), ctypes.c_float(scale), _ptr(part),
-                                 ctypes.c_longlong(part.numel() if part is not None else 0), _stream()))
+                                 ctypes.c_longlong(part.numel() if part is not None else 0), _ptr(cos), _ptr(sin),
+                                 0 if cos is None else cos.shape[0], _stream()))
     return out
 
 

@@ -20,8 +20,8 @@ without them launches nothing for them; a layer with them takes the separate
 rotation kernel, since the fused ones read the product's result as it is.
 
 Over a cache of 8-bit keys and values (KVView.q8) the rotation kernel stores them
-so, and attention reads them: one pair of kernels for every step, whatever the
-number of rows a sequence brings.
+so, and attention reads them; for a few single tokens it rotates and stores by itself,
+as the other one does.
 """
 from __future__ import annotations
 
@@ -169,8 +169,12 @@ class Attention(Mixer):
         kv = ctx.cache.kv_view(unit)
         rot = self.position.rotation()
         # a step of single tokens: the attention kernel rotates and stores by itself; else a kernel of its own does
-        fused = not kv.q8 and not self._between and ops.attention_fuses_rotation(ctx.dtype, self.head_dim, self.n_heads // self.n_kv_heads,
-                                                                   ctx.max_q_len, rot.width if rot else 0, ctx.n_seq, self.n_kv_heads)
+        group, width = self.n_heads // self.n_kv_heads, rot.width if rot else 0
+        if kv.q8:
+            fused = (owns_cache and rot is not None and not self._between
+                     and ops.attention_q8_fuses_rotation(self.head_dim, group, ctx.max_q_len, width, rot.interleaved, ctx.n_seq, self.n_kv_heads))
+        else:
+            fused = not self._between and ops.attention_fuses_rotation(ctx.dtype, self.head_dim, group, ctx.max_q_len, width, ctx.n_seq, self.n_kv_heads)
         unsummed = None
         if isinstance(xn, ops.UnscaledNorm):   # the norm's factor is applied to the product's sums
             ops.gemm_scaled(self.w_qkv[:cols], xn, qkv[:, :cols])
@@ -188,7 +192,7 @@ class Attention(Mixer):
             ops.head_rmsnorm(qkv, 0, self.n_heads, self.head_dim, self.q_norm, self.qk_norm_eps)
             if n_kv:
                 ops.head_rmsnorm(qkv, self.q_dim, n_kv, self.head_dim, self.k_norm, self.qk_norm_eps)
-        if kv.q8:
+        if kv.q8 and not fused:
             pages = self._seq_pages(ctx, kv)
             table, slots = (kv.page_table, ctx.slots) if pages is None else (pages, ctx.tok_seq)      # row i is sequence i's
             q = qkv[:, :self.q_dim]
@@ -202,7 +206,7 @@ class Attention(Mixer):
                         unsummed=unsummed, single_tokens=ctx.max_q_len == 1,
                         seq_pages=getattr(ctx, "seq_pages", {}).get(kv.group) if ctx.max_q_len == 1 else None)
         out = ctx.buffer("attention.out", (t, self.q_dim), ctx.dtype)
-        self.attend(qkv[:, :self.q_dim] if kv.q8 else qkv, out, ctx, kv,
+        self.attend(qkv[:, :self.q_dim] if kv.q8 and not fused else qkv, out, ctx, kv,
                     rotation=(rot.cos, rot.sin, rot.width, rot.interleaved) if fused and rot else None, new_kv=fused and owns_cache)
         if self.out_bias:        # the bias goes into the residual after the product: no norm of it can be left on the way
             ops.gemm(self.w_o, out, residual, ops.EPI_ACCUM_F32, scratch=split)
@@ -239,7 +243,8 @@ class Attention(Mixer):
             bound = ctx.max_kv_len if ctx.max_pages_used is None else ctx.max_pages_used * ops.PAGE
             ops.attention_q8(q, out, self.n_heads, self.n_kv_heads, self.head_dim, ctx.cu_q, ctx.start_pos, slots, table, kv.cache,
                              kv.page_stride, ctx.max_q_len, bound, window=self.window or 0, scale=self.scale,
-                             scratch=lambda n: ctx.scratch("attention.partials", n, torch.float32))
+                             scratch=lambda n: ctx.scratch("attention.partials", n, torch.float32),
+                             rotation=rotation[:2] if rotation else None)
             return
         ops.attention(q, out, self.n_heads, self.n_kv_heads, self.head_dim, ctx.positions, ctx.tok_seq, ctx.slots,
                       kv.page_table, kv.cache, kv.page_stride, kv.v_off, ctx.host["q_lens"], ctx.host["start_pos"],

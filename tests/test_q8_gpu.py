@@ -597,3 +597,58 @@ def test_refusals():
     attend(q=q[:0], out=q[:0])
     attend(cu=i32([0]), start=i32([]), slots=i32([]))
     attend(mq=0)
+
+
+FUSED = [   # past, H, KV, hd, window: single tokens
+    ([0], 4, 2, 32, 0), ([5, 63, 64, 700], 32, 8, 64, 0), ([127, 2300], 8, 1, 96, 0), ([1, 15, 16, 17, 31, 48, 130], 6, 3, 128, 0),
+    ([400, 3], 16, 1, 64, 0), ([500, 64], 8, 4, 32, 0), ([1000, 10, 4095], 8, 2, 64, 70), ([90] * 40, 4, 2, 64, 0), ([64 * i for i in range(20)], 16, 8, 128, 0),
+    ([20000], 8, 2, 32, 0),
+]
+
+
+@pytest.mark.parametrize("past,H,KV,hd,window", FUSED)
+def test_single_tokens_rotated_and_stored_on_the_way(past, H, KV, hd, window):
+    """The same bits, in the cache and in the result, as from the two kernels; a token whose page is missing, one that is not
+    finite and what lies around them as there."""
+    ops = _ops()
+    n = len(past)
+    assert ops.attention_q8_fuses_rotation(hd, H // KV, 1, hd, False, n, KV) == (2 * n * KV <= ops.compute_units())
+    s = Step([1] * n, past, H, KV, hd, units=2, unit=1, seed=hd, pad_cols=8)
+    s.fill()
+    cos, sin = tables(max(past) + 1, hd)
+    if n > 3:
+        s.qkv[1, H * hd + 3] = math.inf                         # a key, and another token's value
+        s.qkv[2, -1] = math.nan
+        s.table[s.slots[3], past[3] // PAGE] = -1               # nowhere to store it
+    before = s.storage.clone()
+    q = s.store(cos=cos, sin=sin)
+    for bound in (None, 64 * s.table.shape[1] + 3000):
+        want = s.attend(q, window, bound_len=bound)
+        kept = s.storage.clone()
+        s.storage.copy_(before)
+        out = torch.full_like(want, 7.0)
+        got = s.attend(s.qkv, window, out=out, bound_len=bound, rotation=(cos, sin))
+        assert torch.equal(s.storage, kept)
+        assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got.nan_to_num(), want.nan_to_num())
+    if n > 3:
+        rows = want.view(n, KV, -1).isnan().all(-1).cpu()
+        assert rows[1, 0] and not rows[1, 1:].any() and rows[2, KV - 1] and not rows[2, :KV - 1].any() and not rows[0].any()
+
+
+def test_refusals_of_rows_to_be_rotated():
+    ops = _ops()
+    s = Step([1, 1], [3, 70], 4, 2, 64)
+    cos, sin = tables(100, 64)
+    s.attend(s.qkv, out=torch.empty(2, 256, dtype=torch.bfloat16, device=DEV), rotation=(cos, sin))
+    for kw in (dict(rotation=(cos, sin), bound_q=2), dict(rotation=(cos[:, :16], sin[:, :16])), dict(rotation=(cos, sin[:50])), dict(rotation=(cos.double(), sin)),
+               dict(rotation=(cos.cpu(), sin.cpu()))):
+        with pytest.raises(ops.KernelError):
+            s.attend(s.qkv, out=torch.empty(2, 256, dtype=torch.bfloat16, device=DEV), **kw)
+    with pytest.raises(ops.KernelError, match="single tokens"):
+        s.attend(s.qkv[:, :256], out=torch.empty(2, 256, dtype=torch.bfloat16, device=DEV), rotation=(cos, sin))
+    odd = Step([1], [3], 4, 2, 48)
+    with pytest.raises(ops.KernelError, match="steps of 32"):
+        odd.attend(odd.qkv, out=torch.empty(1, 192, dtype=torch.bfloat16, device=DEV), rotation=tables(100, 48))
+    many = Step([1], [3], 34, 2, 64)
+    with pytest.raises(ops.KernelError, match="up to 16 heads"):
+        many.attend(many.qkv, out=torch.empty(1, 34 * 64, dtype=torch.bfloat16, device=DEV), rotation=(cos, sin))
