@@ -600,7 +600,7 @@ def test_refusals():
 
 
 FUSED = [   # past, H, KV, hd, window: single tokens
-    ([0], 4, 2, 32, 0), ([5, 63, 64, 700], 32, 8, 64, 0), ([127, 2300], 8, 1, 96, 0), ([1, 15, 16, 17, 31, 48, 130], 6, 3, 128, 0),
+    ([0], 4, 2, 32, 0), ([5, 63, 64, 700], 32, 8, 64, 0), ([127, 2300], 8, 1, 32, 0), ([1, 15, 16, 17, 31, 48, 130], 6, 3, 128, 0),
     ([400, 3], 16, 1, 64, 0), ([500, 64], 8, 4, 32, 0), ([1000, 10, 4095], 8, 2, 64, 70), ([90] * 40, 4, 2, 64, 0), ([64 * i for i in range(20)], 16, 8, 128, 0),
     ([20000], 8, 2, 32, 0),
 ]
