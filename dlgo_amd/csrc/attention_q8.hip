@@ -695,7 +695,8 @@ __global__ __launch_bounds__(WAVE) void attn_combine_kernel(AttnQ8 a) {
 // sums rescaled only where a maximum has grown and maxima exchanged without LDS: 349; pages two ahead: 319 to 334, 660
 // TFLOP/s.  A lone prompt of 2,048 tokens (heads of 64, 38.8 us) waits for its last tiles, 32 pages of 1.1 us one after the
 // other.  Measured and not kept: 64 columns a wave (78 us), eight waves with 256 columns (50 to 59), two teams of waves on
-// alternate pages (45), the scores of the next page beside this one's softmax (-3% for heads of 64, spills for 128).
+// alternate pages (45), the scores of the next page beside this one's softmax (-3% for heads of 64, spills for 128), wave
+// priorities raised around the products or the softmax (337 to 360 against 336).
 #define PF_WAVES 4
 #define PF_EU (HD <= 128 ? 2 : 1)           // waves a SIMD that the registers are to allow
 #define DT ((HD + 31) / 32)                 // tiles of 32 elements of the result

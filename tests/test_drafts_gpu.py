@@ -134,6 +134,58 @@ def test_a_rewound_sequence_goes_on_as_if_nothing_had_been_there(folders, monkey
         eng.rewind(a, 0)
 
 
+@pytest.mark.parametrize("seed", [0, 1])
+def test_random_traffic_over_an_8_bit_cache(folders, plain_q8, seed):
+    """Sequences opened, closed and copied; prompts, pieces, single tokens and drafts that are taken back in part, several
+    sequences a step: every logit that is asked for is the plain implementation's for that text."""
+    from dlgo_amd.engine import Engine, Entry
+    rng = np.random.default_rng(seed)
+    name = "AB"[seed]
+    raw = CONFIGS[name][0]
+    eng = Engine.from_folder(folders[name, "bfloat16"], "bfloat16", max_tokens=640, max_ctx=128, max_slots=5, max_step_tokens=48, cache_dtype="e4m3")
+    cfg, w = plain.read_model(folders[name, "bfloat16"])
+    token = lambda n: rng.integers(0, raw["vocab_size"], size=n).tolist()        # noqa: E731
+    texts, checked = {}, 0
+
+    def check(slot, rows, got):
+        nonlocal checked
+        assert rel_err(got, plain_q8.forward(cfg, w, texts[slot], rows=rows)) <= TOL[name]
+        checked += len(rows)
+    for turn in range(90):
+        kind = rng.choice(["open", "step", "step", "decode", "decode", "drafts", "drafts", "fork", "close"])
+        live = [s for s in texts if len(texts[s]) < 100]
+        if kind == "open" and eng.free_slots() and eng.free_pages()[0] >= 3:
+            texts[eng.open(1)[0]] = []
+        elif kind == "close" and texts:
+            s = rng.choice(list(texts))
+            eng.close([int(s)])
+            del texts[s]
+        elif kind == "fork" and live and eng.free_slots() and eng.free_pages()[0] >= 3:
+            s = int(rng.choice(live))
+            texts[eng.fork(s)] = list(texts[s])
+        elif kind in ("step", "decode", "drafts") and live:
+            mates = [int(s) for s in rng.permutation(live)[:rng.integers(1, 4)]]
+            if kind == "decode":
+                mates = [s for s in mates if texts[s]] or mates[:1]
+                new = [token(1) for _ in mates]
+                out = eng.decode(mates, [t[0] for t in new])
+                for s, t, x in zip(mates, new, out.clone()):
+                    texts[s] += t
+                    check(s, [len(texts[s]) - 1], x[None])
+                continue
+            n = int(rng.integers(2, 7))
+            new = [token(n if kind == "drafts" else int(rng.integers(1, 25))) for _ in mates]
+            out = eng.step([Entry(s, t, range(len(t)), undecided=n - 1 if kind == "drafts" else 0) for s, t in zip(mates, new)])
+            for s, t, x in zip(mates, new, torch.split(out, [len(t) for t in new])):
+                texts[s] += t
+                check(s, list(range(len(texts[s]) - len(t), len(texts[s]))), x)
+                if kind == "drafts":
+                    texts[s] = texts[s][:len(texts[s]) - int(rng.integers(0, n))]
+                    eng.rewind(s, len(texts[s]))
+        eng.cache.check_consistent()
+    assert checked > 200
+
+
 @pytest.mark.parametrize("dtype,cache_dtype", [("bfloat16", "e4m3"), ("bfloat16", None), ("float32", None)])
 def test_steps_of_drafts_are_recorded(folders, dtype, cache_dtype):
     """A shape's third step and those after it are replayed, at lengths that had not been reached when it was recorded, with
