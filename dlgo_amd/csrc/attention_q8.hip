@@ -41,13 +41,13 @@ struct AttnQ8 {
   float scale_log2e;             // not negative; `flip` is its sign
   uint32_t flip;
   int max_q, shared;             // rows of a sequence that are looked at; blocks that take one share of its pages (kv heads * chunks)
-  int dealt, least, fill, most;  // how a sequence's pages are dealt to blocks: see Plan
+  int dealt, fill, most;         // how a sequence's pages are dealt to blocks: see Plan
   int tokens;                    // prompts: tokens of a tile
   const float* cos_t;            // FUSED: the rotation's tables
   const float* sin_t;
   int table_rows;
 };
-enum { WHOLE, EVENLY, BY_LENGTH, BY_TILE };
+enum { WHOLE, EVENLY, BY_TILE };
 
 // Waves of a block: four.  Eight leave room for one block a compute unit (a block's own start, its first trips to memory,
 // is then nobody's time to use): 64 sequences of 2,300 tokens 31.1 against 29.3 us, 16 sequences with drafts 21.6 against 18.7.
@@ -78,48 +78,16 @@ __device__ __forceinline__ Span span_of(const AttnQ8& a, int seq) {
   return s;
 }
 
-// EVENLY: shares of a sequence with n pages: enough to fill the chip, but not more than leave each wave a page, and so many
-// that a wave has at most 16 pages.
+// EVENLY: the blocks that share a sequence of n pages: enough to fill the chip, but not more than leave each wave a page, and
+// so many that a wave has at most 16 pages.
 __device__ __forceinline__ int even_shares(const AttnQ8& a, int n) {
   const int by_wave = (n + WAVES - 1) / WAVES, by_16 = (n + 16 * WAVES - 1) / (16 * WAVES);
   int s = a.fill < by_wave ? a.fill : by_wave;
+  if (n < 16) s = 1;
   if (s < by_16) s = by_16;
   return s < 1 ? 1 : (s > a.most ? a.most : s);
 }
-// BY_LENGTH: sequences are dealt out in shares of about the same number of pages, about BLOCKS blocks in all: one of n pages
-// has round(n / quota) shares, at least one, so that none is longer than one and a half quotas.  The lengths are on the
-// device, so every wave works the shares out from them (a lane a sequence), which costs it 0.7 us.
-#define BLOCKS 768
 #define TILE_PAGES 12            // a tile that sees fewer pages is one block's
-struct Shares {
-  int quota;
-  __device__ __forceinline__ int of(int pages) const {
-    const int n = (pages + (quota >> 1)) / quota;
-    return n < 1 ? 1 : n;
-  }
-};
-__device__ __forceinline__ int wave_running(int v) {
-  const int lane = threadIdx.x & 63;
-#pragma unroll
-  for (int o = 1; o < WAVE; o <<= 1) {
-    const int u = __shfl_up(v, o, WAVE);
-    if (lane >= o) v += u;
-  }
-  return v;
-}
-// `first`: what the lane's sequence (its number modulo 64) is among the first 64
-__device__ __forceinline__ Shares shares_of(const AttnQ8& a, const Span& first) {
-  const int lane = threadIdx.x & 63;
-  unsigned long long sum = lane < a.n_seq ? first.n_pages : 0;
-  for (int i = WAVE + lane; i < a.n_seq; i += WAVE) sum += span_of(a, i).n_pages;
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, WAVE);
-  const unsigned long long quota = (sum * a.shared + BLOCKS - 1) / BLOCKS;
-  Shares s;
-  s.quota = quota < (unsigned)a.least ? a.least : (quota > (1u << 30) ? 1 << 30 : (int)quota);
-  return s;
-}
-
 // BY_TILE: the pages that a tile of a prompt sees ([lo, hi], nothing if hi < lo), and how many blocks share them.
 __device__ __forceinline__ void tile_pages(const AttnQ8& a, const Span& s, int t0, int t1, int& lo, int& hi) {
   const int first = a.window > 0 && s.start + t0 - a.window + 1 > 0 ? s.start + t0 - a.window + 1 : 0;
@@ -164,7 +132,7 @@ __device__ __forceinline__ bf16x8_t eight(uint32_t w0, uint32_t w1, float scale)
 __device__ __forceinline__ uint32_t first_bytes(uint32_t w, int n) { return n >= 4 ? w : (n <= 0 ? 0u : w & ((1u << (8 * n)) - 1u)); }
 
 // ---------------------------------------------------------------------------------------------------------------------
-// Few rows a sequence.  grid: shares * chunks of columns * kv heads, WAVES waves.  A wave holds a whole page of
+// Few rows a sequence.  grid: shares * sequences * chunks of columns * kv heads, WAVES waves.  A wave holds a whole page of
 // its head in registers: the keys of 16 tokens are KLOADS loads of 16 bytes a lane, the values of 16 elements one, all
 // of them consecutive in memory, and each is an operand of the matrix instructions as it lies once its bytes are
 // converted.  The next page's loads are on their way while this one is multiplied.  The scores come out with a lane
@@ -172,12 +140,13 @@ __device__ __forceinline__ uint32_t first_bytes(uint32_t w, int n) { return n >=
 // another but the two exchanges of the maximum.
 //
 // Bound by memory where there is much of it: 64 sequences of 2,048 to 2,303 tokens, 32 heads of 64 over 8: 145 MB in 28.7 us,
-// 5.1 TB/s, what a large copy reaches on this chip; 32 sequences of 64 to 8,192 tokens, heads of 128: 273 MB in 53 us and 5
-// for the join, 4.7 TB/s.  By latency where there is little: a block needs three trips to memory before its first product
+// 5.1 TB/s, what a large copy reaches on this chip; 32 sequences of 64 to 8,192 tokens, heads of 128: 273 MB in 58 us, 4.7
+// TB/s.  By latency where there is little: a block needs three trips to memory before its first product
 // (the sequence's numbers, its page numbers, the page) and hands its result over, 5 us in all: one sequence of 2,300
 // tokens takes 5.2 us and 4 for the join; 16 with up to six drafted tokens each (35 MB) 14.7 and 4.
 // Measured and not kept: eight waves a block (see WAVES), one page's registers in place of two (the same), 128 registers
-// a lane (spills), 4 or 8 pages a wave at least (slower from 8 sequences on).
+// a lane (spills), 4 or 8 pages a wave at least (slower from 8 sequences on), shares of about equal length worked out by
+// every wave from the lengths on the device (0.7 us a kernel, and up to twice the time where the lengths are equal).
 #define COLS(NC) (16 * (NC))
 #define NC_MOST (HD <= 128 ? 2 : 1)                        // blocks of 16 columns whose sums a wave's registers hold beside two pages
 
@@ -232,44 +201,10 @@ __global__ __launch_bounds__(WAVES* WAVE) __attribute__((amdgpu_waves_per_eu(EU_
   const int lane = threadIdx.x & 63, g = lane >> 4, n = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);        // known to be the same in all lanes, as all that follows from it
   const int in_share = blockIdx.x % a.shared, kvh = in_share % a.n_kv, chunk = in_share / a.n_kv, item = blockIdx.x / a.shared;
-  Span s;
-  int split = 0, used = 1, place = item;               // the share's place among the partial results
-  if (a.dealt != BY_LENGTH) {
-    const int seq = item % a.n_seq;                     // WHOLE: item is below n_seq
-    s = span_of(a, seq);
-    if (a.dealt == EVENLY) {
-      used = even_shares(a, s.n_pages);
-      split = item / a.n_seq;
-      if (split >= used) return;
-      place = seq * a.most + split;
-    }
-  } else {
-    Span mine = span_of(a, lane < a.n_seq ? lane : a.n_seq - 1);
-    const Shares sh = shares_of(a, mine);
-    int before = 0, seq = -1;
-    for (int i0 = 0; i0 < a.n_seq; i0 += WAVE) {
-      const int i = i0 + lane;
-      if (i0 > 0) mine = span_of(a, i < a.n_seq ? i : a.n_seq - 1);
-      const int n = i < a.n_seq ? sh.of(mine.n_pages) : 0, upto = before + wave_running(n);
-      const unsigned long long past = __ballot(upto > item);
-      if (past) {
-        const int at = __builtin_ctzll(past);
-        seq = i0 + at;
-        used = __builtin_amdgcn_readlane(n, at);
-        split = item - (__builtin_amdgcn_readlane(upto, at) - used);
-        s.row0 = __builtin_amdgcn_readlane(mine.row0, at);
-        s.rows = __builtin_amdgcn_readlane(mine.rows, at);
-        s.start = __builtin_amdgcn_readlane(mine.start, at);
-        s.len = __builtin_amdgcn_readlane(mine.len, at);
-        s.slot = __builtin_amdgcn_readlane(mine.slot, at);
-        s.first_page = __builtin_amdgcn_readlane(mine.first_page, at);
-        s.n_pages = __builtin_amdgcn_readlane(mine.n_pages, at);
-        break;
-      }
-      before = __builtin_amdgcn_readlane(upto, WAVE - 1);
-    }
-    if (seq < 0) return;                   // fewer shares than there might have been
-  }
+  const int seq = item % a.n_seq, split = item / a.n_seq;
+  const Span s = span_of(a, seq);
+  const int used = a.dealt == EVENLY ? even_shares(a, s.n_pages) : 1;
+  if (split >= used) return;
   const int cols = s.rows * a.group, col0 = chunk * COLS(NC);
   if (col0 >= cols) return;
   const int per = (s.n_pages + used - 1) / used;
@@ -607,7 +542,7 @@ __global__ __launch_bounds__(WAVES* WAVE) __attribute__((amdgpu_waves_per_eu(EU_
       const float inv = L == 0.f ? 0.f : 1.0f / L;       // a row that sees no token at all (its pages are missing): zeros
       Elem<bf16_t>::store4(a.out + (size_t)row * a.ldo + (size_t)h * HD + e4 * 4, acc[0] * inv, acc[1] * inv, acc[2] * inv, acc[3] * inv);
     } else {
-      float* dst = a.part + ((size_t)((size_t)place * a.max_q + row - s.row0) * a.n_heads + h) * PART_ROW;
+      float* dst = a.part + (((size_t)row * a.n_heads + h) * a.most + split) * PART_ROW;
       *(f32x4_t*)(dst + e4 * 4) = acc;
       if (e4 == 0) {
         dst[HD] = M;
@@ -623,34 +558,23 @@ __global__ __launch_bounds__(WAVE) void attn_combine_kernel(AttnQ8 a) {
   const int lane = threadIdx.x, h = blockIdx.x % a.n_heads, r = blockIdx.x / a.n_heads, seq = blockIdx.y;
   const Span s = span_of(a, seq);
   if (r >= s.rows) return;
-  int used, place = 0, pages = s.n_pages;              // the sequence's shares, the first one's place, the pages they share
+  int pages = s.n_pages, used;                         // the pages that are shared, and by how many blocks
   if (a.dealt == BY_TILE) {
     const int t0 = r / a.tokens * a.tokens, t1 = t0 + a.tokens < s.rows ? t0 + a.tokens : s.rows;
     int lo, hi;
     tile_pages(a, s, t0, t1, lo, hi);
     pages = hi - lo + 1;
     used = tile_shares(a, pages);
-    if (used == 1) return;
-  } else if (a.dealt == EVENLY) {
-    used = even_shares(a, s.n_pages);
-    place = seq * a.most;
-    if (used == 1) return;                             // written by its block
   } else {
-    const Span mine = span_of(a, lane < a.n_seq ? lane : a.n_seq - 1);
-    const Shares sh = shares_of(a, mine);
-    used = sh.of(s.n_pages);
-    if (used == 1) return;
-    for (int i = lane; i < seq; i += WAVE) place += sh.of(i < WAVE ? mine.n_pages : span_of(a, i).n_pages);
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) place += __shfl_xor(place, o, WAVE);
+    used = even_shares(a, pages);
   }
+  if (used == 1) return;                               // written by its block
   const int row = s.row0 + r;
-  const size_t step = a.dealt == BY_TILE ? (size_t)PART_ROW : (size_t)a.max_q * a.n_heads * PART_ROW;
-  const float* base = a.part + (a.dealt == BY_TILE ? ((size_t)row * a.n_heads + h) * a.most : ((size_t)place * a.max_q + r) * a.n_heads + h) * PART_ROW;
+  const float* base = a.part + ((size_t)row * a.n_heads + h) * a.most * PART_ROW;
   const int per = (pages + used - 1) / used;
   const int filled = (pages + per - 1) / per;          // shares that were given pages
   float M = -INFINITY;
-  for (int i = lane; i < filled; i += WAVE) M = fmaxf(M, base[i * step + HD]);
+  for (int i = lane; i < filled; i += WAVE) M = fmaxf(M, base[(size_t)i * PART_ROW + HD]);
   M = wave_max(M);
   constexpr int NE = (HD + WAVE - 1) / WAVE;
   float L = 0.f, acc[NE];
@@ -661,7 +585,7 @@ __global__ __launch_bounds__(WAVE) void attn_combine_kernel(AttnQ8 a) {
     float mm[8], ll[8], v[8][NE];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const float* p = base + (i0 + i < filled ? i0 + i : filled - 1) * step;
+      const float* p = base + (size_t)(i0 + i < filled ? i0 + i : filled - 1) * PART_ROW;
       mm[i] = p[HD];
       ll[i] = p[HD + 1];
 #pragma unroll
@@ -944,7 +868,7 @@ __global__ __launch_bounds__(PF_WAVES* WAVE) __attribute__((amdgpu_waves_per_eu(
 // What a launch looks like, from sizes that the host knows.  max_q_len and max_kv_len bound the sequences' rows and
 // lengths (a recorded launch passes the context's).
 struct Plan {
-  int tiled, nc, chunks, dealt, least, fill, most, tokens;
+  int tiled, nc, chunks, dealt, fill, most, tokens;
   long long items;                           // shares of sequences that there may be
 };
 static Plan plan_of(int n_seq, int n_heads, int n_kv, int max_q_len, int max_kv_len, int window) {
@@ -981,30 +905,26 @@ static Plan plan_of(int n_seq, int n_heads, int n_kv, int max_q_len, int max_kv_
   p.nc = cols <= 16 ? 1 : 2;
   if (p.nc > NC_MOST) p.nc = NC_MOST;
   p.chunks = (int)((cols + 16 * p.nc - 1) / (16 * p.nc));
-  // How the pages are dealt (head size 64 and 128, us): with up to a quarter of the chip's blocks evenly, each sequence
-  // to as many blocks as any (one sequence of 2,300 tokens 8.4 against 9.9 by length, 16 with drafts 18.1 against 21.3);
-  // with more of them by length, where an even deal leaves the longest to too few (32 sequences of 64 to 8,192 tokens 56.9
-  // against 63.6); and where the sequences fill the chip each to one block, unless some may be longer than 96 pages.
-  const long long blocks = (long long)n_seq * n_kv * p.chunks;
-  p.items = n_seq;
-  if (blocks <= chip / 4) {
-    const int by_wave = (pages + WAVES - 1) / WAVES, by_16 = (pages + 16 * WAVES - 1) / (16 * WAVES);
-    p.fill = (int)((chip + blocks - 1) / blocks);
-    p.most = p.fill < by_wave ? p.fill : by_wave;
-    if (p.most < by_16) p.most = by_16;
-    if (p.most < 1) p.most = 1;
-    p.dealt = p.most > 1 ? EVENLY : WHOLE;
-    p.items *= p.most;
-  } else {
-    p.least = blocks >= chip ? 16 * WAVES : WAVES;
-    p.dealt = pages + p.least / 2 >= 2 * p.least ? BY_LENGTH : WHOLE;        // the least length with two shares
-    if (p.dealt) p.items += BLOCKS / (n_kv * p.chunks);
-  }
+  // How the pages are dealt.  One block a (sequence, kv head) takes `turn` ns for every page a wave; dealing them to as many
+  // blocks as fill the chip costs a launch that joins their results, 4 us, and saves nothing of the time that the memory
+  // needs (counted at 0.7 of the bound, since lengths differ).  Dealt and whole, us: one sequence of 24 and 40 pages 8.5 and
+  // 8.0, 9.3 and 10.6 (head size 64), 9.6 and 10.0, 10.4 and 13.3 (128); 16 of 32 and 126 pages 12.1 and 10.5, 28.2 and 25.7,
+  // 18.9 and 14.8, 46.3 and 41.5; 4 of 313 to 512 pages 27 and 88; 16 of up to 64 pages with drafts 18.3 and 20.9.  However
+  // many sequences there are, one of more than 128 pages goes to up to eight blocks at least.
+  const long long pairs = (long long)n_seq * n_kv * p.chunks, turn = (400 + 7 * HD / 2) * (p.nc == 2 ? 8 : 5) / 5;
+  const int by_wave = (pages + WAVES - 1) / WAVES, by_16 = (pages + 16 * WAVES - 1) / (16 * WAVES);
+  const bool pays = by_wave * turn - pairs * pages * q8_head_bytes(HD) / 5200 * 7 / 10 > 4000;
+  p.fill = pays && pairs < chip ? (int)((chip + pairs - 1) / pairs) : 1;
+  p.most = p.fill < by_wave ? p.fill : by_wave;
+  if (pages > 128 && p.most < by_16) p.most = by_16 < 8 ? by_16 : (p.most < 8 ? 8 : p.most);       // (blocks that a short sequence has no use for)
+  if (p.most < 1) p.most = 1;
+  p.dealt = p.most > 1 ? EVENLY : WHOLE;
+  p.items = (long long)n_seq * p.most;
   return p;
 }
 
-static long long scratch_of(const Plan& p, int n_rows, int n_heads, int max_q_len) {
-  return p.dealt == WHOLE ? 0 : (p.tiled ? (long long)n_rows * p.most : p.items * max_q_len) * n_heads * PART_ROW;
+static long long scratch_of(const Plan& p, int n_rows, int n_heads) {
+  return p.dealt == WHOLE ? 0 : (long long)n_rows * p.most * n_heads * PART_ROW;
 }
 
 extern "C" int dlgo_attention_q8_head_dim() { return HD; }
@@ -1013,7 +933,7 @@ extern "C" int dlgo_attention_q8_head_dim() { return HD; }
 extern "C" long long dlgo_attention_q8_scratch(int n_rows, int n_seq, int n_heads, int n_kv, int max_q_len, int max_kv_len, int window) {
   if (n_rows <= 0 || n_seq <= 0 || n_kv <= 0 || n_heads < n_kv || max_q_len <= 0 || max_kv_len <= 0) return 0;
   const Plan p = plan_of(n_seq, n_heads, n_kv, max_q_len, max_kv_len, window);
-  return scratch_of(p, n_rows, n_heads, max_q_len);
+  return scratch_of(p, n_rows, n_heads);
 }
 
 template <int NC, bool FUSED>
@@ -1048,9 +968,9 @@ extern "C" const char* dlgo_attention_q8(const void* q, int ldq, void* out, int 
   const Plan p = plan_of(n_seq, n_heads, n_kv, max_q_len, max_kv_len, window);
   AttnQ8 a = {(const bf16_t*)q, (bf16_t*)out, part, cu_q, start_pos, slots, page_table, (const uint8_t*)cache, page_stride, ldq, ldo, n_rows, n_seq,
               n_heads, n_kv, n_heads / n_kv, n_slots, max_pages, n_pages, window > 0 ? window : 0,
-              (scale < 0 ? -scale : scale) * 1.44269504088896341f, scale < 0 ? 0x80008000u : 0u, max_q_len, n_kv * p.chunks, p.dealt, p.least, p.fill, p.most, p.tokens, cos_t, sin_t, table_rows};
+              (scale < 0 ? -scale : scale) * 1.44269504088896341f, scale < 0 ? 0x80008000u : 0u, max_q_len, n_kv * p.chunks, p.dealt, p.fill, p.most, p.tokens, cos_t, sin_t, table_rows};
   hipError_t e = hipSuccess;
-  const long long need = scratch_of(p, n_rows, n_heads, max_q_len), blocks = p.items * (p.tiled ? (long long)n_kv * p.most : a.shared);
+  const long long need = scratch_of(p, n_rows, n_heads), blocks = p.items * (p.tiled ? (long long)n_kv * p.most : a.shared);
   DLGO_REQUIRE(need == 0 || (part && part_elems >= need && ((uintptr_t)part & 15) == 0), "attention_q8: scratch of %lld floats is needed, %lld given", need, part ? part_elems : 0ll);
   DLGO_REQUIRE(blocks < (1ll << 31), "attention_q8: too many rows at once");
   if (p.tiled) {

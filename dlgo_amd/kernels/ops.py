@@ -868,12 +868,13 @@ def _attention_q8_scratch(head_dim, rows, n_seq, n_heads, n_kv, max_q_len, max_k
 
 def attention_q8_fuses_rotation(head_dim: int, group: int, max_q_len: int, rot_width: int, interleaved: bool, n_seq: int, n_kv: int) -> bool:
     """True if attention_q8() should rotate the queries and take in the new keys and values itself for such a step: one row a
-    sequence, heads rotated whole, in halves, of sizes in steps of 32 up to 128, up to 16 of them a kv head; and at most one
-    (sequence, kv head) pair for every second compute unit, so that a launch costs more than the rotation repeated in every
-    wave (8 layers of 32 heads over 8 behind 1,024 tokens, ms a step fused and not, head size 64 at 8, 16 and 24 sequences: 0.529
-    and 0.563, 0.567 and 0.601, 0.682 and 0.676; 128: 1.183 and 1.187, 1.272 and 1.278, 1.334 and 1.278)."""
+    sequence, heads rotated whole, in halves, of sizes in steps of 32 up to 128, up to 16 of them a kv head; and so few
+    (sequence, kv head) pairs that a launch costs more than the rotation repeated in every wave: two a compute unit with heads of
+    up to 64, one with 128 (8 layers of 32 heads over 8 behind 1,024 tokens, ms a step fused and not: head size 64, 8, 32 and 64
+    sequences 0.529 and 0.561, 0.632 and 0.644, 0.719 and 0.734; 128, 16, 32 and 48 sequences 1.210 and 1.234, 1.269 and 1.267,
+    1.427 and 1.381)."""
     return (max_q_len == 1 and head_dim % 32 == 0 and head_dim <= 128 and rot_width == head_dim and not interleaved and group <= 16
-            and 2 * n_seq * n_kv <= compute_units())
+            and n_seq * n_kv * max(head_dim, 64) <= 128 * compute_units())
 
 
 def attention_q8(q: torch.Tensor, out: torch.Tensor, n_heads: int, n_kv: int, head_dim: int, cu_q: torch.Tensor,

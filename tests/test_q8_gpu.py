@@ -396,7 +396,7 @@ def test_attention_with_a_table_for_far_longer_sequences():
             s.check(s.attend(q, bound_len=bound), q)
 
 
-UNEQUAL = [   # sequences, rows each, the longest pasts, H, KV, hd, window: pages dealt by length, in groups of 64 sequences
+UNEQUAL = [   # sequences, rows each, the longest pasts, H, KV, hd, window
     (150, (1,), [1300, 40], 3, 1, 16, 0),
     (130, (0, 1, 2), [700, 650, 5], 6, 1, 32, 90),
     (20, (1,), [9000, 300], 32, 8, 64, 0),
@@ -612,7 +612,7 @@ def test_single_tokens_rotated_and_stored_on_the_way(past, H, KV, hd, window):
     finite and what lies around them as there."""
     ops = _ops()
     n = len(past)
-    assert ops.attention_q8_fuses_rotation(hd, H // KV, 1, hd, False, n, KV) == (2 * n * KV <= ops.compute_units())
+    assert ops.attention_q8_fuses_rotation(hd, H // KV, 1, hd, False, n, KV) == (n * KV * max(hd, 64) <= 128 * ops.compute_units())
     s = Step([1] * n, past, H, KV, hd, units=2, unit=1, seed=hd, pad_cols=8)
     s.fill()
     cos, sin = tables(max(past) + 1, hd)
