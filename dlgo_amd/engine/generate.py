@@ -209,6 +209,37 @@ def fill_drafts(drafts: List[List[int]], room: Sequence[int], last: Sequence[int
     return [x + [t] * (r - len(x)) for x, r, t in zip(drafts, room, last)]
 
 
+def _decide(engine, sampler, live, logits, drafts):
+    """(kept, tokens): how many of each entry's drafts are kept, and the token after them.  A request that asks for no
+    drafts and draws its tokens has them drawn by the sampler, as in a batch where nobody drafts: the verification sums
+    a row in another precision, so the same number may fall on a neighbour there.  (Greedy, both take the lowest index
+    of the maximum.)"""
+    def verify(logits, which):
+        uniforms = [[uniform(live[i].seed ^ _VERIFY_STREAM, live[i].index, len(live[i].tokens) + j) for j in range(len(drafts[i]))]
+                    + [uniform(live[i].seed, live[i].index, len(live[i].tokens))] for i in which]
+        return sampler.verify(logits, [drafts[i] for i in which], [live[i].config.sampler for i in which], uniforms)
+
+    drawn = [i for i, l in enumerate(live) if l.config.lookup_drafts <= 0 and not l.config.sampler.greedy]
+    if not drawn:
+        return verify(logits, range(len(live)))
+    first, n = [], 0
+    for x in drafts:
+        first.append(n)
+        n += len(x) + 1
+    kept, tokens = [0] * len(live), [0] * len(live)
+    verified = [i for i in range(len(live)) if i not in set(drawn)]
+    if verified:
+        rows = [r for i in verified for r in range(first[i], first[i] + len(drafts[i]) + 1)]
+        for i, k, tok in zip(verified, *verify(_take(engine, logits, rows), verified)):
+            kept[i], tokens[i] = k, tok
+    _, wait = sampler.choose_async(_take(engine, logits, [first[i] for i in drawn]), [live[i].config.sampler for i in drawn],
+                                   [uniform(live[i].seed, live[i].index, len(live[i].tokens)) for i in drawn],
+                                   keys=[live[i].slot for i in drawn])
+    for i, tok in zip(drawn, wait()):
+        tokens[i] = tok
+    return kept, tokens
+
+
 def _drafted_batch(engine, sampler, live, logits, prompts, results, stats, on_token) -> None:
     """The decode loop of a batch in which some requests draft tokens.  `logits` has one row per entry of `live`: those
     after the prompts.  drafts[i] are the tokens whose logits, and the place after them, the rows of entry i are."""
@@ -234,9 +265,7 @@ def _drafted_batch(engine, sampler, live, logits, prompts, results, stats, on_to
             live, drafts = [live[r] for r in keep], [drafts[r] for r in keep]
         if not live:
             return
-        uniforms = [[uniform(l.seed ^ _VERIFY_STREAM, l.index, len(l.tokens) + j) for j in range(len(x))]
-                    + [uniform(l.seed, l.index, len(l.tokens))] for l, x in zip(live, drafts)]
-        kept, tokens = sampler.verify(logits, drafts, [l.config.sampler for l in live], uniforms)
+        kept, tokens = _decide(engine, sampler, live, logits, drafts)
         now = time.perf_counter()
         stats.step_ms.append((now - last) * 1000.0)
         last = now

@@ -106,7 +106,9 @@ def with_lookup_drafts(n: int) -> Option:
     """Draft up to n tokens a step by looking up where the text's last tokens stood before, and have one step of the model
     verify them all: fewer steps where the text repeats itself, the same distribution of tokens.  Takes greedy decoding
     or a temperature alone (no top-k, top-p, min-p or repetition penalty); a batch that holds a request with one of those
-    drafts nothing."""
+    drafts nothing.  Which tokens a seed gives a request that drafts at a temperature depends on what was drafted, and that
+    on its batch; requests that ask for no drafts get the tokens that they get anywhere, but a batch in which somebody
+    drafts waits for the host at every step."""
     def opt(c: GenerateConfig) -> None:
         c.lookup_drafts = int(n)
     return opt
