@@ -313,8 +313,9 @@ class Cache:
         last = (new_len - 1) // PAGE
         return [i for i in range(first, last + 1) if i not in held]
 
-    def can_reserve(self, wants: Sequence[Tuple[int, int]]) -> Optional[str]:
-        """None if every (slot, new_len) fits, else the reason."""
+    def can_reserve(self, wants: Sequence[Tuple[int, int]], settled: bool = False) -> Optional[str]:
+        """None if every (slot, new_len) fits, else the reason.  settled: as if settle() had been called for these slots;
+        nothing is given back yet, so that a refused step leaves its slots as they were, drafts to be rewound among it."""
         for slot, new_len in wants:
             self._check_live(slot)
             if new_len > self.max_ctx:
@@ -322,12 +323,15 @@ class Cache:
         for gi, g in enumerate(self.groups):
             # a windowed group: a sequence never holds more than its window and the longest piece of a step, because
             # each piece gives back what no later token sees before the next piece asks for more
+            free = g.pool.n_free
             if g.spec.window is None:
                 need = sum(len(self.pages_wanted(s, n, gi)) for s, n in wants)
             else:
-                need = sum(min(len(self.pages_wanted(s, n, gi)), max(0, g.pages_per_seq - len(self._held[s][gi]))) for s, n in wants)
-            if need > g.pool.n_free:
-                return f"cache full: the step needs {need} more pages of {PAGE} tokens, {g.pool.n_free} of {g.pool.n_pages} are free"
+                gone = {s: len(self._unseen(s, gi, int(self.lengths[s]))) if settled else 0 for s, _ in wants}
+                free += sum(gone.values())
+                need = sum(min(len(self.pages_wanted(s, n, gi)), max(0, g.pages_per_seq - len(self._held[s][gi]) + gone[s])) for s, n in wants)
+            if need > free:
+                return f"cache full: the step needs {need} more pages of {PAGE} tokens, {free} of {g.pool.n_pages} are free"
         return None
 
     def page_demand(self, n_tokens: int) -> Tuple[int, ...]:
@@ -370,13 +374,17 @@ class Cache:
                 self._check_live(slot)
                 self._give_unseen(slot, int(self.lengths[slot]))
 
+    def _unseen(self, slot: int, group: int, length: int) -> List[int]:
+        """Page indices that the slot holds in `group` and no token at a position >= length sees."""
+        first = self.groups[group].first_needed_page(length)
+        return [i for i in self._held[slot][group] if i < first]
+
     def _give_unseen(self, slot: int, length: int) -> None:
         for gi, g in enumerate(self.groups):
             if g.spec.window is None:
                 continue
-            first = g.first_needed_page(length)
             held = self._held[slot][gi]
-            gone = [i for i in held if i < first]
+            gone = self._unseen(slot, gi, length)
             if gone:
                 g.pool.give([held.pop(i) for i in gone])
                 g.table_host[slot, gone] = -1

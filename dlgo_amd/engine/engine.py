@@ -345,10 +345,10 @@ class Engine:
         if tokens.min() < 0 or tokens.max() >= self.vocab:
             bad = int(tokens[(tokens < 0) | (tokens >= self.vocab)][0])
             raise EngineError(f"step: token id {bad} is outside the vocabulary of {self.vocab}")
-        self.cache.settle(seen)
-        why = self.cache.can_reserve([(e.slot, s + n) for e, s, n in zip(entries, starts, q_lens)])
+        why = self.cache.can_reserve([(e.slot, s + n) for e, s, n in zip(entries, starts, q_lens)], settled=True)
         if why:
             raise EngineError(f"step: {why}")
+        self.cache.settle(seen)                 # from here on the step is not refused any more
         self.steps_run += 1
 
         if (sink is None
@@ -527,10 +527,10 @@ class Engine:
             if (starts + 1 > self.max_ctx).any():
                 raise EngineError(f"decode: a sequence would exceed the context of {self.max_ctx}")
             if needs_pages:
-                self.cache.settle(slots)
-                why = self.cache.can_reserve([(int(s), int(st) + 1) for s, st in zip(slot_arr, starts)])
+                why = self.cache.can_reserve([(int(s), int(st) + 1) for s, st in zip(slot_arr, starts)], settled=True)
                 if why:
                     raise EngineError(f"decode: {why}")
+                self.cache.settle(slots)
         if b > self.graph_max_batch:
             # more sequences than the fixed arrays of a recorded step hold: in runs of that many (the call as a whole is
             # checked by now), into a buffer of this call
