@@ -17,7 +17,8 @@ through a handful of calls, so its decisions can be tested with stand-ins:
     engine:  open(n) -> slots, close(slots), step(entries) -> logits rows (the prompts),
              decode(slots, ids) -> logits rows (one token each; ids as the sampler left them on the device),
              max_ctx, free_slots(), free_pages() and page_demand(n_tokens) (per storage group of the cache);
-             where drafts are wanted also rewind(slot, length) (and can_rewind)
+             where drafts are wanted also rewind(slot, length) (and can_rewind, and logits_rows: the rows of logits that
+             a step of drafts may have)
     sampler: start(keys), choose_async(logits, configs, uniforms, keys=) -> (ids on the device, wait() -> ids on the host);
              where drafts are wanted also verify(logits, drafts, configs, uniforms) -> (kept counts, tokens)
 
@@ -201,6 +202,19 @@ _VERIFY_STREAM = 0x5DEECE66D
 FILL_ROWS = 64
 
 
+#: drafts of a sequence that a verification takes at most, whatever a request asks for
+MOST_DRAFTS = 1024
+
+
+def draft_room(engine, live) -> List[int]:
+    """How many tokens each request may draft for the next step: as many as it asks for, but no more than may still be
+    emitted (a step may emit a token more than it drafts), nor than its share of the rows of logits that the engine keeps
+    room for (logits_rows: a step of drafts has a row for every draft and one more a sequence)."""
+    share = getattr(engine, "logits_rows", MOST_DRAFTS) // max(1, len(live)) - 1
+    return [max(0, min(l.config.lookup_drafts, l.config.max_tokens - len(l.tokens) - 1, engine.max_ctx - 2 - l.pos, share, MOST_DRAFTS))
+            for l in live]
+
+
 def fill_drafts(drafts: List[List[int]], room: Sequence[int], last: Sequence[int]) -> List[List[int]]:
     """Where some sequence has drafts and the step stays small, every sequence that may draft brings as many as it has
     room for, so that steps keep one shape, which the engine records: the last token again, refused unless it is right."""
@@ -297,8 +311,7 @@ def _drafted_batch(engine, sampler, live, logits, prompts, results, stats, on_to
         live = still
         if not live:
             return
-        # a step may emit a token more than it drafts: no more drafts than what may still be emitted allows
-        room = [min(l.config.lookup_drafts, l.config.max_tokens - len(l.tokens) - 1, engine.max_ctx - 2 - l.pos) for l in live]
+        room = draft_room(engine, live)
         drafts = fill_drafts([texts[l.index].propose(r) for l, r in zip(live, room)], room, [l.tokens[-1] for l in live])
         logits = engine.step([Entry(l.slot, [l.tokens[-1]] + x, list(range(len(x) + 1)), undecided=len(x)) for l, x in zip(live, drafts)])
         stats.steps += 1

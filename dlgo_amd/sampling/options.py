@@ -103,8 +103,8 @@ def with_ignore_eos(on: bool = True) -> Option:
 
 
 def with_lookup_drafts(n: int) -> Option:
-    """Draft up to n tokens a step by looking up where the text's last tokens stood before, and have one step of the model
-    verify them all: fewer steps where the text repeats itself, the same distribution of tokens.  Takes greedy decoding
+    """Draft up to n tokens a step (1,024 at most, and no more than the engine's logits_rows for a whole batch) by looking up
+    where the text's last tokens stood before, and have one step of the model verify them all: fewer steps where the text repeats itself, the same distribution of tokens.  Takes greedy decoding
     or a temperature alone (no top-k, top-p, min-p or repetition penalty); a batch that holds a request with one of those
     drafts nothing.  Which tokens a seed gives a request that drafts at a temperature depends on what was drafted, and that
     on its batch; requests that ask for no drafts get the tokens that they get anywhere, but a batch in which somebody
