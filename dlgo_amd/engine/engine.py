@@ -97,7 +97,7 @@ class Engine:
                  prompt_graph_limit: int = 32, prompt_graph_bytes: int = 1 << 30, cache_dtype: Optional[str] = None):
         """`model` holds its weights already (see from_folder / from_random).  use_graphs: steps of single tokens are
         recorded per batch size, and per shape steps of fresh prompts of up to prompt_graph_max_tokens rows and steps of
-        drafts (as many for each sequence, every row wanted) of up to graph_max_batch rows (the
+        drafts (Entry.undecided; as many for each sequence, every row wanted) of up to graph_max_batch rows (the
         prompt_graph_limit most recently used shapes are kept, as long as the logits they keep stay within
         prompt_graph_bytes), the second time a size or shape is seen.  cache_dtype: None keeps keys and values in the run
         dtype, "e4m3" in 8 bits (bfloat16 runs only: half the cache's bytes, each element rounded to 4 significant bits)."""
@@ -366,16 +366,7 @@ class Engine:
         seq_of = np.repeat(np.arange(len(entries)), q_lens)
         pos_all = np.concatenate([np.arange(s, s + n) for s, n in zip(starts, q_lens)])
 
-        # Fresh prompts of a shape seen before, and as many drafts behind each sequence (a step that wants every row):
-        # the launches depend on the rows per sequence and the wanted places only (and on a bound of the lengths: the
-        # context's, for drafts), so the step is recorded the second time the shape comes and replayed from then on.
-        shape = None
-        fresh = not any(starts)
-        # (a recording keeps its logits: not where those would be more than 64 MB)
-        if (self.use_graphs and sink is None and n_out and total <= min(self.max_step_tokens, self.prompt_graph_max_tokens)
-                and n_out * self.vocab * 4 <= min(64 << 20, self.prompt_graph_bytes)
-                and (fresh or (n_out == total <= self.graph_max_batch and len(set(q_lens)) == 1))):
-            shape = (tuple(q_lens), tuple(wanted), fresh)
+        shape = self._shape_to_record(entries, q_lens, starts, wanted) if sink is None else None
         out = None
         if sink is None and (shape is None or shape not in self._prompt_graphs):
             out = torch.empty((n_out, self.vocab), dtype=torch.float32, device=self.device)
@@ -409,6 +400,20 @@ class Engine:
             for i, sl, q in zip(seqs, slots, piece_q):
                 self.cache.advance(int(sl), int(q), starts[i] + q_lens[i] - entries[i].undecided)
         return out
+
+    def _shape_to_record(self, entries: Sequence[Entry], q_lens: Sequence[int], starts: Sequence[int], wanted: Sequence[int]):
+        """The key of a step that is recorded the second time it comes and replayed from then on, None for any other.  Fresh
+        prompts, and drafts (some undecided) of equal number behind each sequence with every row wanted: the launches
+        depend on the rows per sequence and the wanted places only (and on a bound of the lengths: the context's, for drafts).
+        Other steps behind a past are sized by their own lengths."""
+        total, n_out = sum(q_lens), len(wanted)
+        if not self.use_graphs or not n_out or total > min(self.max_step_tokens, self.prompt_graph_max_tokens):
+            return None
+        if n_out * self.vocab * 4 > min(64 << 20, self.prompt_graph_bytes):         # a recording keeps its logits
+            return None
+        fresh = not any(starts)
+        drafts = n_out == total <= self.graph_max_batch and len(set(q_lens)) == 1 and all(e.undecided for e in entries)
+        return (tuple(q_lens), tuple(wanted), fresh) if fresh or drafts else None
 
     def _run_piece(self, ctx: StepContext, arrays: Dict[str, torch.Tensor], sel: np.ndarray, out: Optional[torch.Tensor],
                    sink: Optional[Callable[[int, torch.Tensor], None]]) -> None:
