@@ -98,7 +98,7 @@ class Engine:
         """`model` holds its weights already (see from_folder / from_random).  use_graphs: steps of single tokens are
         recorded per batch size, and per shape steps of fresh prompts of up to prompt_graph_max_tokens rows and steps of
         drafts (Entry.undecided; as many for each sequence, every row wanted) of up to graph_max_batch rows (the
-        prompt_graph_limit most recently used shapes are kept, as long as the logits they keep stay within
+        prompt_graph_limit most recently used shapes of either kind are kept, as long as the logits they keep stay within
         prompt_graph_bytes), the second time a size or shape is seen.  cache_dtype: None keeps keys and values in the run
         dtype, "e4m3" in 8 bits (bfloat16 runs only: half the cache's bytes, each element rounded to 4 significant bits)."""
         _require_gpu()
@@ -415,6 +415,18 @@ class Engine:
         drafts = n_out == total <= self.graph_max_batch and len(set(q_lens)) == 1 and all(e.undecided for e in entries)
         return (tuple(q_lens), tuple(wanted), fresh) if fresh or drafts else None
 
+    def _drop_recordings(self) -> None:
+        """Called after a recording was kept: the least recently used ones go where there are too many of the newest one's
+        kind (prompts and drafts have prompt_graph_limit places each) or all their logits take too much."""
+        kept = self._prompt_graphs
+        kind = next(reversed(kept))[2]
+        same = [k for k in kept if k[2] == kind]
+        for k in same[:max(0, len(same) - self.prompt_graph_limit)]:
+            kept.pop(k)
+        held = sum(g.logits.numel() * 4 for g in kept.values())
+        while len(kept) > 1 and held > self.prompt_graph_bytes:
+            held -= kept.pop(next(iter(kept))).logits.numel() * 4
+
     def _run_piece(self, ctx: StepContext, arrays: Dict[str, torch.Tensor], sel: np.ndarray, out: Optional[torch.Tensor],
                    sink: Optional[Callable[[int, torch.Tensor], None]]) -> None:
         """The model on the rows of one piece of a step, and the logits of the wanted rows that lie in it (output rows
@@ -476,10 +488,7 @@ class Engine:
             if was_enabled:
                 gc.enable()
         self._prompt_graphs[shape] = _PromptGraph(graph, meta, logits, ctx)
-        # the least recently used recordings go when there are too many or their logits take too much
-        held = lambda: sum(p.logits.numel() * 4 for p in self._prompt_graphs.values())
-        while len(self._prompt_graphs) > 1 and (len(self._prompt_graphs) > self.prompt_graph_limit or held() > self.prompt_graph_bytes):
-            self._prompt_graphs.pop(next(iter(self._prompt_graphs)))
+        self._drop_recordings()
         graph.replay()
         return logits.clone()
 

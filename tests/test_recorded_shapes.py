@@ -1,4 +1,6 @@
-"""Which steps are recorded (no GPU: the engine's own bookkeeping)."""
+"""Which steps are recorded, and which recordings stay (no GPU: the engine's own bookkeeping)."""
+from types import SimpleNamespace
+
 import pytest
 
 from dlgo_amd.engine.engine import Engine, Entry
@@ -40,3 +42,31 @@ def test_other_steps_behind_a_past_are_not(undecided):
     comes again, and the step is sized by its own lengths."""
     assert shape(engine(), [5, 5], [7, 90], undecided) is None
     assert shape(engine(), [5], [7], undecided and undecided[1:]) is None
+
+
+def keep(eng, key, mb=0.1):
+    eng._prompt_graphs.pop(key, None)
+    eng._prompt_graphs[key] = SimpleNamespace(logits=SimpleNamespace(numel=lambda: int(mb * (1 << 20)) // 4))
+    eng._drop_recordings()
+
+
+def test_shapes_of_drafts_do_not_push_out_prompts():
+    """Three places for either kind: ten shapes of drafts (a batch that thins out) leave the prompts' recordings."""
+    eng = engine()
+    prompts = [((n,), (n - 1,), True) for n in (5, 6, 7)]
+    drafts = [((n,), tuple(range(n)), False) for n in range(2, 12)]
+    for k in prompts + drafts:
+        keep(eng, k)
+    assert list(eng._prompt_graphs) == prompts + drafts[-3:]
+    keep(eng, ((9,), (8,), True))
+    assert list(eng._prompt_graphs) == prompts[1:] + drafts[-3:] + [((9,), (8,), True)]
+
+
+def test_recordings_that_keep_too_much_go_whatever_they_are():
+    eng = engine()
+    keys = [((5,), (4,), True), ((2,), (0, 1), False), ((6,), (5,), True), ((3,), (0, 1, 2), False)]
+    for k in keys:
+        keep(eng, k, 0.4)
+    assert list(eng._prompt_graphs) == keys[-2:]             # 1 MB in all
+    keep(eng, keys[0], 5)
+    assert list(eng._prompt_graphs) == keys[:1]              # the newest one stays
