@@ -59,7 +59,8 @@ class Stats:
     batches: int = 0
     steps: int = 0
     step_ms: List[float] = field(default_factory=list)
-    drafted_tokens: int = 0        # drafts that were verified, and those of them that were kept
+    drafted_tokens: int = 0        # drafts that were looked up and verified, and those of them that were kept (what only
+                                   # fills a step up to one shape counts as neither)
     kept_drafts: int = 0
 
     @property
@@ -264,6 +265,7 @@ def _drafted_batch(engine, sampler, live, logits, prompts, results, stats, on_to
 
     texts = {l.index: LookupDrafts(prompts[l.index]) for l in live}
     drafts: List[List[int]] = [[] for _ in live]
+    found = [0] * len(live)                            # how many of them were looked up; the others fill the step up
     last = time.perf_counter()
     while live:
         keep = []
@@ -276,7 +278,7 @@ def _drafted_batch(engine, sampler, live, logits, prompts, results, stats, on_to
                 keep.append(row)
         if len(keep) != len(live):
             logits = _take(engine, logits, keep) if keep else None
-            live, drafts = [live[r] for r in keep], [drafts[r] for r in keep]
+            live, drafts, found = [live[r] for r in keep], [drafts[r] for r in keep], [found[r] for r in keep]
         if not live:
             return
         kept, tokens = _decide(engine, sampler, live, logits, drafts)
@@ -284,9 +286,9 @@ def _drafted_batch(engine, sampler, live, logits, prompts, results, stats, on_to
         stats.step_ms.append((now - last) * 1000.0)
         last = now
         still = []
-        for l, x, k, tok in zip(live, drafts, kept, tokens):
-            stats.drafted_tokens += len(x)
-            stats.kept_drafts += k
+        for l, x, k, tok, own in zip(live, drafts, kept, tokens, found):
+            stats.drafted_tokens += own
+            stats.kept_drafts += min(k, own)
             if k < len(x):
                 engine.rewind(l.slot, l.pos + k)       # the refused drafts were given to the sequence: not any more
             new = list(x[:k]) + [int(tok)]
@@ -312,7 +314,9 @@ def _drafted_batch(engine, sampler, live, logits, prompts, results, stats, on_to
         if not live:
             return
         room = draft_room(engine, live)
-        drafts = fill_drafts([texts[l.index].propose(r) for l, r in zip(live, room)], room, [l.tokens[-1] for l in live])
+        drafts = [texts[l.index].propose(r) for l, r in zip(live, room)]
+        found = [len(x) for x in drafts]
+        drafts = fill_drafts(drafts, room, [l.tokens[-1] for l in live])
         logits = engine.step([Entry(l.slot, [l.tokens[-1]] + x, list(range(len(x) + 1)), undecided=len(x)) for l, x in zip(live, drafts)])
         stats.steps += 1
 

@@ -52,3 +52,15 @@ def test_a_batch_where_only_a_drawn_request_is_left():
     results, _ = generate(DraftEngine(max_ctx=64), samp, [[5, 6, 7, 5, 6, 7]] * 2, [plain, drafting])
     assert results[0].tokens == [1000 + int(1e6 * uniform(4, 0, j)) for j in range(12)] and len(results[1].tokens) == 3
     assert all(xs for xs, _ in samp.verified)
+
+
+def test_what_fills_a_step_up_is_not_counted_as_drafts():
+    """Two requests, one whose text repeats three tokens and one whose text never does: the second one's rows fill the step."""
+    say = lambda slot, n: 5 + n % 3 if slot == 0 else 100 + n                    # noqa: E731
+    draft = GenerateConfig(max_tokens=20, sampler=SamplerConfig(temperature=0), lookup_drafts=5)
+    samp = DraftSampler(say)
+    _, stats = generate(DraftEngine(max_ctx=64), samp, [[5, 6, 7] * 3, [1, 2, 3, 4]], [draft, draft])
+    rows = sum(len(x) for xs, _ in samp.verified for x in xs)
+    looked_up = sum(min(3, len(xs[0])) for xs, _ in samp.verified if len(xs) == 2)       # the text behind the last match is three tokens long
+    assert any(len(xs) == 2 and len(xs[1]) == 5 for xs, _ in samp.verified)
+    assert stats.drafted_tokens == looked_up < rows and 0 < stats.kept_drafts <= looked_up
