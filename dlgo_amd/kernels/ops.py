@@ -739,6 +739,14 @@ def _same_device(name: str, first: torch.Tensor, *others: Optional[torch.Tensor]
 _BF16, _F32, _I32, _U8 = torch.bfloat16, torch.float32, torch.int32, torch.uint8
 
 
+def _given_scratch(name: str, t: torch.Tensor, dtype: torch.dtype, beside: torch.Tensor) -> torch.Tensor:
+    """A caller's scratch buffer: its elements lie in a row in memory (the kernels count on as many as it has), beside the others."""
+    _need(t, f"{name}: scratch", dtype, 1)
+    if not t.is_contiguous() or t.device != beside.device:
+        raise KernelError(f"{name}: scratch must lie in a row in memory on {beside.device} (strides {t.stride()}, {t.device})")
+    return t
+
+
 def _current_device() -> int:
     return _raw_device() if _raw_device is not None else torch.cuda.current_device()
 
@@ -933,7 +941,7 @@ def attention_q8(q: torch.Tensor, out: torch.Tensor, n_heads: int, n_kv: int, he
     part = None
     if need:
         part = scratch(need) if scratch is not None else torch.empty(need, dtype=torch.float32, device=q.device)
-        _need(part, "attention_q8: scratch", torch.float32, 1)
+        _given_scratch("attention_q8", part, torch.float32, q)
     _check(lib.dlgo_attention_q8(_ptr(q), _rows(q, "attention_q8: query rows"), _ptr(out), _rows(out, "attention_q8: output"), t, n_seq,
                                  n_heads, n_kv, head_dim, _ptr(cu_q), _ptr(start_pos), _ptr(slots), _ptr(page_table),
                                  n_slots, max_pages, _ptr(cache), ctypes.c_longlong(page_stride), n_pages,
@@ -1079,7 +1087,7 @@ def verify_drafts(logits: torch.Tensor, draft_tokens: torch.Tensor, cu_drafts: t
     lib = _lib("verify")
     need = _verify_drafts_scratch(n, d, v, model_drafts)
     work = scratch(need) if scratch is not None else torch.empty(need, dtype=torch.uint8, device=logits.device)
-    _need(work, "verify_drafts: scratch", torch.uint8, 1)
+    _given_scratch("verify_drafts", work, torch.uint8, logits)
     _check(lib.dlgo_verify_drafts(_ptr(logits), ctypes.c_longlong(_rows(logits, "verify_drafts: logits")), _ptr(draft_tokens),
                                   _ptr(draft_logits if model_drafts else None),
                                   ctypes.c_longlong(_rows(draft_logits, "verify_drafts: draft logits") if model_drafts else 0),
