@@ -878,8 +878,8 @@ static Plan plan_of(int n_seq, int n_heads, int n_kv, int max_q_len, int max_kv_
   const long long cols = (long long)max_q_len * group;
   int pages = (max_kv_len + Q8_PAGE - 1) / Q8_PAGE;
   if (window > 0) {
-    const int seen = (window + max_q_len + Q8_PAGE - 2) / Q8_PAGE + 1;
-    if (seen < pages) pages = seen;
+    const long long seen = ((long long)window + max_q_len + Q8_PAGE - 2) / Q8_PAGE + 1;      // a window may be any int
+    if (seen < pages) pages = (int)seen;
   }
   const int chip = 512;
   // Up to 32 columns: with 20 and 32 of them the tiles are slower for heads of 64 (16 sequences with up to 24 columns behind

@@ -936,7 +936,8 @@ def attention_q8(q: torch.Tensor, out: torch.Tensor, n_heads: int, n_kv: int, he
         return out
     max_q_len = min(int(max_q_len), t)
     max_kv_len = max(1, min(int(max_kv_len), max_pages * PAGE))
-    need = _attention_q8_scratch(head_dim, t, n_seq, n_heads, n_kv, max_q_len, max_kv_len, int(window))
+    window = min(int(window), 2 ** 31 - 1)          # (no sequence is longer)
+    need = _attention_q8_scratch(head_dim, t, n_seq, n_heads, n_kv, max_q_len, max_kv_len, window)
     lib = _lib("attention_q8", (("HEAD_DIM", head_dim),))
     part = None
     if need:
@@ -945,7 +946,7 @@ def attention_q8(q: torch.Tensor, out: torch.Tensor, n_heads: int, n_kv: int, he
     _check(lib.dlgo_attention_q8(_ptr(q), _rows(q, "attention_q8: query rows"), _ptr(out), _rows(out, "attention_q8: output"), t, n_seq,
                                  n_heads, n_kv, head_dim, _ptr(cu_q), _ptr(start_pos), _ptr(slots), _ptr(page_table),
                                  n_slots, max_pages, _ptr(cache), ctypes.c_longlong(page_stride), n_pages,
-                                 max_q_len, max_kv_len, int(window), ctypes.c_float(scale), _ptr(part),
+                                 max_q_len, max_kv_len, window, ctypes.c_float(scale), _ptr(part),
                                  ctypes.c_longlong(part.numel() if part is not None else 0), _ptr(cos), _ptr(sin),
                                  0 if cos is None else cos.shape[0], _stream()))
     return out
