@@ -218,8 +218,9 @@ def variant(module: str, dtype=None, defines: Defines = ()) -> Variant:
     return module, tuple(defines)
 
 
-#: head sizes compiled ahead by build_all(): those of the test configurations and of the benchmark shapes
-DEFAULT_HEAD_DIMS = (16, 32, 48, 64, 80, 128, 256)
+#: head sizes compiled ahead by build_all(): those of the test configurations and of the benchmark shapes, and 96, the one
+#: size whose pieces of 16 fill two loads of the 8-bit attention unevenly in the kernel that rotates by itself
+DEFAULT_HEAD_DIMS = (16, 32, 48, 64, 80, 96, 128, 256)
 
 
 def all_variants(head_dims: Sequence[int] = DEFAULT_HEAD_DIMS) -> list[Variant]:
