@@ -13,6 +13,13 @@ from .options import SamplerConfig
 RECENT = 64   # tokens the repetition penalty looks back on (models/llm/generate.go:361-365)
 
 
+def _below_one(uniforms: Sequence[Sequence[float]], n: int) -> np.ndarray:
+    """n numbers of [0, 1) as float32 of [0, 1): what would round up to one (1 - 2^-25 and more) is the largest below it, for
+    a draft that is sure of its token (u * 1 < 1) and a draw (the first sum above u times the whole) need u < 1."""
+    u = np.fromiter((v for row in uniforms for v in row), dtype=np.float32, count=n)
+    return np.minimum(u, np.float32(1 - 2.0 ** -24))
+
+
 class Sampler:
     #: the tokens a request has been given are also kept on the device (start(), and keys= of the choose calls), so
     #: that the repetition penalty does not need them back from the host before the next choice
@@ -178,7 +185,7 @@ class Sampler:
         parts = (np.fromiter((t for x in drafts for t in x), dtype=np.int32, count=d),
                  np.concatenate([[0], np.cumsum(lens)]).astype(np.int32),
                  np.array([max(0.0, c.temperature) for c in configs], dtype=np.float32).view(np.int32),
-                 np.fromiter((v for u in uniforms for v in u), dtype=np.float32, count=n + d).view(np.int32))
+                 _below_one(uniforms, n + d).view(np.int32))
         offs, total = [], 0
         for a in parts:
             offs.append(total)
