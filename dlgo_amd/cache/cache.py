@@ -96,7 +96,8 @@ class KVGroup:
         if self.q8:          # bytes: each head's keys, values and powers of two lie together
             if spec.head_dim % 16 or spec.head_dim > 256:
                 raise CacheError(f"cache: e4m3 keys and values take head sizes in steps of 16, up to 256, not {spec.head_dim}")
-            self.unit_elems = spec.kv_heads * 2 * PAGE * (spec.head_dim + 1)
+            from ..kernels.ops import q8_page_bytes
+            self.unit_elems = q8_page_bytes(spec.kv_heads, spec.head_dim)
             dtype = torch.uint8
         else:
             self.unit_elems = 2 * spec.kv_heads * PAGE * spec.head_dim     # keys then values of one unit in a page

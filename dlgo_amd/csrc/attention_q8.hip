@@ -78,8 +78,9 @@ __device__ __forceinline__ Span span_of(const AttnQ8& a, int seq) {
   return s;
 }
 
-// EVENLY: the blocks that share a sequence of n pages: enough to fill the chip, but not more than leave each wave a page, and
-// so many that a wave has at most 16 pages.
+// EVENLY: the blocks that share a sequence of n pages: enough to fill the chip, but not more than leave each wave a page, and so
+// many that a wave has at most 16 pages, as far as the launch has them (`most`; else a wave has n / (4 * most) pages: 64 of
+// a sequence of 2,048 pages among so many others that each goes to eight blocks at most).
 __device__ __forceinline__ int even_shares(const AttnQ8& a, int n) {
   const int by_wave = (n + WAVES - 1) / WAVES, by_16 = (n + 16 * WAVES - 1) / (16 * WAVES);
   int s = a.fill < by_wave ? a.fill : by_wave;
@@ -112,7 +113,8 @@ __device__ __forceinline__ float max_16(float x) {
   return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
 // Sums are rescaled only where a maximum has grown by more than 2^8 over the one that they stand for: a probability is
-// then at most 2^8, which costs float32 and bfloat16 none of their places.
+// then at most 2^8, which costs float32 and bfloat16 none of their places.  (It takes 2^8 of their range: values from
+// 2^119 on may overflow the sums.)
 __device__ __forceinline__ bool has_grown(float mx, float m, float scale_log2e) { return (mx - m) * scale_log2e > 8.f; }
 
 typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2_t;
@@ -619,9 +621,10 @@ __global__ __launch_bounds__(WAVE) void attn_combine_kernel(AttnQ8 a) {
 // for 8 prompts of 64 to 2,048 tokens behind up to 2,048, 32 heads of 128 over 8).  Operands asked for four steps ahead: 366;
 // sums rescaled only where a maximum has grown and maxima exchanged without LDS: 349; pages two ahead: 319 to 334, 660
 // TFLOP/s.  A lone prompt of 2,048 tokens (heads of 64, 38.8 us) waits for its last tiles, 32 pages of 1.1 us one after the
-// other.  Measured and not kept: 64 columns a wave (78 us), eight waves with 256 columns (50 to 59), two teams of waves on
-// alternate pages (45), the scores of the next page beside this one's softmax (-3% for heads of 64, spills for 128), wave
-// priorities raised around the products or the softmax (337 to 360 against 336).
+// other.  Measured on that prompt and not kept: 64 columns a wave (78 us), eight waves with 256 columns (50 to 59: there are too
+// few tiles of that size; with many tiles it was not measured), two teams of waves on alternate pages (45), the scores of the
+// next page beside this one's softmax (-3%, and spills with heads of 128).  On the eight prompts: wave priorities raised
+// around the products or the softmax (337 to 360 against 336).
 #define PF_WAVES 4
 #define PF_EU (HD <= 128 ? 2 : 1)           // waves a SIMD that the registers are to allow
 #define DT ((HD + 31) / 32)                 // tiles of 32 elements of the result

@@ -8,8 +8,9 @@
 // number).  What comes out is then distributed as the target's own tokens would be.  T = 0: a draft is kept if it is the
 // row's maximum (the lowest index among equals), and the token after is the maximum.
 //
-// Everything that decides is held in 64 bits: an index of a vocabulary of 128,256 flat weights owns 2^-17 of the sum, and
-// a sum in 32 bits would put about one draw in a hundred beside its neighbour.  computerex/dlgo draws from float32
+// Everything that decides is held in 64 bits, a logit's weight right to 1.1 * 10^-12 of itself (exp2_neg, 40 bits): an index of
+// a vocabulary of 128,256 flat weights owns 2^-17 of the sum, and a sum in 32 bits would put about one draw in a hundred
+// beside its neighbour.  computerex/dlgo draws from float32
 // probabilities in one pass over a sorted row (ops/sampling.go); it verifies no drafts.
 //
 // Every row of logits is read once, by blocks of 4,096 elements that each leave a maximum, its index and a sum; the row that

@@ -721,7 +721,7 @@ def _q8_cache(name: str, cache: torch.Tensor, page_stride: int, n_kv: int, head_
         _need(cache, f"{name}: cache", torch.uint8, 1)
     if head_dim % 16 or not 16 <= head_dim <= Q8_MAX_HEAD_DIM:
         raise KernelError(f"{name}: the 8-bit cache takes head sizes in steps of 16, up to {Q8_MAX_HEAD_DIM}, not {head_dim}")
-    page, size = n_kv * 2 * PAGE * (head_dim + 1), cache.numel()
+    page, size = q8_page_bytes(n_kv, head_dim), cache.numel()
     if page_stride < page or size < page or not cache.is_contiguous():
         raise KernelError(f"{name}: a cache of {size} bytes with pages {page_stride} bytes apart does not hold pages of {page} bytes")
     return min((size - page) // page_stride + 1, 2 ** 31 - 1)
@@ -898,7 +898,8 @@ def attention_q8(q: torch.Tensor, out: torch.Tensor, n_heads: int, n_kv: int, he
     of them.  Rows behind the last sequence's are left as they were.  max_q_len and max_kv_len (host) bound the
     rows a sequence brings and the tokens it holds afterwards: a captured step passes what it allows for; rows and
     tokens beyond the bounds are left out or slow, never out of bounds.  scratch(n) returns a float32 buffer of at least n elements for what
-    several blocks find of a row (allocated here if not given).  A row that finds no page at all is zeros.
+    several blocks find of a row (allocated here if not given).  A row that finds no page at all is zeros.  A query head that
+    is not finite gives NaN, or zeros where all its scores are -inf.
 
     rotation = (cos, sin), where attention_q8_fuses_rotation() says so (one row a sequence): q holds the step's unrotated
     [q | k | v] rows, the kernel rotates the queries and does what rope_kv_q8() does for the keys and values, to the bit."""
