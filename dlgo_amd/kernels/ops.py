@@ -72,6 +72,14 @@ def _rows(t: torch.Tensor, name: str) -> int:
     return strides[0] if t.shape[0] > 1 else max(strides[0], t.shape[1])
 
 
+def _rows32(t: torch.Tensor, name: str) -> int:
+    """_rows() for a kernel that takes the stride as a 32-bit number."""
+    stride = _rows(t, name)
+    if stride >= 2 ** 31:
+        raise KernelError(f"{name}: rows {stride} elements apart, at most {2 ** 31 - 1} are taken")
+    return stride
+
+
 def _check(err: Optional[bytes]) -> None:
     if err:
         raise KernelError(err.decode())
@@ -839,7 +847,7 @@ def rope_kv_q8(qkv: torch.Tensor, q_out: torch.Tensor, n_heads: int, n_kv: int, 
         if unsummed.rows != t or unsummed.cols < (n_heads + (2 * n_kv if write_kv else 0)) * head_dim or unsummed.scratch.get_device() != qkv.get_device():
             raise KernelError(f"rope_kv_q8: unsummed rows [{unsummed.rows}, {unsummed.cols}] do not fit {t} rows of qkv")
         part = (_ptr(unsummed.scratch), unsummed.runs, ctypes.c_longlong(unsummed.rows * unsummed.cols), unsummed.cols)
-    _check(_lib("kv_q8").dlgo_rope_kv_q8(_ptr(qkv), _rows(qkv, "rope_kv_q8: qkv rows"), _ptr(q_out), _rows(q_out, "rope_kv_q8: query rows"),
+    _check(_lib("kv_q8").dlgo_rope_kv_q8(_ptr(qkv), _rows32(qkv, "rope_kv_q8: qkv rows"), _ptr(q_out), _rows32(q_out, "rope_kv_q8: query rows"),
                                          t, n_heads, n_kv, head_dim, rot, int(interleaved), _ptr(cos), _ptr(sin), table_rows,
                                          _ptr(positions), _ptr(tok_seq), _ptr(slots), n_seq, _ptr(page_table), n_slots, max_pages,
                                          _ptr(cache), ctypes.c_longlong(page_stride), n_pages, int(write_kv), *part, _stream()))
@@ -944,7 +952,7 @@ def attention_q8(q: torch.Tensor, out: torch.Tensor, n_heads: int, n_kv: int, he
     if need:
         part = scratch(need) if scratch is not None else torch.empty(need, dtype=torch.float32, device=q.device)
         _given_scratch("attention_q8", part, torch.float32, q)
-    _check(lib.dlgo_attention_q8(_ptr(q), _rows(q, "attention_q8: query rows"), _ptr(out), _rows(out, "attention_q8: output"), t, n_seq,
+    _check(lib.dlgo_attention_q8(_ptr(q), _rows32(q, "attention_q8: query rows"), _ptr(out), _rows32(out, "attention_q8: output"), t, n_seq,
                                  n_heads, n_kv, head_dim, _ptr(cu_q), _ptr(start_pos), _ptr(slots), _ptr(page_table),
                                  n_slots, max_pages, _ptr(cache), ctypes.c_longlong(page_stride), n_pages,
                                  max_q_len, max_kv_len, window, ctypes.c_float(scale), _ptr(part),

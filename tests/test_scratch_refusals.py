@@ -1,4 +1,4 @@
-"""Scratch buffers that the 8-bit attention and the verification must not be given."""
+"""Scratch buffers and rows that the operators of the 8-bit cache and of drafts must not be given."""
 import pytest
 import torch
 
@@ -48,3 +48,12 @@ def test_the_calls_refuse_them():
             s.attend(q, scratch=lambda n: make(n, torch.float32))
         with pytest.raises(ops.KernelError, match="verify_drafts: scratch"):
             ops.verify_drafts(**v, scratch=lambda n: make(n, torch.uint8))
+
+
+def test_rows_further_apart_than_a_32_bit_number_says():
+    """The kernels take a row's stride in 32 bits: its low ones alone would name other rows."""
+    far = torch.empty_strided((2, 256), (2 ** 32 + 256, 1), dtype=torch.bfloat16, device="meta")
+    near = torch.empty_strided((2, 256), (2 ** 31 - 8, 1), dtype=torch.bfloat16, device="meta")
+    assert ops._rows(far, "x") == 2 ** 32 + 256 and ops._rows32(near, "x") == 2 ** 31 - 8
+    with pytest.raises(ops.KernelError, match="x: rows 4294967552 elements apart"):
+        ops._rows32(far, "x")
