@@ -242,7 +242,7 @@ def _decide(engine, sampler, live, logits, drafts):
         first.append(n)
         n += len(x) + 1
     kept, tokens = [0] * len(live), [0] * len(live)
-    verified = [i for i in range(len(live)) if i not in set(drawn)]
+    verified = sorted(set(range(len(live))) - set(drawn))
     if verified:
         rows = [r for i in verified for r in range(first[i], first[i] + len(drafts[i]) + 1)]
         for i, k, tok in zip(verified, *verify(_take(engine, logits, rows), verified)):
